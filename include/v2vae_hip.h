@@ -334,6 +334,93 @@ int64_t v2vae_ws_offset_gmoments(const v2vae_problem* p);
 int64_t v2vae_ws_offset_xhat_float(const v2vae_problem* p);
 int64_t v2vae_ws_offset_xhat_remainder(const v2vae_problem* p);
 
+/* ------------------------------------------------------------------------------------------------------------------------
+ * Dense layers and distillation: what a network equaliser is made of, and how it is trained without pilots from the soft
+ * decisions of a fitted VAE.  (The reference's network equalisers, lib/torch_components.py:122-222 and
+ * lib/real_equalization.py:232-431, are pilot-trained torch modules on stock operators; these entry points have no counterpart.)
+ * One element type per call for every activation, weight and gradient; sums, soft-max statistics and pre-activations are
+ * float.  Matrices are row-major with unit stride inside a row; the ld_* fields give the elements between rows, any alignment.
+ * Inputs are only read, so their rows may overlap (windows that slide over one sequence) or coincide; outputs are contiguous.
+ * float32 products run as six bf16 products of three-piece splits: float32 accuracy for finite operands up to 3.38e38, while an
+ * infinite operand gives NaN (not inf) in the outputs it enters.  rows = 0 is allowed everywhere: outputs without rows are
+ * left alone, parameter gradients are set to zero. */
+#define V2VAE_F32 0
+#define V2VAE_BF16 1
+#define V2VAE_F16 2
+
+#define V2VAE_ACT_NONE 0
+#define V2VAE_ACT_RELU 1
+#define V2VAE_ACT_SILU 2 /* z / (1 + exp(-z)) */
+#define V2VAE_ACT_GELU 3 /* z Phi(z), Phi the normal distribution function (erf form) */
+#define V2VAE_ACT_TANH 4
+
+typedef struct v2vae_dense {
+    int32_t dtype;      /* V2VAE_F32, V2VAE_BF16 or V2VAE_F16 */
+    int32_t activation; /* V2VAE_ACT_* */
+    int64_t rows;       /* rows of x and y, 0 ... 2^30 */
+    int64_t in;         /* columns of x and of the weights, 1 ... 2^30 */
+    int64_t out;        /* rows of the weights, columns of y, 1 ... 2^30 */
+    int64_t ld_x;       /* >= 0, as all of these */
+    int64_t ld_w;       /* gated block: of the gate weights */
+    int64_t ld_w2;      /* gated block: of the up weights; otherwise ignored */
+    int64_t ld_res;     /* where a residual is passed */
+    int64_t ld_dy;      /* backward */
+} v2vae_dense;
+
+/* y [rows][out] = act(x w^T + bias) + residual.  w [out][in]; bias [out] and residual may be NULL.  z (float [rows][out], may be
+ * NULL) receives the pre-activations that v2vae_linear_bwd needs when there is an activation.  ws: v2vae_linear_workspace_bytes
+ * (d, 0) bytes, may be NULL if that is 0. */
+int v2vae_linear_fwd(const v2vae_dense* d, const void* x, const void* w, const void* bias, const void* residual, void* y,
+                     float* z, void* ws, void* stream);
+
+/* Gradients given dy [rows][out]: with dz = dy act'(z), dx [rows][in] = dz w, dw [out][in] = dz^T x, dbias [out] = column sums
+ * of dz (the residual's gradient is dy itself).  Each output may be NULL; z may be NULL without an activation.  dz is rounded to
+ * the element type once before the two products (dbias is summed before that).  ws: v2vae_linear_workspace_bytes(d, 1). */
+int v2vae_linear_bwd(const v2vae_dense* d, const void* x, const void* w, const float* z, const void* dy, void* dx, void* dw,
+                     void* dbias, void* ws, void* stream);
+size_t v2vae_linear_workspace_bytes(const v2vae_dense* d, int backward); /* 0 also for an invalid description */
+
+/* Gated feed-forward block: h [rows][out] = act(x wg^T + bg) * (x wu^T + bu); wg, wu [out][in], biases may be NULL.  gu (float
+ * [2][rows][out], may be NULL) receives both pre-activations for v2vae_gated_bwd. */
+int v2vae_gated_fwd(const v2vae_dense* d, const void* x, const void* wg, const void* wu, const void* bg, const void* bu,
+                    void* h, float* gu, void* ws, void* stream);
+
+/* Gradients given dh [rows][out] (row stride ld_dy): dg = dh u act'(g), du = dh act(g); dx = dg wg + du wu, dwg = dg^T x,
+ * dwu = du^T x, dbg / dbu the column sums.  Each output may be NULL.  ws: v2vae_gated_workspace_bytes(d, 1). */
+int v2vae_gated_bwd(const v2vae_dense* d, const void* x, const void* wg, const void* wu, const float* gu, const void* dh,
+                    void* dx, void* dwg, void* dwu, void* dbg, void* dbu, void* ws, void* stream);
+size_t v2vae_gated_workspace_bytes(const v2vae_dense* d, int backward);
+
+/* Distillation from a teacher's top logits.  Row r: student logits z[vocab], teacher logits t[k] at classes index[k].  An entry
+ * with index < 0 or t = -inf is absent; a class named twice counts twice.  With p = softmax over the present entries of t / T and
+ * log q = log softmax(z / T):  loss = T^2 sum_j p_j (log p_j - log q[index_j]);  d loss / d z = T (q - sum_{index_j = v} p_j).
+ * A row without present entries has loss 0 and gradient 0.  A student logit of -inf has q = 0 (loss +inf if its p is not 0).
+ * An index >= vocab makes the row's loss and gradient NaN (nothing is read there). */
+typedef struct v2vae_distill {
+    int32_t dtype;         /* of the student's logits and their gradient: V2VAE_F32, V2VAE_BF16, V2VAE_F16 */
+    int32_t teacher_dtype; /* of the teacher's logits */
+    int32_t index_bits;    /* 32 or 64 */
+    int32_t k;             /* teacher entries per row, 1 ... V2VAE_DISTILL_MAX_K */
+    int64_t rows;          /* 0 ... 2^30 */
+    int64_t vocab;         /* 1 ... 2^30 */
+    int64_t ld_logits;     /* >= vocab */
+    int64_t ld_teacher;    /* >= k */
+    int64_t ld_index;      /* >= k */
+    float temperature;     /* > 0, finite */
+    int32_t reserved;      /* must be 0 */
+} v2vae_distill;
+#define V2VAE_DISTILL_MAX_K 1024
+
+/* loss [rows]; stats (float [rows][2], may be NULL) receives the row maximum and the sum of exponentials for the backward call. */
+int v2vae_distill_fwd(const v2vae_distill* d, const void* logits, const void* teacher, const void* index, float* loss,
+                      float* stats, void* stream);
+/* grad [rows][vocab] (contiguous) = weight[r] * d loss_r / d z. */
+int v2vae_distill_bwd(const v2vae_distill* d, const void* logits, const void* teacher, const void* index, const float* stats,
+                      const float* weight, void* grad, void* stream);
+/* Both in one pass over the logits, the rows' weights known beforehand: loss (unweighted) and grad (weighted). */
+int v2vae_distill_step(const v2vae_distill* d, const void* logits, const void* teacher, const void* index, const float* weight,
+                       float* loss, void* grad, void* stream);
+
 const char* v2vae_version(void);
 
 /* Text of the last HIP error seen by the calling thread inside this library (debugging aid). */

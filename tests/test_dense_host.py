@@ -1,0 +1,120 @@
+"""Refusals of the dense layers and the distillation loss, on the host: nothing is launched."""
+import ctypes as C
+
+import pytest
+import torch
+
+from volterra_vae_amd import _lib, dense_ops
+
+P = 0x1000  # an aligned address that no call may reach
+
+
+def dense(**over):
+    d = dict(dtype=0, activation=0, rows=64, in_=50, out=30, ld_x=50, ld_w=50, ld_w2=50, ld_res=30, ld_dy=30)
+    d.update(over)
+    return _lib.Dense(*[d[f] for f, _ in _lib.Dense._fields_])
+
+
+def distill(**over):
+    d = dict(dtype=0, teacher_dtype=0, index_bits=32, k=4, rows=8, vocab=100, ld_logits=100, ld_teacher=4, ld_index=4, temperature=1.0, reserved=0)
+    d.update(over)
+    return _lib.Distill(*[d[f] for f, _ in _lib.Distill._fields_])
+
+
+BAD = [dict(dtype=3), dict(dtype=-1), dict(activation=5), dict(activation=-1), dict(rows=-1), dict(in_=0), dict(out=0), dict(ld_x=-1),
+       dict(ld_w=-4)]
+
+
+@pytest.mark.parametrize("over", BAD, ids=str)
+def test_bad_descriptions_are_refused(over):
+    d = dense(**over)
+    assert _lib.lib.v2vae_linear_fwd(d, P, P, None, None, P, None, P, None) == _lib.EINVAL
+    assert _lib.lib.v2vae_linear_bwd(d, P, P, P, P, P, P, P, P, None) == _lib.EINVAL
+    assert _lib.lib.v2vae_gated_fwd(d, P, P, P, None, None, P, None, P, None) == _lib.EINVAL
+    assert _lib.lib.v2vae_gated_bwd(d, P, P, P, P, P, P, P, P, P, P, P, None) == _lib.EINVAL
+    for back in (0, 1):
+        assert _lib.lib.v2vae_linear_workspace_bytes(d, back) == 0 and _lib.lib.v2vae_gated_workspace_bytes(d, back) == 0
+
+
+def test_sizes_beyond_the_limits_are_refused():
+    for over in (dict(rows=(1 << 30) + 1), dict(in_=(1 << 30) + 1), dict(out=1 << 31), dict(rows=1 << 30, out=1 << 30)):
+        assert _lib.lib.v2vae_linear_fwd(dense(**over), P, P, None, None, P, None, P, None) == _lib.ESIZE
+        assert _lib.lib.v2vae_linear_workspace_bytes(dense(**over), 1) == 0
+    assert _lib.lib.v2vae_distill_fwd(distill(k=1025, ld_teacher=1025, ld_index=1025), P, P, P, P, None, None) == _lib.ESIZE
+    assert _lib.lib.v2vae_distill_fwd(distill(rows=(1 << 30) + 1), P, P, P, P, None, None) == _lib.ESIZE
+
+
+def test_missing_and_misaligned_pointers_are_refused():
+    f = _lib.lib.v2vae_linear_fwd
+    d = dense()
+    for bad in ((None, P, None, None, P, None), (P, None, None, None, P, None), (P, P, None, None, None, None), (P + 2, P, None, None, P, None),
+                (P, P, P + 1, None, P, None), (P, P, None, P + 2, P, None), (P, P, None, None, P, P + 2)):
+        assert f(d, *bad, P, None) == _lib.EINVAL
+    assert f(d, P, P, None, None, P, None, P + 8, None) == _lib.EINVAL          # the workspace is 256-byte aligned
+    assert f(dense(ld_res=-1), P, P, None, P, P, None, P, None) == _lib.EINVAL
+    b = _lib.lib.v2vae_linear_bwd
+    assert b(d, P, P, None, None, P, P, P, P, None) == _lib.EINVAL               # no dy
+    assert b(d, P, P, None, P, P, P, P, None, None) == _lib.EINVAL               # no workspace
+    assert b(dense(activation=2), P, P, None, P, P, P, P, P, None) == _lib.EINVAL  # an activation without its pre-activations
+    assert b(d, None, P, None, P, P, P, P, P, None) == _lib.EINVAL               # dw without x
+    assert b(dense(ld_dy=-1), P, P, None, P, P, P, P, P, None) == _lib.EINVAL
+    g = _lib.lib.v2vae_gated_bwd
+    assert g(d, P, P, P, None, P, P, P, P, P, P, P, None) == _lib.EINVAL
+    assert g(d, P, P, None, P, P, P, P, P, P, P, P, None) == _lib.EINVAL
+    assert _lib.lib.v2vae_gated_fwd(d, P, P, None, None, None, P, None, P, None) == _lib.EINVAL
+    assert f(None, P, P, None, None, P, None, P, None) == _lib.EINVAL
+
+
+@pytest.mark.parametrize("over", [dict(dtype=3), dict(teacher_dtype=-1), dict(index_bits=16), dict(k=0), dict(rows=-1), dict(vocab=0),
+                                  dict(ld_logits=99), dict(ld_teacher=3), dict(ld_index=3), dict(temperature=0.0),
+                                  dict(temperature=-1.0), dict(temperature=float("nan")), dict(temperature=float("inf")),
+                                  dict(temperature=1e-44), dict(reserved=1)], ids=str)
+def test_bad_distillations_are_refused(over):
+    d = distill(**over)
+    assert _lib.lib.v2vae_distill_fwd(d, P, P, P, P, None, None) == _lib.EINVAL
+    assert _lib.lib.v2vae_distill_bwd(d, P, P, P, P, P, P, None) == _lib.EINVAL
+    assert _lib.lib.v2vae_distill_step(d, P, P, P, P, P, P, None) == _lib.EINVAL
+
+
+def test_distillation_pointers():
+    d = distill()
+    assert _lib.lib.v2vae_distill_fwd(d, P, P, P, None, None, None) == _lib.EINVAL
+    assert _lib.lib.v2vae_distill_bwd(d, P, P, P, None, P, P, None) == _lib.EINVAL   # statistics of the forward pass
+    assert _lib.lib.v2vae_distill_step(d, P, P, P, None, P, P, None) == _lib.EINVAL
+    assert _lib.lib.v2vae_distill_fwd(d, P + 2, P, P, P, None, None) == _lib.EINVAL
+    assert _lib.lib.v2vae_distill_fwd(distill(index_bits=64), P, P, P + 4, P, None, None) == _lib.EINVAL
+
+
+def test_no_rows_launch_nothing():
+    assert _lib.lib.v2vae_linear_fwd(dense(rows=0), None, None, None, None, None, None, None, None) == _lib.OK
+    assert _lib.lib.v2vae_gated_fwd(dense(rows=0), None, None, None, None, None, None, None, None, None) == _lib.OK
+    assert _lib.lib.v2vae_distill_step(distill(rows=0), None, None, None, None, None, None, None) == _lib.OK
+
+
+def test_the_python_layer_refuses_what_is_not_on_a_gpu_or_not_a_tensor():
+    x, w = torch.zeros(4, 3), torch.zeros(5, 3)
+    with pytest.raises(RuntimeError, match="no CPU implementation"):
+        dense_ops.linear(x, w)
+    with pytest.raises(RuntimeError, match="no CPU implementation"):
+        dense_ops.gated_linear(x, w, w)
+    with pytest.raises(RuntimeError, match="no CPU implementation"):
+        dense_ops.topk_distillation(x, torch.zeros(4, 2), torch.zeros(4, 2, dtype=torch.int32))
+    with pytest.raises(ValueError, match="none of none, relu, silu, gelu, tanh"):
+        dense_ops.linear(x, w, activation="selu")
+    with pytest.raises(ValueError, match="x must be a tensor"):
+        dense_ops.linear([[1.0]], w)
+    with pytest.raises(ValueError, match="rows"):
+        dense_ops.linear(x, w, residual=torch.zeros(3, 5))
+
+
+def test_structures_match_the_header():
+    """Field names and order of the two argument blocks, and their sizes under the C rules."""
+    import os
+    import re
+    text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "v2vae_hip.h")).read()
+    text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
+    for name, struct in (("v2vae_dense", _lib.Dense), ("v2vae_distill", _lib.Distill)):
+        body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), text, flags=re.S).group(1)
+        declared = re.findall(r"(\w+)\s+(\w+);", body)
+        kinds = {"int32_t": C.c_int32, "int64_t": C.c_int64, "float": C.c_float}
+        assert [(n.rstrip("_"), t) for n, t in struct._fields_] == [(n, kinds[k]) for k, n in declared]

@@ -1,0 +1,358 @@
+"""Dense layers (linear, gated block) against their formulas in float64: sizes, strides, alignment, activations, gradients.
+
+Tolerances.  With S2 = sqrt(sum_k x_k^2 w_k^2), a float32 sum of n rounded steps over such terms is off by about sqrt(n) 2^-24 S2
+(independent roundings of partial sums no larger than a few S2); 8 of these are allowed.  A float32 product in three bf16 pieces
+takes 6 accumulations per 16 terms and drops less than 2^-24 of a term, which the same bound covers.  A value rounded to the
+tensors' type is off by at most u = finfo.eps / 2 of itself: once for a result, and once per term (at random, 6 sigma of u S2) for
+dz, which is rounded before the two gradient products.  Activations have slopes up to 1.13 and second derivatives up to 1 and
+are computed to a few units of 2^-24; the factor 4 on the float32 part of the gradients covers them.
+Below finfo.tiny the step of a type is fixed at tiny * eps (2^-24 in float16), so a rounding is off by up to tiny * eps / 2 there
+(2^-25), however small the value: once for a result, and for dz times sqrt(sum of squares) of what it is multiplied with.
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+EPS32 = 2.0 ** -24
+
+
+def dev():
+    return torch.device("cuda", 0)
+
+
+def u(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def normal(gen, *shape, scale=1.0, dtype=torch.float32):
+    return (torch.randn(shape, generator=gen, dtype=torch.float64) * scale).to(dtype).to(dev())
+
+
+def act64(kind, z):
+    return {"none": lambda v: v, "relu": torch.relu, "silu": torch.nn.functional.silu, "gelu": torch.nn.functional.gelu,
+            "tanh": torch.tanh}[kind](z)
+
+
+def s2(a, b):
+    """sqrt(a^2 b^2) over the contraction of a [M, K] with b [N, K]."""
+    return ((a * a) @ (b * b).t()).sqrt()
+
+
+def floor_of(dtype):
+    f = torch.finfo(dtype)
+    return f.tiny * f.eps / 2
+
+
+def near(got, ref, bound, what):
+    assert got.shape == ref.shape, what
+    bound = bound + floor_of(got.dtype)
+    err = (got.double() - ref).abs()
+    worst = float((err - bound).max()) if err.numel() else -1.0
+    assert torch.isfinite(got).all() and worst <= 0, f"{what}: error {float(err.max()):.3g} beyond its bound by {worst:.3g}"
+
+
+def steps(k, dtype):
+    return (6 * k / 16 if dtype == torch.float32 else k / 16) + 16
+
+
+def laid_out(t, how):
+    """The same values with another row stride / start: rows `pad` elements apart further, starting `lead` elements in."""
+    lead, pad = {"plain": (0, 0), "odd": (1, 3), "wide": (8, 8)}[how]
+    if how == "plain" or t.dim() != 2:
+        return t
+    buf = torch.full((lead + t.shape[0] * (t.shape[1] + pad) + 8,), 7.0, dtype=t.dtype, device=t.device)
+    v = torch.as_strided(buf, t.shape, (t.shape[1] + pad, 1), lead)
+    v.copy_(t)
+    return v
+
+
+SHAPES = [(1, 1, 1), (1, 4096, 72), (2, 129, 5), (5, 64, 130), (11, 50, 64), (16, 1000, 33), (17, 50, 64), (64, 64, 64), (65, 8, 1),
+          (129, 130, 67), (200, 257, 300), (1000, 96, 33), (40, 3000, 24), (257, 512, 384), (2500, 48, 40), (3, 8200, 9)]
+
+
+def linear_case(m, k, n, dtype, act, bias, residual, how, seed):
+    gen = torch.Generator().manual_seed(seed)
+    x = laid_out(normal(gen, m, k, dtype=dtype), how)
+    w = laid_out(normal(gen, n, k, scale=k ** -0.5, dtype=dtype), how)
+    b = normal(gen, n, scale=0.5, dtype=dtype) if bias else None
+    r = laid_out(normal(gen, m, n, dtype=dtype), how) if residual else None
+    dy = laid_out(normal(gen, m, n, dtype=dtype), how)
+    return x, w, b, r, dy
+
+
+def check_linear(x, w, b, r, dy, act, got_y, grads, dtype):
+    X, W, D = x.detach().double(), w.detach().double(), dy.double()
+    leaves = [X.requires_grad_(True), W.requires_grad_(True)]
+    B = b.detach().double().requires_grad_(True) if b is not None else None
+    z = X @ W.t() + (B if B is not None else 0.0)
+    y = act64(act, z)
+    y = y + r.detach().double() if r is not None else y
+    ref = torch.autograd.grad(y, leaves + ([B] if B is not None else []), D)
+    X, W, y, z = X.detach(), W.detach(), y.detach(), z.detach()
+    k, (m, n) = X.shape[1], y.shape
+    f32 = 8 * EPS32 * steps(k, dtype) ** 0.5
+    extra = (B.detach().abs() if B is not None else 0.0) + (r.detach().double().abs() if r is not None else 0.0)
+    near(got_y, y, u(dtype) * y.abs() + 1.13 * f32 * s2(X, W) + 16 * EPS32 * (extra + y.abs()) + 1e-30, "y")
+    if grads is None:
+        return
+    rounded, low = (0.0, 0.0) if act == "none" else (6 * u(dtype), 6 * floor_of(dtype))
+    dx, dw, db = grads
+    zerr = (1 + s2(X, W).max())   # an error of z of f32 * S2 enters act' with a second derivative up to 1
+    near(dx, ref[0], u(dtype) * ref[0].abs() + (rounded + 32 * EPS32 * (steps(n, dtype) ** 0.5 + steps(k, dtype) ** 0.5) * zerr)
+         * s2(D, W.t()) + low * s2(torch.ones_like(D), W.t()) + 1e-30, "dx")
+    near(dw, ref[1], u(dtype) * ref[1].abs() + (rounded + 32 * EPS32 * (steps(m, dtype) ** 0.5 + steps(k, dtype) ** 0.5) * zerr)
+         * s2(D.t(), X.t()) + low * s2(torch.ones_like(D).t(), X.t()) + 1e-30, "dw")
+    if db is not None:
+        near(db, ref[2], u(dtype) * ref[2].abs() + 32 * EPS32 * (m ** 0.5 + steps(k, dtype) ** 0.5) * zerr
+             * (D * D).sum(0).sqrt() + 1e-30, "db")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_linear_matches_its_formula(shape, dtype):
+    from volterra_vae_amd.dense_ops import linear_backward, linear_forward
+    m, k, n = shape
+    seed = m * 7 + k * 3 + n
+    kinds = ["none", "silu", "gelu", "tanh", "silu"]
+    for i, how in enumerate(["plain", "odd", "wide"]):
+        act = kinds[(seed + i) % 5]
+        x, w, b, r, dy = linear_case(m, k, n, dtype, act, (seed + i) % 2 == 0, i > 0, how, seed + i)
+        y, z = linear_forward(x, w, b, residual=r, activation=act, keep=True)
+        y2, _ = linear_forward(x, w, b, residual=r, activation=act)
+        assert torch.equal(y, y2)
+        grads = linear_backward(dy, x, w, z, activation=act, need=(True, True, b is not None))
+        check_linear(x, w, b, r, dy, act, y, grads, dtype)
+        again = linear_backward(dy, x, w, z, activation=act, need=(True, True, b is not None))
+        assert all(p is None or torch.equal(p, q) for p, q in zip(grads, again))
+
+
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "tanh"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16", "f16"])
+def test_linear_through_autograd_and_leading_dimensions(dtype, act):
+    from volterra_vae_amd.dense_ops import linear
+    x, w, b, r, dy = linear_case(6 * 35, 72, 56, dtype, act, True, True, "plain", 3)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b, r)]
+    y = linear(leaves[0].view(6, 35, 72), leaves[1], leaves[2], residual=leaves[3].view(6, 35, 56), activation=act)
+    assert y.shape == (6, 35, 56)
+    y.backward(dy.view(6, 35, 56))
+    check_linear(x, w, b, r, dy, act, y.detach().view(-1, 56), [t.grad for t in leaves[:3]], dtype)
+    assert torch.equal(leaves[3].grad, dy)
+    # the registered op is the same call; a gradient that is one number for all (stride 0) is accepted
+    op = torch.ops.v2vae.linear(leaves[0], leaves[1], leaves[2], residual=leaves[3], activation=act)
+    assert torch.equal(op, y.view(-1, 56))
+    (g,) = torch.autograd.grad(op.sum(), leaves[2])
+    check_linear(x, w, b, r, torch.ones_like(dy), act, op.detach(),
+                 torch.autograd.grad(linear(leaves[0], leaves[1], leaves[2], residual=leaves[3], activation=act),
+                                     leaves[:3], torch.ones_like(dy)), dtype)
+    assert g.shape == b.shape
+
+
+def check_gated(x, wg, wu, bg, bu, dh, act, h, grads, dtype):
+    t = [v.detach().double().requires_grad_(True) if v is not None else None for v in (x, wg, wu, bg, bu)]
+    X, G, U = t[:3]
+    g = X @ G.t() + (t[3] if bg is not None else 0.0)
+    up = X @ U.t() + (t[4] if bu is not None else 0.0)
+    ref_h = act64(act, g) * up
+    D = dh.double()
+    ref = torch.autograd.grad(ref_h, [v for v in t if v is not None], D)
+    X, G, U, g, up, ref_h = (v.detach() for v in (X, G, U, g, up, ref_h))
+    k, (m, n) = X.shape[1], ref_h.shape
+    a = act64(act, g).abs()
+    bias = (0.0 if bg is None else bg.double().abs()), (0.0 if bu is None else bu.double().abs())
+    f32 = 8 * EPS32 * steps(k, dtype) ** 0.5
+    zg, zu = f32 * s2(X, G) + 16 * EPS32 * bias[0], f32 * s2(X, U) + 16 * EPS32 * bias[1]
+    near(h, ref_h, u(dtype) * ref_h.abs() + 1.13 * zg * up.abs() + zu * a + 16 * EPS32 * ref_h.abs() + 1e-30, "h")
+    if grads is None:
+        return
+    # |dg| <= 1.13 |dh u|, |du| <= |dh act(g)|; both rounded once
+    dg, du = 1.13 * D.abs() * up.abs(), D.abs() * a
+    slack = 32 * EPS32 * (1 + max(float(s2(X, G).max()), float(s2(X, U).max())))
+    e_g, e_u = D.abs() * (1 + up.abs()), D.abs() * (1 + a)       # what errors of g and u are multiplied with
+
+    def product(i, p, q, axis_steps, names):
+        terms = sum(6 * u(dtype) * s2(v, o) + 6 * floor_of(dtype) * s2(torch.ones_like(v), o) + slack * (axis_steps ** 0.5 + steps(k, dtype) ** 0.5) * s2(e, o) for v, e, o in zip(p, q, names))
+        near(grads[i], ref[i], u(dtype) * ref[i].abs() + terms + 1e-30, f"gradient {i}")
+
+    product(0, (dg, du), (e_g, e_u), steps(2 * n, dtype), (G.t(), U.t()))
+    product(1, (dg.t(),), (e_g.t(),), steps(m, dtype), (X.t(),))
+    product(2, (du.t(),), (e_u.t(),), steps(m, dtype), (X.t(),))
+    if bg is not None:
+        for i, e in ((3, e_g), (4, e_u)):
+            near(grads[i], ref[i], u(dtype) * ref[i].abs() + slack * (m ** 0.5 + steps(k, dtype) ** 0.5) * (e * e).sum(0).sqrt() + 1e-30,
+                 f"gradient {i}")
+
+
+def gated_case(m, k, n, dtype, bias, how, seed):
+    gen = torch.Generator().manual_seed(seed)
+    x = laid_out(normal(gen, m, k, dtype=dtype), how)
+    wg, wu = (laid_out(normal(gen, n, k, scale=k ** -0.5, dtype=dtype), h) for h in (how, "wide" if how == "odd" else how))
+    bg, bu = (normal(gen, n, scale=0.5, dtype=dtype) if bias else None for _ in range(2))
+    return x, wg, wu, bg, bu, laid_out(normal(gen, m, n, dtype=dtype), how)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_gated_block_matches_its_formula(shape, dtype):
+    from volterra_vae_amd.dense_ops import gated_backward, gated_forward
+    m, k, n = shape
+    for i, how in enumerate(["plain", "odd", "wide"]):
+        act = ["silu", "gelu", "tanh"][(m + i) % 3]
+        x, wg, wu, bg, bu, dh = gated_case(m, k, n, dtype, i != 1, how, m + k + n + i)
+        h, gu = gated_forward(x, wg, wu, bg, bu, activation=act, keep=True)
+        assert torch.equal(h, gated_forward(x, wg, wu, bg, bu, activation=act)[0])
+        need = (True, True, True, bg is not None, bu is not None)
+        grads = gated_backward(dh, x, wg, wu, gu, activation=act, need=need)
+        check_gated(x, wg, wu, bg, bu, dh, act, h, grads, dtype)
+        again = gated_backward(dh, x, wg, wu, gu, activation=act, need=need)
+        assert all(p is None or torch.equal(p, q) for p, q in zip(grads, again))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16", "f16"])
+def test_gated_block_through_autograd(dtype):
+    from volterra_vae_amd.dense_ops import gated_linear
+    x, wg, wu, bg, bu, dh = gated_case(150, 88, 104, dtype, True, "plain", 5)
+    leaves = [t.clone().requires_grad_(True) for t in (x, wg, wu, bg, bu)]
+    h = gated_linear(leaves[0].view(3, 50, 88), *leaves[1:], activation="gelu")
+    h.backward(dh.view(3, 50, 104))
+    check_gated(x, wg, wu, bg, bu, dh, "gelu", h.detach().view(150, 104), [t.grad for t in leaves], dtype)
+    assert torch.equal(torch.ops.v2vae.gated_linear(*leaves, activation="gelu").view(-1), h.view(-1))
+    # only one of the gradients wanted: the others are not formed and the one is the same
+    only = [t.detach().clone() for t in leaves]
+    only[2].requires_grad_(True)
+    (g,) = torch.autograd.grad(gated_linear(*only, activation="gelu"), only[2], dh)
+    assert torch.equal(g, leaves[2].grad)
+
+
+def test_gradients_agree_with_differences():
+    """Central differences of float64-accumulated losses through the float32 kernels: step h = 2^-6, truncation h^2 / 6 times the third
+    derivative along the direction (of order 1) and rounding 2^-24 / h of the values: 2e-3 of the directional derivative's scale."""
+    from volterra_vae_amd.dense_ops import gated_linear, linear
+    gen = torch.Generator().manual_seed(11)
+    x, w, b = normal(gen, 90, 40), normal(gen, 30, 40, scale=0.15), normal(gen, 30, scale=0.3)
+    wu, c = normal(gen, 30, 40, scale=0.15), normal(gen, 90, 30)
+    for f, args in ((lambda *a: linear(*a, activation="gelu"), (x, w, b)), (lambda *a: gated_linear(a[0], a[1], a[2]), (x, w, wu))):
+        for i in range(len(args)):
+            leaves = [t.clone().requires_grad_(j == i) for j, t in enumerate(args)]
+            (g,) = torch.autograd.grad(f(*leaves), leaves[i], c)
+            v = normal(gen, *args[i].shape, scale=args[i].numel() ** -0.5)
+            h = 2.0 ** -6
+            hi, lo = ([t + s * h * v if j == i else t for j, t in enumerate(args)] for s in (1, -1))
+            fd = ((f(*hi).double() - f(*lo).double()) * c.double()).sum() / (2 * h)
+            scale = float(g.double().norm() * v.double().norm())
+            assert abs(float(fd) - float((g.double() * v.double()).sum())) <= 2e-3 * scale
+
+
+def test_rows_of_an_input_may_overlap():
+    """Sliding windows of one sequence as a strided matrix, in both layouts of a product (x and its weight gradient)."""
+    from volterra_vae_amd.dense_ops import linear_backward, linear_forward
+    gen = torch.Generator().manual_seed(2)
+    for dtype in DTYPES:
+        y = normal(gen, 8 * 600 + 70, dtype=dtype)
+        for window, hop in ((50, 2), (64, 8), (25, 1)):
+            x = torch.as_strided(y, (600, window), (hop, 1), 3)
+            w, dy = normal(gen, 20, window, scale=0.2, dtype=dtype), normal(gen, 600, 20, dtype=dtype)
+            same = x.contiguous()
+            assert torch.equal(linear_forward(x, w)[0], linear_forward(same, w)[0])
+            for p, q in zip(linear_backward(dy, x, w), linear_backward(dy, same, w)):
+                assert torch.equal(p, q)
+
+
+def test_no_rows_give_empty_outputs_and_zero_parameter_gradients():
+    from volterra_vae_amd.dense_ops import gated_linear, linear
+    for dtype in DTYPES:
+        x = torch.empty((0, 12), dtype=dtype, device=dev(), requires_grad=True)
+        w, wu = (torch.randn(7, 12, device=dev()).to(dtype).requires_grad_(True) for _ in range(2))
+        b = torch.randn(7, device=dev()).to(dtype).requires_grad_(True)
+        for y, leaves in ((linear(x, w, b, activation="silu"), (x, w, b)), (linear(x, w, b), (x, w, b)),
+                          (gated_linear(x, w, wu, b, None), (x, w, wu, b))):
+            assert y.shape == (0, 7)
+            for g, leaf in zip(torch.autograd.grad(y, leaves, torch.empty_like(y)), leaves):
+                assert g.shape == leaf.shape and float(g.abs().sum()) == 0.0
+
+
+def test_what_lies_beside_the_outputs_rows_and_the_inputs_is_left_alone():
+    """NaN around strided inputs never reaches an output, and a result of few rows writes nothing behind them."""
+    from volterra_vae_amd import _lib
+    from volterra_vae_amd.dense_ops import _dense, linear_backward, linear_forward
+    gen = torch.Generator().manual_seed(4)
+    for dtype in DTYPES:
+        for m, k, n in ((3, 50, 40), (70, 50, 40), (130, 64, 72)):
+            buf = torch.full((m + 4, k + 24), float("nan"), dtype=dtype, device=dev())
+            x = buf[2:2 + m, 8:8 + k]
+            x.copy_(normal(gen, m, k, dtype=dtype))
+            wbuf = torch.full((n + 2, k + 8), float("nan"), dtype=dtype, device=dev())
+            w = wbuf[1:1 + n, :k]
+            w.copy_(normal(gen, n, k, scale=0.1, dtype=dtype))
+            y, _ = linear_forward(x, w)
+            assert torch.isfinite(y).all()
+            assert all(torch.isfinite(t).all() for t in linear_backward(y, x, w))
+            out = torch.full((m + 3, n), 5.0, dtype=dtype, device=dev())
+            d = _dense(x, w, 0)
+            ws = torch.empty(max(256, _lib.lib.v2vae_linear_workspace_bytes(d, 0)), dtype=torch.uint8, device=dev())
+            _lib.check(_lib.lib.v2vae_linear_fwd(d, x.data_ptr(), w.data_ptr(), None, None, out.data_ptr(), None, ws.data_ptr(),
+                                                 torch.cuda.current_stream().cuda_stream))
+            assert torch.equal(out[:m], y) and bool((out[m:] == 5.0).all())
+
+
+def test_extreme_pre_activations_have_finite_gradients():
+    from volterra_vae_amd.dense_ops import gated_linear, linear
+    for dtype in DTYPES:
+        x = torch.tensor([[-300.0], [-90.0], [-20.0], [0.0], [20.0], [90.0], [300.0]] * 5, device=dev()).to(dtype).requires_grad_(True)
+        w = torch.ones((3, 1), dtype=dtype, device=dev(), requires_grad=True)
+        for act in ("silu", "gelu", "tanh", "relu"):
+            y = linear(x, w, activation=act)
+            ref = act64(act, x.detach().double() @ w.detach().double().t())
+            assert torch.allclose(y.double(), ref, rtol=2 * u(dtype) + 1e-6, atol=1e-6)
+            for g in torch.autograd.grad(y, (x, w), torch.ones_like(y)):
+                assert torch.isfinite(g).all()
+            h = gated_linear(x, w, w, activation=act)
+            X, W = x.detach().double().requires_grad_(True), w.detach().double().requires_grad_(True)
+            H = act64(act, X @ W.t()) * (X @ W.t())
+            for g, r in zip(torch.autograd.grad(h, (x, w), torch.ones_like(h)), torch.autograd.grad(H, (X, W), torch.ones_like(H))):
+                # dw sums 300 * 300 over five rows: beyond float16's 65504, inf there and only there
+                assert not torch.isnan(g).any() and bool((torch.isfinite(g) | (r.abs() > torch.finfo(dtype).max)).all())
+
+
+def test_calls_on_another_stream():
+    from volterra_vae_amd.dense_ops import gated_linear, linear
+    x, wg, wu, bg, bu, dh = gated_case(300, 128, 160, torch.bfloat16, True, "plain", 8)
+    want = linear(gated_linear(x, wg, wu, bg, bu), wg.t().contiguous())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = linear(gated_linear(x, wg, wu, bg, bu), wg.t().contiguous())
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+
+
+def test_a_captured_block_replays_with_new_inputs():
+    """Forward and explicit backward of linear(gated_linear(x)) in one HIP graph, replayed on changing inputs with eager calls of the
+    same operators in between; every replay against the eager result."""
+    from volterra_vae_amd.dense_ops import gated_backward, gated_forward, linear_backward, linear_forward
+    for dtype, m in ((torch.float32, 200), (torch.bfloat16, 2000), (torch.float16, 4)):
+        x, wg, wu, bg, bu, _ = gated_case(m, 96, 64, dtype, True, "plain", 9)
+        wd, dy = wg.t().contiguous(), torch.ones((m, 96), dtype=dtype, device=dev())
+
+        def block():
+            h, gu = gated_forward(x, wg, wu, bg, bu, keep=True)
+            y, z = linear_forward(h, wd, residual=x, activation="tanh", keep=True)
+            dh, dwd, _ = linear_backward(dy, h, wd, z, activation="tanh", need=(True, True, False))
+            return [y, dwd, *gated_backward(dh, x, wg, wu, gu)]
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            block()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured = block()
+        for r in range(4):
+            x.copy_(x.roll(1, 0) * 0.9 + 0.01 * r)
+            eager = [t.clone() for t in block()]
+            graph.replay()
+            torch.cuda.synchronize()
+            for p, q in zip(captured, eager):
+                assert torch.equal(p, q)

@@ -81,6 +81,17 @@ class SynthArgs(C.Structure):
                 ("sym_lo", C.c_int64), ("sym_cnt", C.c_int64)]
 
 
+class Dense(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("activation", C.c_int32), ("rows", C.c_int64), ("in_", C.c_int64), ("out", C.c_int64),
+                ("ld_x", C.c_int64), ("ld_w", C.c_int64), ("ld_w2", C.c_int64), ("ld_res", C.c_int64), ("ld_dy", C.c_int64)]
+
+
+class Distill(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("teacher_dtype", C.c_int32), ("index_bits", C.c_int32), ("k", C.c_int32),
+                ("rows", C.c_int64), ("vocab", C.c_int64), ("ld_logits", C.c_int64), ("ld_teacher", C.c_int64),
+                ("ld_index", C.c_int64), ("temperature", C.c_float), ("reserved", C.c_int32)]
+
+
 EXPORTS = {
     # name: (restype, argtypes)
     "v2vae_version": (C.c_char_p, []),
@@ -111,6 +122,15 @@ EXPORTS = {
     "v2vae_adam_schedule": (C.c_int, [C.c_int64, C.c_int64, C.c_void_p, C.c_float, C.c_float, C.c_void_p, C.c_void_p]),
     "v2vae_fit_persistent": (C.c_int, [C.POINTER(Problem), C.POINTER(FitArgs), C.c_void_p]),
     "v2vae_fit_persistent_kind": (C.c_int, [C.POINTER(Problem)]),
+    "v2vae_linear_fwd": (C.c_int, [C.POINTER(Dense)] + [C.c_void_p] * 8),
+    "v2vae_linear_bwd": (C.c_int, [C.POINTER(Dense)] + [C.c_void_p] * 9),
+    "v2vae_linear_workspace_bytes": (C.c_size_t, [C.POINTER(Dense), C.c_int]),
+    "v2vae_gated_fwd": (C.c_int, [C.POINTER(Dense)] + [C.c_void_p] * 9),
+    "v2vae_gated_bwd": (C.c_int, [C.POINTER(Dense)] + [C.c_void_p] * 12),
+    "v2vae_gated_workspace_bytes": (C.c_size_t, [C.POINTER(Dense), C.c_int]),
+    "v2vae_distill_fwd": (C.c_int, [C.POINTER(Distill)] + [C.c_void_p] * 6),
+    "v2vae_distill_bwd": (C.c_int, [C.POINTER(Distill)] + [C.c_void_p] * 7),
+    "v2vae_distill_step": (C.c_int, [C.POINTER(Distill)] + [C.c_void_p] * 7),
     "v2vae_ws_offset_moments": (C.c_int64, [C.POINTER(Problem)]),
     "v2vae_ws_offset_gmoments": (C.c_int64, [C.POINTER(Problem)]),
     "v2vae_ws_offset_xhat_float": (C.c_int64, [C.POINTER(Problem)]),

@@ -1,0 +1,398 @@
+// Dense layers behind the C ABI: argument checks, workspace, choice of product kernel, and the elementwise half of the backward.
+#include <math.h>
+
+#include "v2vae_dense.h"
+
+namespace v2vae {
+
+// ---- dz = dy act'(z) and its column sums -------------------------------------------------------------------------------------
+// One pass over dy and the float pre-activations; memory bound.  A block owns a strip of columns and a chunk of rows, sums its
+// columns in float in a fixed order (per thread along the rows, then over the block's row threads) and leaves one partial per
+// chunk; k_column_join adds the chunks.  dz is rounded to T here, once, after its contribution to the column sum.
+struct SlopeArgs {
+    const void* dy;
+    int64_t ld_dy;
+    const float* z[2];  // pre-activations [M][N] (NULL: no activation), gated: gate and up
+    void* d[2];         // dz [M][N] (NULL: only the sums)
+    float* part[2];     // [chunks][N] (NULL: no sums)
+    int64_t M, rows_per_chunk;
+    int N, act, cx;     // cx threads along the columns, 256 / cx along the rows
+};
+
+template <typename T, int V, bool GATED> __global__ __launch_bounds__(256) void k_dense_slopes(SlopeArgs a) {
+    struct alignas(V * sizeof(T)) TV { T e[V]; };
+    struct alignas(V * 4) FV { float e[V]; };
+    __shared__ float s_sum[GATED ? 2 : 1][256 * V];
+    const int tid = threadIdx.x, cx = a.cx, ry = 256 / cx, tx = tid % cx, ty = tid / cx;
+    const int64_t n = ((int64_t)blockIdx.x * cx + tx) * V;
+    const int64_t lo = (int64_t)blockIdx.y * a.rows_per_chunk, hi = lo + a.rows_per_chunk < a.M ? lo + a.rows_per_chunk : a.M;
+    float s0[V], s1[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) s0[v] = s1[v] = 0.f;
+    if (n < a.N) {
+        for (int64_t m = lo + ty; m < hi; m += ry) {
+            const TV dy = *reinterpret_cast<const TV*>((const T*)a.dy + m * a.ld_dy + n);
+            TV o0, o1;
+            if constexpr (GATED) {
+                const FV gate = *reinterpret_cast<const FV*>(a.z[0] + m * a.N + n), up = *reinterpret_cast<const FV*>(a.z[1] + m * a.N + n);
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    float val;
+                    const float slope = act_slope(a.act, gate.e[v], &val), d = (float)dy.e[v];
+                    const float dg = d * up.e[v] * slope, du = d * val;
+                    s0[v] += dg;
+                    s1[v] += du;
+                    o0.e[v] = (T)dg;
+                    o1.e[v] = (T)du;
+                }
+                *reinterpret_cast<TV*>((T*)a.d[0] + m * a.N + n) = o0;
+                *reinterpret_cast<TV*>((T*)a.d[1] + m * a.N + n) = o1;
+            } else {
+                FV z;
+                if (a.z[0]) z = *reinterpret_cast<const FV*>(a.z[0] + m * a.N + n);
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    float val, d = (float)dy.e[v];
+                    if (a.z[0]) d *= act_slope(a.act, z.e[v], &val);
+                    s0[v] += d;
+                    o0.e[v] = (T)d;
+                }
+                if (a.d[0]) *reinterpret_cast<TV*>((T*)a.d[0] + m * a.N + n) = o0;
+            }
+        }
+    }
+    if (a.part[0] == nullptr) return;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        s_sum[0][tid * V + v] = s0[v];
+        if constexpr (GATED) s_sum[1][tid * V + v] = s1[v];
+    }
+    __syncthreads();
+    for (int i = tid; i < cx * V; i += 256) {
+        const int64_t col = (int64_t)blockIdx.x * cx * V + i;
+        if (col >= a.N) continue;
+#pragma unroll
+        for (int q = 0; q < (GATED ? 2 : 1); ++q) {
+            float s = 0.f;
+            for (int y = 0; y < ry; ++y) s += s_sum[q][y * cx * V + i];
+            a.part[q][(int64_t)blockIdx.y * a.N + col] = s;
+        }
+    }
+}
+
+// out[n] = sum of the chunks' partials, in a fixed order; 32 columns x 8 lanes a block
+template <typename T> __global__ __launch_bounds__(256) void k_column_join(const float* part0, const float* part1, void* out0, void* out1,
+                                                                           int chunks, int N) {
+    __shared__ float s_sum[8][33];
+    const float* part = blockIdx.y ? part1 : part0;
+    T* out = (T*)(blockIdx.y ? out1 : out0);
+    const int c = threadIdx.x & 31, y = threadIdx.x >> 5, n = blockIdx.x * 32 + c;
+    float s = 0.f;
+    if (out && n < N)
+        for (int i = y; i < chunks; i += 8) s += part[(int64_t)i * N + n];
+    s_sum[y][c] = s;
+    __syncthreads();
+    if (y == 0 && out && n < N) {
+        float t = 0.f;
+        for (int i = 0; i < 8; ++i) t += s_sum[i][c];
+        out[n] = (T)t;
+    }
+}
+
+// ---- host side ---------------------------------------------------------------------------------------------------------------
+static int elem_bytes(int dtype) { return dtype == V2VAE_F32 ? 4 : 2; }
+static bool aligned_to(const void* p, int n) { return ((uintptr_t)p % n) == 0; }
+static size_t round_up(size_t n) { return (n + 255) & ~(size_t)255; }
+
+constexpr int64_t DENSE_MAX = (int64_t)1 << 30;
+
+static int check_dense(const v2vae_dense* d, bool gated, bool backward, bool residual) {
+    if (!d || d->dtype < V2VAE_F32 || d->dtype > V2VAE_F16) return V2VAE_EINVAL;
+    if (d->activation < V2VAE_ACT_NONE || d->activation > V2VAE_ACT_TANH) return V2VAE_EINVAL;
+    if (d->rows < 0 || d->in < 1 || d->out < 1) return V2VAE_EINVAL;
+    if (d->rows > DENSE_MAX || d->in > DENSE_MAX || d->out > DENSE_MAX) return V2VAE_ESIZE;
+    if (d->ld_x < 0 || d->ld_w < 0 || (gated && d->ld_w2 < 0)) return V2VAE_EINVAL;
+    if ((residual && d->ld_res < 0) || (backward && d->ld_dy < 0)) return V2VAE_EINVAL;
+    // tiles of 64 x 64 (gated forward: 64 x 64 features) are counted in 31 bits
+    const int64_t m = (d->rows + 63) / 64, n = (d->out + 63) / 64, k = (d->in + 63) / 64;
+    if (m * n >= INT32_MAX || m * k >= INT32_MAX || n * k >= INT32_MAX) return V2VAE_ESIZE;
+    return V2VAE_OK;
+}
+
+// How a product M x N x K is cut: tile size and the number of parts of the contraction.
+struct Cut { int tile, splits, per; };
+static Cut cut_product(int64_t M, int64_t N, int64_t K, int segs, int batch, int dtype, bool gated) {
+    const int64_t bk = dtype == V2VAE_F32 ? 32 : 64, steps = ((K + bk - 1) / bk) * segs;
+    const int64_t big = ((M + 127) / 128) * ((N + (gated ? 63 : 127)) / (gated ? 64 : 128)) * batch;
+    const int64_t small = ((M + 63) / 64) * ((N + 63) / 64) * batch;
+    Cut c;
+    int64_t tiles;
+    if (big >= 256 || (big * (steps / 8) >= 256)) { c.tile = 0; tiles = big; } else { c.tile = 1; tiles = small; }
+    int64_t s = 1;
+    if (tiles < 256) {
+        s = 512 / (tiles < 1 ? 1 : tiles);
+        if (s > steps / 8) s = steps / 8;
+        if (s < 1) s = 1;
+    }
+    c.per = (int)((steps + s - 1) / s);
+    if (c.per < 1) c.per = 1;
+    c.splits = (int)((steps + c.per - 1) / c.per);
+    if (c.splits < 1) c.splits = 1;
+    return c;
+}
+static size_t partial_bytes(const Cut& c, int64_t M, int64_t N, int batch, bool gated) {
+    return c.splits > 1 ? round_up((size_t)c.splits * batch * M * N * (gated ? 2 : 1) * 4) : 0;
+}
+
+static void slope_shape(int64_t M, int64_t N, int V, int* cx, int* gx, int* chunks) {
+    const int64_t cols = (N + V - 1) / V;
+    int c = 1;
+    while (c < cols && c < 64) c *= 2;
+    *cx = c;
+    *gx = (int)((cols + c - 1) / c);
+    int64_t n = 2048 / *gx;
+    const int64_t most = M / ((256 / c) * 4);
+    if (n > most) n = most;
+    if (n > 512) n = 512;
+    *chunks = (int)(n < 1 ? 1 : n);
+}
+
+// workspace of the backward pass: dz (two for the gated block), the column partials, the partials of the two products
+struct BwdLayout { size_t dz[2], part[2], prod, total; };
+static BwdLayout bwd_layout(const v2vae_dense* d, bool gated) {
+    BwdLayout l;
+    const int n = gated ? 2 : 1;
+    size_t o = 0;
+    for (int i = 0; i < 2; ++i) {
+        l.dz[i] = o;
+        if (i < n && (gated || d->activation != V2VAE_ACT_NONE)) o += round_up((size_t)d->rows * d->out * elem_bytes(d->dtype));
+    }
+    int cx, gx, c1, c4;
+    slope_shape(d->rows, d->out, 1, &cx, &gx, &c1);
+    slope_shape(d->rows, d->out, 4, &cx, &gx, &c4);
+    for (int i = 0; i < 2; ++i) {
+        l.part[i] = o;
+        if (i < n) o += round_up((size_t)(c1 > c4 ? c1 : c4) * d->out * 4);
+    }
+    l.prod = o;
+    const Cut cx_ = cut_product(d->rows, d->in, d->out, n, 1, d->dtype, false);
+    const Cut cw = cut_product(d->out, d->in, d->rows, 1, n, d->dtype, false);
+    const size_t a = partial_bytes(cx_, d->rows, d->in, 1, false), b = partial_bytes(cw, d->out, d->in, n, false);
+    l.total = o + (a > b ? a : b);
+    return l;
+}
+
+static int run_product(GemmArgs& g, int dtype, int layout, bool gated, float* partial, hipStream_t st) {
+    if (g.M == 0 || g.N == 0) return V2VAE_OK;
+    const Cut c = cut_product(g.M, g.N, g.K, g.segs, g.batch, dtype, gated);
+    g.splits = c.splits;
+    g.steps_per_split = c.per;
+    g.partial = c.splits > 1 ? partial : nullptr;
+    const int e = 16 / elem_bytes(dtype), bytes = elem_bytes(dtype);
+    auto vec = [&](const void* p0, const void* p1, int64_t ld0, int64_t ld1) {
+        return aligned_to(p0, 16) && (p1 == nullptr || aligned_to(p1, 16)) && (ld0 * bytes) % 16 == 0 && (ld1 * bytes) % 16 == 0 && g.K % e == 0;
+    };
+    g.vec_a = layout != LAYOUT_MM && vec(g.a[0], g.a[1], g.lda, g.lda);
+    g.vec_b = layout == LAYOUT_KK && vec(g.b[0], g.b[1], g.ldb[0], g.ldb[1]);
+    if (dtype == V2VAE_F32) return gemm_staged_f32(g, layout, gated, c.tile, st);
+    if (dtype == V2VAE_BF16) return gemm_staged_bf16(g, layout, gated, c.tile, st);
+    return gemm_staged_f16(g, layout, gated, c.tile, st);
+}
+
+static int forward(const v2vae_dense* d, const void* x, const void* w0, const void* w1, const void* b0, const void* b1,
+                   const void* res, void* y, float* z, void* ws, hipStream_t st) {
+    const bool gated = w1 != nullptr;
+    GemmArgs g = {};
+    g.a[0] = x;
+    g.b[0] = w0;
+    g.b[1] = w1;
+    g.c[0] = y;
+    g.lda = d->ld_x;
+    g.ldb[0] = d->ld_w;
+    g.ldb[1] = gated ? d->ld_w2 : d->ld_w;
+    g.ldc = d->out;
+    g.M = (int)d->rows;
+    g.N = (int)d->out;
+    g.K = (int)d->in;
+    g.segs = g.batch = g.splits = 1;
+    g.bias[0] = b0;
+    g.bias[1] = b1;
+    g.residual = res;
+    g.ldr = d->ld_res;
+    g.z[0] = z;
+    g.z[1] = z ? z + (int64_t)d->rows * d->out : nullptr;
+    g.act = d->activation;
+    if (d->rows <= ROWS_MAX) {
+        const int e = 16 / elem_bytes(d->dtype);
+        g.vec_a = aligned_to(x, 16) && d->ld_x % e == 0 && d->in % e == 0;
+        g.vec_b = aligned_to(w0, 16) && d->ld_w % e == 0 && (!gated || (aligned_to(w1, 16) && d->ld_w2 % e == 0)) && d->in % e == 0;
+        return dense_rows(g, d->dtype, gated, st);
+    }
+    return run_product(g, d->dtype, LAYOUT_KK, gated, (float*)ws, st);
+}
+
+static int backward(const v2vae_dense* d, const void* x, const void* w0, const void* w1, const float* z, const void* dy, void* dx,
+                    void* dw0, void* dw1, void* db0, void* db1, void* ws, hipStream_t st) {
+    const bool gated = w1 != nullptr, act = gated || d->activation != V2VAE_ACT_NONE;
+    const BwdLayout l = bwd_layout(d, gated);
+    char* const base = (char*)ws;
+    const int64_t M = d->rows;
+    const void* dz[2] = {dy, nullptr};
+    int64_t ld_dz = d->ld_dy;
+    const bool want_b = db0 || db1, want_dz = dx || dw0 || dw1;
+    if ((act && want_dz) || want_b) {
+        SlopeArgs s = {};
+        s.dy = dy;
+        s.ld_dy = d->ld_dy;
+        s.M = M;
+        s.N = (int)d->out;
+        s.act = d->activation;
+        s.z[0] = act ? z : nullptr;
+        s.z[1] = gated ? z + M * d->out : nullptr;
+        if (act) {
+            s.d[0] = base + l.dz[0];
+            s.d[1] = gated ? base + l.dz[1] : nullptr;
+            dz[0] = s.d[0];
+            dz[1] = s.d[1];
+            ld_dz = d->out;
+        }
+        if (want_b) {
+            s.part[0] = (float*)(base + l.part[0]);
+            s.part[1] = gated ? (float*)(base + l.part[1]) : nullptr;
+        }
+        const int bytes = elem_bytes(d->dtype);
+        const bool v4 = d->out % 4 == 0 && d->ld_dy % 4 == 0 && aligned_to(dy, 4 * bytes) && (!act || aligned_to(z, 16));
+        int gx, chunks;
+        slope_shape(M, d->out, v4 ? 4 : 1, &s.cx, &gx, &chunks);
+        s.rows_per_chunk = (M + chunks - 1) / chunks;
+        const dim3 grid(gx, chunks);
+        auto go = [&](auto t) {
+            typedef decltype(t) T;
+            if (gated) {
+                if (v4) hipLaunchKernelGGL((k_dense_slopes<T, 4, true>), grid, dim3(256), 0, st, s);
+                else hipLaunchKernelGGL((k_dense_slopes<T, 1, true>), grid, dim3(256), 0, st, s);
+            } else {
+                if (v4) hipLaunchKernelGGL((k_dense_slopes<T, 4, false>), grid, dim3(256), 0, st, s);
+                else hipLaunchKernelGGL((k_dense_slopes<T, 1, false>), grid, dim3(256), 0, st, s);
+            }
+            if (want_b)
+                hipLaunchKernelGGL((k_column_join<T>), dim3((unsigned)((d->out + 31) / 32), gated ? 2 : 1), dim3(256), 0, st, s.part[0],
+                                   s.part[1], db0, db1, chunks, (int)d->out);
+        };
+        if (d->dtype == V2VAE_F32) go(float());
+        else if (d->dtype == V2VAE_BF16) go(bf16_t());
+        else go(f16_t());
+        const int rc = dense_launch_error("dense layer, backward");
+        if (rc != V2VAE_OK) return rc;
+    }
+    float* const prod = (float*)(base + l.prod);
+    if (dx) {
+        GemmArgs g = {};
+        g.a[0] = dz[0];
+        g.a[1] = dz[1];
+        g.b[0] = w0;
+        g.b[1] = w1;
+        g.c[0] = dx;
+        g.lda = ld_dz;
+        g.ldb[0] = d->ld_w;
+        g.ldb[1] = gated ? d->ld_w2 : d->ld_w;
+        g.ldc = d->in;
+        g.M = (int)M;
+        g.N = (int)d->in;
+        g.K = (int)d->out;
+        g.segs = gated ? 2 : 1;
+        g.batch = 1;
+        const int rc = run_product(g, d->dtype, LAYOUT_KM, false, prod, st);
+        if (rc != V2VAE_OK) return rc;
+    }
+    if (dw0 || dw1) {
+        GemmArgs g = {};
+        g.a[0] = dw0 ? dz[0] : dz[1];
+        g.a[1] = dz[1];
+        g.b[0] = g.b[1] = x;
+        g.c[0] = dw0 ? dw0 : dw1;
+        g.c[1] = dw1;
+        g.lda = ld_dz;
+        g.ldb[0] = g.ldb[1] = d->ld_x;
+        g.ldc = d->in;
+        g.M = (int)d->out;
+        g.N = (int)d->in;
+        g.K = (int)M;
+        g.segs = 1;
+        g.batch = dw0 && dw1 ? 2 : 1;
+        return run_product(g, d->dtype, LAYOUT_MM, false, prod, st);
+    }
+    return V2VAE_OK;
+}
+
+}  // namespace v2vae
+
+using namespace v2vae;
+
+extern "C" {
+
+size_t v2vae_linear_workspace_bytes(const v2vae_dense* d, int backward) {
+    if (check_dense(d, false, backward != 0, false) != V2VAE_OK) return 0;
+    if (backward) return bwd_layout(d, false).total;
+    if (d->rows <= ROWS_MAX) return 0;
+    return partial_bytes(cut_product(d->rows, d->out, d->in, 1, 1, d->dtype, false), d->rows, d->out, 1, false);
+}
+
+size_t v2vae_gated_workspace_bytes(const v2vae_dense* d, int backward) {
+    if (check_dense(d, true, backward != 0, false) != V2VAE_OK) return 0;
+    if (backward) return bwd_layout(d, true).total;
+    if (d->rows <= ROWS_MAX) return 0;
+    return partial_bytes(cut_product(d->rows, d->out, d->in, 1, 1, d->dtype, true), d->rows, d->out, 1, true);
+}
+
+int v2vae_linear_fwd(const v2vae_dense* d, const void* x, const void* w, const void* bias, const void* residual, void* y, float* z,
+                     void* ws, void* stream) {
+    const int rc = check_dense(d, false, false, residual != nullptr);
+    if (rc != V2VAE_OK) return rc;
+    if (d->rows == 0) return V2VAE_OK;
+    const int b = elem_bytes(d->dtype);
+    if (!x || !w || !y || !aligned_to(x, b) || !aligned_to(w, b) || !aligned_to(y, b) || !aligned_to(z, 4) || !aligned_to(ws, 256) ||
+        !aligned_to(bias, b) || !aligned_to(residual, b))
+        return V2VAE_EINVAL;
+    if (!ws && v2vae_linear_workspace_bytes(d, 0) > 0) return V2VAE_EINVAL;
+    return forward(d, x, w, nullptr, bias, nullptr, residual, y, z, ws, (hipStream_t)stream);
+}
+
+int v2vae_linear_bwd(const v2vae_dense* d, const void* x, const void* w, const float* z, const void* dy, void* dx, void* dw,
+                     void* dbias, void* ws, void* stream) {
+    const int rc = check_dense(d, false, true, false);
+    if (rc != V2VAE_OK) return rc;
+    const int b = elem_bytes(d->dtype);
+    if (d->rows > 0 && (!dy || (dw && !x) || (dx && !w) || (d->activation != V2VAE_ACT_NONE && !z))) return V2VAE_EINVAL;
+    if (!aligned_to(x, b) || !aligned_to(w, b) || !aligned_to(z, 4) || !aligned_to(dy, b) || !aligned_to(dx, b) || !aligned_to(dw, b) ||
+        !aligned_to(dbias, b) || !aligned_to(ws, 256) || !ws)
+        return V2VAE_EINVAL;
+    return backward(d, x, w, nullptr, z, dy, dx, dw, nullptr, dbias, nullptr, ws, (hipStream_t)stream);
+}
+
+int v2vae_gated_fwd(const v2vae_dense* d, const void* x, const void* wg, const void* wu, const void* bg, const void* bu, void* h,
+                    float* gu, void* ws, void* stream) {
+    const int rc = check_dense(d, true, false, false);
+    if (rc != V2VAE_OK) return rc;
+    if (d->rows == 0) return V2VAE_OK;
+    const int b = elem_bytes(d->dtype);
+    if (!x || !wg || !wu || !h || !aligned_to(x, b) || !aligned_to(wg, b) || !aligned_to(wu, b) || !aligned_to(h, b) ||
+        !aligned_to(gu, 4) || !aligned_to(ws, 256) || !aligned_to(bg, b) || !aligned_to(bu, b))
+        return V2VAE_EINVAL;
+    if (!ws && v2vae_gated_workspace_bytes(d, 0) > 0) return V2VAE_EINVAL;
+    return forward(d, x, wg, wu, bg, bu, nullptr, h, gu, ws, (hipStream_t)stream);
+}
+
+int v2vae_gated_bwd(const v2vae_dense* d, const void* x, const void* wg, const void* wu, const float* gu, const void* dh, void* dx,
+                    void* dwg, void* dwu, void* dbg, void* dbu, void* ws, void* stream) {
+    const int rc = check_dense(d, true, true, false);
+    if (rc != V2VAE_OK) return rc;
+    const int b = elem_bytes(d->dtype);
+    if (!wg || !wu || !ws || (d->rows > 0 && (!dh || !gu || ((dwg || dwu) && !x)))) return V2VAE_EINVAL;
+    if (!aligned_to(x, b) || !aligned_to(wg, b) || !aligned_to(wu, b) || !aligned_to(gu, 4) || !aligned_to(dh, b) || !aligned_to(dx, b) ||
+        !aligned_to(dwg, b) || !aligned_to(dwu, b) || !aligned_to(dbg, b) || !aligned_to(dbu, b) || !aligned_to(ws, 256))
+        return V2VAE_EINVAL;
+    return backward(d, x, wg, wu, gu, dh, dx, dwg, dwu, dbg, dbu, ws, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,296 @@
+// The staged matrix product of the dense layers: D[m][n] = sum_k A(m, k) B(n, k), any strides, any alignment, any size.
+//
+// A workgroup of four waves owns a (64 TM) x (64 TN) tile of D, each wave 32 TM x 32 TN of it in accumulators of
+// v_mfma_f32_32x32x16.  A contraction step of 128 bytes of every row goes global -> registers -> LDS: the next step's loads are
+// in flight while the current one is multiplied, and the step through registers is what makes the rest general:
+//  * float32: every element is split into three bf16 pieces (exact sum, see v2vae_bf16_split.h; here the gfx950 conversion
+//    instruction rounds two at a time) and six piece products per element pair are accumulated in float: float32 results at six
+//    bf16 instructions (bf16 pipe / 6 = 417 TF) where the f32 matrix instructions give 157 TF.
+//  * an operand whose rows, not whose contraction, are contiguous (both operands of a weight gradient) is read with lanes along
+//    the rows and transposed by the store into LDS;
+//  * rows and contraction ends that do not fill a tile, and rows that are not 16-byte aligned, are loaded element by element.
+// LDS rows are 128 (float: 64) bytes of 16-bit pieces plus 16 bytes: the row stride is an odd multiple of 16 bytes, so the
+// 16-byte reads of 16 consecutive rows touch every bank once.
+#ifndef V2VAE_DENSE_GEMM_H
+#define V2VAE_DENSE_GEMM_H
+#include "v2vae_dense.h"
+
+namespace v2vae {
+
+template <typename T> struct Elem;
+template <> struct Elem<float> { static constexpr int NP = 3, BK = 32; typedef bf16x8 frag; };
+template <> struct Elem<bf16_t> { static constexpr int NP = 1, BK = 64; typedef bf16x8 frag; };
+template <> struct Elem<f16_t> { static constexpr int NP = 1, BK = 64; typedef f16x8 frag; };
+
+__device__ __forceinline__ f32x16 mma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mma32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+// two floats -> their three bf16 pieces, each pair packed in a word
+__device__ __forceinline__ void split_pair(float x0, float x1, unsigned p[3]) {
+    typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        const bf16x2 h = {(__bf16)x0, (__bf16)x1};
+        const unsigned u = __builtin_bit_cast(unsigned, h);
+        p[i] = u;
+        x0 -= __uint_as_float(u << 16);
+        x1 -= __uint_as_float(u & 0xFFFF0000u);
+    }
+}
+
+// One operand's tile of one contraction step: ROWS rows x BK, held by 256 threads between the global load and the LDS store.
+template <typename T, int ROWS, bool KC> struct Stage;
+
+// contraction contiguous: eight lanes along a row (16 bytes each), 32 rows a pass
+template <typename T, int ROWS> struct Stage<T, ROWS, true> {
+    static constexpr int E = 16 / sizeof(T), PASS = ROWS / 32, BK = Elem<T>::BK, ROWB = BK * 2 + 16;
+    Vec16<T> v[PASS];
+    // row_of(r): pointer of tile row r at k = 0, or NULL beyond the matrix
+    template <typename F> __device__ __forceinline__ void load(int tid, int k0, int K, bool vec, F row_of) {
+        const int k = k0 + (tid & 7) * E;
+#pragma unroll
+        for (int j = 0; j < PASS; ++j) {
+            const T* p = row_of((tid >> 3) + 32 * j);
+            v[j].raw = u32x4{0, 0, 0, 0};
+            if (p == nullptr) continue;
+            if (vec) {
+                if (k < K) v[j].raw = *reinterpret_cast<const u32x4*>(p + k);
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (k + e < K) v[j].e[e] = p[k + e];
+            }
+        }
+    }
+    __device__ __forceinline__ void store(int tid, char* lds) const {
+#pragma unroll
+        for (int j = 0; j < PASS; ++j) {
+            char* d = lds + ((tid >> 3) + 32 * j) * ROWB;
+            if constexpr (sizeof(T) == 4) {
+                unsigned lo[3], hi[3];
+                split_pair(v[j].e[0], v[j].e[1], lo);
+                split_pair(v[j].e[2], v[j].e[3], hi);
+#pragma unroll
+                for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x2*>(d + p * ROWS * ROWB + (tid & 7) * 8) = u32x2{lo[p], hi[p]};
+            } else {
+                *reinterpret_cast<u32x4*>(d + (tid & 7) * 16) = v[j].raw;
+            }
+        }
+    }
+};
+
+// rows contiguous: lanes along the rows (element loads, coalesced at any alignment), every thread KT consecutive k of its row
+template <typename T, int ROWS> struct Stage<T, ROWS, false> {
+    static constexpr int BK = Elem<T>::BK, ROWB = BK * 2 + 16, KT = BK * ROWS / 256;
+    T v[KT];
+    template <typename F> __device__ __forceinline__ void load(int tid, int k0, int K, int64_t ld, F row_of) {
+        const int k = k0 + (tid / ROWS) * KT;
+        const T* p = row_of(tid % ROWS);
+        if (p != nullptr) p += (int64_t)k * ld;
+#pragma unroll
+        for (int e = 0; e < KT; ++e) v[e] = (p != nullptr && k + e < K) ? p[e * ld] : (T)0.f;
+    }
+    __device__ __forceinline__ void store(int tid, char* lds) const {
+        char* d = lds + (tid % ROWS) * ROWB + (tid / ROWS) * KT * 2;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int e = 0; e < KT; e += 8) {
+                unsigned q[4][3];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) split_pair(v[e + 2 * i], v[e + 2 * i + 1], q[i]);
+#pragma unroll
+                for (int p = 0; p < 3; ++p)
+                    *reinterpret_cast<u32x4*>(d + p * ROWS * ROWB + e * 2) = u32x4{q[0][p], q[1][p], q[2][p], q[3][p]};
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < KT; e += 8) {
+                Vec16<T> w;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) w.e[i] = v[e + i];
+                *reinterpret_cast<u32x4*>(d + e * 2) = w.raw;
+            }
+        }
+    }
+};
+
+// Block number -> tile: consecutive blocks go to the eight XCDs in turn, so every XCD gets a contiguous run of tiles (its own
+// L2), walked in groups of eight tile rows.
+__device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int* tm, int* tn) {
+    const int total = tiles_m * tiles_n, q = total / 8, r = total % 8, x = id & 7, i = id >> 3;
+    const int t = x * q + (x < r ? x : r) + i;
+    const int group = 8 * tiles_n, g = t / group, first = g * 8, rows = tiles_m - first < 8 ? tiles_m - first : 8;
+    const int in = t - g * group;
+    *tm = first + in % rows;
+    *tn = in / rows;
+}
+
+template <typename T, int TM, int TN, bool AKC, bool BKC, bool GATED>
+__global__ __launch_bounds__(256, 2) void k_gemm_staged(GemmArgs g) {
+    constexpr int NP = Elem<T>::NP, BK = Elem<T>::BK, ROWB = BK * 2 + 16, BM = 64 * TM, BN = 64 * TN;
+    static_assert(!GATED || TN == 2, "a gated wave holds one gate and one up block");
+    typedef typename Elem<T>::frag frag;
+    __shared__ __align__(16) char lds[NP * (BM + BN) * ROWB];
+    char* const lds_a = lds;
+    char* const lds_b = lds + NP * BM * ROWB;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
+    const int out_bn = GATED ? BN / 2 : BN;
+    const int tiles_m = (g.M + BM - 1) / BM, tiles_n = (g.N + out_bn - 1) / out_bn;
+    int tm, tn;
+    tile_of(blockIdx.x, tiles_m, tiles_n, &tm, &tn);
+    const int split = blockIdx.y, bat = blockIdx.z;
+    const int m0 = tm * BM, n0 = tn * out_bn;
+    const int steps_seg = (g.K + BK - 1) / BK, steps = steps_seg * g.segs;
+    const int s_lo = split * g.steps_per_split, s_hi = s_lo + g.steps_per_split < steps ? s_lo + g.steps_per_split : steps;
+
+    Stage<T, BM, AKC> sa;
+    Stage<T, BN, BKC> sb;
+    auto fetch = [&](int s) {
+        const int seg = s >= steps_seg ? 1 : 0, k0 = (s - seg * steps_seg) * BK, sel = seg | bat;
+        const T* a = (const T*)g.a[sel];
+        const T* b = (const T*)g.b[sel];
+        auto row_a = [&](int r) -> const T* {
+            const int m = m0 + r;
+            return m < g.M ? a + (AKC ? (int64_t)m * g.lda : (int64_t)m) : nullptr;
+        };
+        auto row_b = [&](int r) -> const T* {
+            if constexpr (GATED) {  // blocks of 32 rows: gate and up of the same features in turn, so that a wave holds both
+                const int n = n0 + (r >> 6) * 32 + (r & 31);
+                const T* w = (const T*)((r & 32) ? g.b[1] : g.b[0]);
+                return n < g.N ? w + (int64_t)n * g.ldb[(r >> 5) & 1] : nullptr;
+            } else {
+                const int n = n0 + r;
+                return n < g.N ? b + (BKC ? (int64_t)n * g.ldb[sel] : (int64_t)n) : nullptr;
+            }
+        };
+        if constexpr (AKC) sa.load(tid, k0, g.K, g.vec_a != 0, row_a); else sa.load(tid, k0, g.K, g.lda, row_a);
+        if constexpr (BKC) sb.load(tid, k0, g.K, g.vec_b != 0, row_b); else sb.load(tid, k0, g.K, g.ldb[sel], row_b);
+    };
+
+    f32x16 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+
+    if (s_lo < s_hi) {
+        fetch(s_lo);
+        sa.store(tid, lds_a);
+        sb.store(tid, lds_b);
+    }
+    __syncthreads();
+    const char* const fa = lds_a + (wm * 32 * TM + (lane & 31)) * ROWB + (lane >> 5) * 16;
+    const char* const fb = lds_b + (wn * 32 * TN + (lane & 31)) * ROWB + (lane >> 5) * 16;
+    for (int s = s_lo; s < s_hi; ++s) {
+        if (s + 1 < s_hi) fetch(s + 1);
+#pragma unroll
+        for (int kk = 0; kk < BK / 16; ++kk) {
+            frag a[TM][NP], b[TN][NP];
+#pragma unroll
+            for (int p = 0; p < NP; ++p) {
+#pragma unroll
+                for (int i = 0; i < TM; ++i) a[i][p] = *reinterpret_cast<const frag*>(fa + (p * BM + i * 32) * ROWB + kk * 32);
+#pragma unroll
+                for (int j = 0; j < TN; ++j) b[j][p] = *reinterpret_cast<const frag*>(fb + (p * BN + j * 32) * ROWB + kk * 32);
+            }
+            // piece products, the smallest first
+#pragma unroll
+            for (int sum = NP - 1; sum >= 0; --sum)
+#pragma unroll
+                for (int p = 0; p <= sum; ++p)
+#pragma unroll
+                    for (int i = 0; i < TM; ++i)
+#pragma unroll
+                        for (int j = 0; j < TN; ++j) acc[i][j] = mma32(a[i][p], b[j][sum - p], acc[i][j]);
+        }
+        __syncthreads();
+        if (s + 1 < s_hi) {
+            sa.store(tid, lds_a);
+            sb.store(tid, lds_b);
+        }
+        __syncthreads();
+    }
+
+    // lane: column lane % 32 of a block, rows 8 (e / 4) + 4 (lane / 32) + e % 4
+    float* const part = g.partial ? g.partial + ((int64_t)bat * g.splits + split) * ((int64_t)g.M * (GATED ? 2 : 1) * g.N) : nullptr;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int m = m0 + (wm * TM + i) * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+            if (m >= g.M) continue;
+            if constexpr (GATED) {
+                const int n = n0 + wn * 32 + (lane & 31);
+                if (n >= g.N) continue;
+                if (part) {
+                    part[(int64_t)m * 2 * g.N + n] = acc[i][0][e];
+                    part[(int64_t)m * 2 * g.N + g.N + n] = acc[i][1][e];
+                } else {
+                    finish_gated<T>(g, m, n, acc[i][0][e], acc[i][1][e]);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < TN; ++j) {
+                    const int n = n0 + (wn * TN + j) * 32 + (lane & 31);
+                    if (n >= g.N) continue;
+                    if (part) part[(int64_t)m * g.N + n] = acc[i][j][e];
+                    else if (bat == 0) finish_value<T>(g, m, n, acc[i][j][e]);
+                    else ((T*)g.c[1])[(int64_t)m * g.ldc + n] = (T)acc[i][j][e];
+                }
+            }
+        }
+}
+
+// Sums of a split contraction, added in the order of the splits, and the rest of the epilogue.
+template <typename T, bool GATED> __global__ __launch_bounds__(256) void k_gemm_join(GemmArgs g) {
+    const int64_t per = (int64_t)g.M * g.N * (GATED ? 2 : 1), count = (int64_t)g.M * g.N;
+    const int bat = blockIdx.y;
+    const float* base = g.partial + bat * (int64_t)g.splits * per;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
+        const int64_t m = i / g.N;
+        const int n = (int)(i - m * g.N);
+        if constexpr (GATED) {
+            float s0 = 0.f, s1 = 0.f;
+            for (int s = 0; s < g.splits; ++s) {
+                s0 += base[s * per + m * 2 * g.N + n];
+                s1 += base[s * per + m * 2 * g.N + g.N + n];
+            }
+            finish_gated<T>(g, m, n, s0, s1);
+        } else {
+            float s0 = 0.f;
+            for (int s = 0; s < g.splits; ++s) s0 += base[s * per + i];
+            if (bat == 0) finish_value<T>(g, m, n, s0);
+            else ((T*)g.c[1])[m * g.ldc + n] = (T)s0;
+        }
+    }
+}
+
+template <typename T, int TM, int TN, bool AKC, bool BKC, bool GATED> void launch_staged(const GemmArgs& g, hipStream_t st) {
+    const int bn = GATED ? 32 * TN : 64 * TN;
+    const int64_t tiles = (int64_t)((g.M + 64 * TM - 1) / (64 * TM)) * ((g.N + bn - 1) / bn);
+    hipLaunchKernelGGL((k_gemm_staged<T, TM, TN, AKC, BKC, GATED>), dim3((unsigned)tiles, g.splits, g.batch), dim3(256), 0, st, g);
+    if (g.partial) {
+        int64_t blocks = ((int64_t)g.M * g.N + 255) / 256;
+        if (blocks > 4096) blocks = 4096;
+        hipLaunchKernelGGL((k_gemm_join<T, GATED>), dim3((unsigned)blocks, g.batch), dim3(256), 0, st, g);
+    }
+}
+
+// tile: 0 = 128 x 128, 1 = 64 x 64 (gated: 64 rows x 64 features)
+template <typename T> int gemm_staged(const GemmArgs& g, int layout, bool gated, int tile, hipStream_t st) {
+    if (gated) {
+        if (tile == 0) launch_staged<T, 2, 2, true, true, true>(g, st); else launch_staged<T, 1, 2, true, true, true>(g, st);
+    } else if (layout == LAYOUT_KK) {
+        if (tile == 0) launch_staged<T, 2, 2, true, true, false>(g, st); else launch_staged<T, 1, 1, true, true, false>(g, st);
+    } else if (layout == LAYOUT_KM) {
+        if (tile == 0) launch_staged<T, 2, 2, true, false, false>(g, st); else launch_staged<T, 1, 1, true, false, false>(g, st);
+    } else {
+        if (tile == 0) launch_staged<T, 2, 2, false, false, false>(g, st); else launch_staged<T, 1, 1, false, false, false>(g, st);
+    }
+    return dense_launch_error("dense matrix product");
+}
+
+}  // namespace v2vae
+#endif

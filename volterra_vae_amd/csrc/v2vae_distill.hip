@@ -1,0 +1,344 @@
+// Distillation from a teacher's top logits: loss, gradient, or both in one pass over the student's logits.
+//
+// Row by row: with s = z / T,  m = max s,  l = sum exp(s - m),  q = exp(s - m) / l;  over the k teacher entries p = softmax(t / T),
+// loss = T^2 sum_j p_j (log p_j - (s_j - m - log l)),  dz = w T (q - p at its classes).  The dense part is bound by reading z and
+// writing dz once: a row is held in registers between the maximum, the sum and the gradient where it fits, by a group of lanes of
+// one wave (short rows) or by a whole workgroup (long ones); longer rows still are read again, out of the caches.  The k
+// sparse terms are patched over the dense gradient afterwards by the threads that hold the entries; a class that a row names
+// twice is patched by the first of its entries with the sum, so no two threads write one address and no atomics are needed.
+#include <math.h>
+
+#include "v2vae_dense.h"
+
+namespace v2vae {
+
+struct DistillArgs {
+    const void* z;
+    const void* t;
+    const void* index;
+    const float* weight;  // [rows], gradient weight
+    float* loss;          // [rows] or NULL
+    float* stats;         // [rows][2]: written by the loss pass, read by the gradient pass
+    void* grad;           // [rows][V] or NULL
+    int64_t ld_z, ld_t, ld_i;
+    int64_t rows;
+    int V, k, teacher_dtype, wide_index;
+    float inv_t, T;
+};
+
+enum { DO_LOSS = 1, DO_GRAD = 2 };
+
+__device__ __forceinline__ float teacher_at(const DistillArgs& a, int64_t row, int j) {
+    const int64_t o = row * a.ld_t + j;
+    return a.teacher_dtype == V2VAE_F32 ? ((const float*)a.t)[o]
+           : a.teacher_dtype == V2VAE_BF16 ? (float)((const bf16_t*)a.t)[o] : (float)((const f16_t*)a.t)[o];
+}
+// class of entry j: -1 absent, -2 beyond the vocabulary
+__device__ __forceinline__ int class_at(const DistillArgs& a, int64_t row, int j) {
+    const int64_t o = row * a.ld_i + j;
+    const int64_t c = a.wide_index ? ((const int64_t*)a.index)[o] : (int64_t)((const int32_t*)a.index)[o];
+    return c < 0 ? -1 : c >= a.V ? -2 : (int)c;
+}
+
+// Reductions over the lanes of a group: G lanes of a wave, or all 1024 / 256 threads of a workgroup through LDS.  Every lane
+// gets the result; the order is fixed.
+template <int G> struct Lanes {
+    float* scratch;
+    __device__ __forceinline__ float max(float v) const {
+#pragma unroll
+        for (int d = (G < 64 ? G : 64) / 2; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
+        if constexpr (G > 64) {
+            __syncthreads();
+            if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
+            __syncthreads();
+            v = scratch[0];
+#pragma unroll
+            for (int i = 1; i < G / 64; ++i) v = fmaxf(v, scratch[i]);
+        }
+        return v;
+    }
+    __device__ __forceinline__ float sum(float v) const {
+#pragma unroll
+        for (int d = (G < 64 ? G : 64) / 2; d > 0; d >>= 1) v += __shfl_xor(v, d);
+        if constexpr (G > 64) {
+            __syncthreads();
+            if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
+            __syncthreads();
+            v = scratch[0];
+#pragma unroll
+            for (int i = 1; i < G / 64; ++i) v += scratch[i];
+        }
+        return v;
+    }
+    __device__ __forceinline__ void sync() const {
+        if constexpr (G > 64) __syncthreads();
+        else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    }
+};
+
+constexpr float LOG2E = 1.4426950408889634f;
+// exp(s - m) for scaled values: the difference first (exact where it matters), then the base-2 exponential of the hardware
+__device__ __forceinline__ float exp_diff(float z, float zmax, float c) { return __builtin_amdgcn_exp2f((z - zmax) * c); }
+
+// G lanes a row, NV 16-byte pieces of the row held by each lane (HELD), or the row read once per pass.  MODE: DO_LOSS | DO_GRAD.
+// A DO_GRAD pass alone takes maximum and sum from `stats`.
+template <typename T, int G, int NV, bool HELD, int MODE>
+__global__ __launch_bounds__(G > 64 ? G : 256) void k_distill(DistillArgs a) {
+    constexpr int E = Vec16<T>::N, ROWS = G > 64 ? 1 : 256 / G;
+    constexpr bool STATS_GIVEN = MODE == DO_GRAD;
+    __shared__ float s_red[16];
+    __shared__ float s_p[V2VAE_DISTILL_MAX_K > 0 ? (G > 64 ? V2VAE_DISTILL_MAX_K : 1) : 1];
+    __shared__ int s_c[G > 64 ? V2VAE_DISTILL_MAX_K : 1];
+    const Lanes<G> lanes{s_red};
+    const int tid = G > 64 ? threadIdx.x : threadIdx.x % G;
+    const int64_t row = (int64_t)blockIdx.x * ROWS + (G > 64 ? 0 : threadIdx.x / G);
+    if (row >= a.rows) return;  // G > 64: a workgroup has one row; G <= 64: whole groups leave, shuffles stay within a group
+    const T* const z = (const T*)a.z + row * a.ld_z;
+    // pieces are cut at 16-byte addresses: `off` elements of the first piece lie before the row
+    const int off = (int)(((uintptr_t)z & 15) / sizeof(T));
+    const T* const z0 = z - off;
+    const int pieces = (a.V + off + E - 1) / E;
+    auto get = [&](int i) {
+        Vec16<T> v;
+        const int lo = i * E - off;
+        if (lo >= 0 && lo + E <= a.V) {
+            v.raw = *reinterpret_cast<const u32x4*>(z0 + i * E);
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) v.e[e] = (lo + e >= 0 && lo + e < a.V) ? z[lo + e] : (T)(-INFINITY);
+        }
+        return v;
+    };
+
+    const float c = a.inv_t * LOG2E;
+    Vec16<T> held[HELD ? NV : 1];
+    float zmax = -INFINITY, l = 0.f;
+    if constexpr (HELD) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (tid + i * G < pieces) held[i] = get(tid + i * G);
+            else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) held[i].e[e] = (T)(-INFINITY);
+            }
+        }
+    }
+    if constexpr (!STATS_GIVEN) {
+        if constexpr (HELD) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < E; ++e) zmax = fmaxf(zmax, (float)held[i].e[e]);
+            zmax = lanes.max(zmax);
+            const float zm = zmax == -INFINITY ? 0.f : zmax;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < E; ++e) l += exp_diff((float)held[i].e[e], zm, c);
+            l = lanes.sum(l);
+        } else {
+            // one pass with a running maximum per thread, joined at the end
+            float mine = -INFINITY;
+            for (int i = tid; i < pieces; i += G) {
+                const Vec16<T> v = get(i);
+                float top = (float)v.e[0];
+#pragma unroll
+                for (int e = 1; e < E; ++e) top = fmaxf(top, (float)v.e[e]);
+                if (top > mine) {
+                    l *= exp_diff(mine, top, c);
+                    mine = top;
+                }
+                const float zm = mine == -INFINITY ? 0.f : mine;
+#pragma unroll
+                for (int e = 0; e < E; ++e) l += exp_diff((float)v.e[e], zm, c);
+            }
+            zmax = lanes.max(mine);
+            l = lanes.sum(mine == -INFINITY ? l : l * exp_diff(mine, zmax, c));
+        }
+        if (a.stats && tid == 0) {
+            a.stats[2 * row] = zmax;
+            a.stats[2 * row + 1] = l;
+        }
+    } else {
+        zmax = a.stats[2 * row];
+        l = a.stats[2 * row + 1];
+    }
+    const float zm = zmax == -INFINITY ? 0.f : zmax;
+
+    // the teacher's entries: probabilities over the present ones
+    float tmax = -INFINITY;
+    int bad = 0;
+    for (int j = tid; j < a.k; j += G) {
+        const int cls = class_at(a, row, j);
+        const float t = teacher_at(a, row, j);
+        bad |= cls == -2 || (cls >= 0 && t != t);  // a class beyond the vocabulary, a NaN
+        if (cls >= 0) tmax = fmaxf(tmax, t);
+    }
+    const float any_bad = lanes.max(bad ? 1.f : 0.f);
+    tmax = lanes.max(tmax);
+    float mass = 0.f;
+    if (tmax != -INFINITY) {
+        for (int j = tid; j < a.k; j += G) {
+            const int cls = class_at(a, row, j);
+            if (cls >= 0) mass += expf((teacher_at(a, row, j) - tmax) * a.inv_t);
+        }
+    }
+    mass = lanes.sum(mass);
+    const bool some = mass != 0.f;  // inf among the teacher's logits: NaN, present
+    const float inv_mass = some ? 1.f / mass : 0.f, log_mass = logf(some ? mass : 1.f), log_l = logf(l);
+
+    if constexpr (MODE & DO_LOSS) {
+        float part = 0.f;
+        for (int j = tid; j < a.k; j += G) {
+            const int cls = class_at(a, row, j);
+            if (cls < 0 || !some) continue;
+            const float lt = (teacher_at(a, row, j) - tmax) * a.inv_t, p = expf(lt) * inv_mass;
+            if (p == 0.f) continue;
+            const float zj = (float)z[cls];
+            const float log_q = zj == -INFINITY ? -INFINITY : (zj - zm) * a.inv_t - log_l;
+            part += p * (lt - log_mass - log_q);
+        }
+        part = lanes.sum(part);
+        if (tid == 0) a.loss[row] = any_bad != 0.f ? NAN : a.T * a.T * part;
+    }
+    if constexpr (MODE & DO_GRAD) {
+        const float wt = any_bad != 0.f ? NAN : a.weight[row] * a.T;
+        const bool live = some || any_bad != 0.f;
+        const float inv_l = l == 0.f ? 0.f : 1.f / l, scale = wt * inv_l;
+        T* const out = (T*)a.grad + row * a.V;
+        const bool same_phase = (int)(((uintptr_t)out & 15) / sizeof(T)) == off;
+        auto put = [&](int i, const Vec16<T>& v) {
+            Vec16<T> o;
+#pragma unroll
+            for (int e = 0; e < E; ++e) o.e[e] = (T)(live ? exp_diff((float)v.e[e], zm, c) * scale : 0.f);
+            const int lo = i * E - off;
+            if (same_phase && lo >= 0 && lo + E <= a.V) {
+                *reinterpret_cast<u32x4*>(out + lo) = o.raw;
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (lo + e >= 0 && lo + e < a.V) out[lo + e] = o.e[e];
+            }
+        };
+        if constexpr (HELD) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (tid + i * G < pieces) put(tid + i * G, held[i]);
+        } else {
+            for (int i = tid; i < pieces; i += G) put(i, get(i));
+        }
+        if constexpr (G > 64) {
+            for (int j = tid; j < a.k; j += G) {
+                const int cls = class_at(a, row, j);
+                s_c[j] = cls;
+                s_p[j] = cls >= 0 && some ? expf((teacher_at(a, row, j) - tmax) * a.inv_t) * inv_mass : 0.f;
+            }
+        }
+        lanes.sync();
+        for (int j = tid; j < a.k; j += G) {
+            const int cls = G > 64 ? s_c[j] : class_at(a, row, j);
+            if (cls < 0 || !some) continue;
+            float p = 0.f;
+            bool first = true;
+            for (int i = 0; i < a.k; ++i) {
+                if (G > 64) {
+                    if (s_c[i] == cls) { p += s_p[i]; first &= i >= j; }
+                } else if (class_at(a, row, i) == cls) {
+                    p += expf((teacher_at(a, row, i) - tmax) * a.inv_t) * inv_mass;
+                    first &= i >= j;
+                }
+            }
+            if (first) out[cls] = (T)(wt * (exp_diff((float)z[cls], zm, c) * inv_l - p));
+        }
+    }
+}
+
+template <typename T, int G, int NV, bool HELD> static void go(const DistillArgs& a, int mode, hipStream_t st) {
+    constexpr int ROWS = G > 64 ? 1 : 256 / G, NT = G > 64 ? G : 256;
+    const dim3 grid((unsigned)((a.rows + ROWS - 1) / ROWS));
+    if (mode == DO_LOSS) hipLaunchKernelGGL((k_distill<T, G, NV, HELD, DO_LOSS>), grid, dim3(NT), 0, st, a);
+    else if (mode == DO_GRAD) hipLaunchKernelGGL((k_distill<T, G, NV, HELD, DO_GRAD>), grid, dim3(NT), 0, st, a);
+    else hipLaunchKernelGGL((k_distill<T, G, NV, HELD, DO_LOSS | DO_GRAD>), grid, dim3(NT), 0, st, a);
+}
+
+template <typename T> static int distill(const DistillArgs& a, int mode, hipStream_t st) {
+    constexpr int E = Vec16<T>::N;
+    const int64_t pieces = (a.V + 2 * E - 2) / E;  // of a row that starts anywhere in a piece
+    if (pieces <= 8) go<T, 8, 1, true>(a, mode, st);
+    else if (pieces <= 16) go<T, 16, 1, true>(a, mode, st);
+    else if (pieces <= 32) go<T, 16, 2, true>(a, mode, st);
+    else if (pieces <= 64) go<T, 32, 2, true>(a, mode, st);
+    else if (pieces <= 256) go<T, 64, 4, true>(a, mode, st);
+    else if (pieces <= 1024) go<T, 256, 4, true>(a, mode, st);
+    else if (pieces <= 4096) go<T, 1024, 4, true>(a, mode, st);
+    else if (pieces <= 8192) go<T, 1024, 8, true>(a, mode, st);
+    else go<T, 1024, 1, false>(a, mode, st);
+    return dense_launch_error("distillation");
+}
+
+static int check_distill(const v2vae_distill* d) {
+    if (!d || d->dtype < V2VAE_F32 || d->dtype > V2VAE_F16 || d->teacher_dtype < V2VAE_F32 || d->teacher_dtype > V2VAE_F16) return V2VAE_EINVAL;
+    if ((d->index_bits != 32 && d->index_bits != 64) || d->reserved != 0 || d->k < 1 || d->rows < 0 || d->vocab < 1) return V2VAE_EINVAL;
+    if (!(d->temperature > 0.f) || !isfinite(d->temperature) || !isfinite(1.f / d->temperature)) return V2VAE_EINVAL;
+    if (d->ld_logits < d->vocab || d->ld_teacher < d->k || d->ld_index < d->k) return V2VAE_EINVAL;
+    if (d->k > V2VAE_DISTILL_MAX_K || d->rows > ((int64_t)1 << 30) || d->vocab > ((int64_t)1 << 30)) return V2VAE_ESIZE;
+    return V2VAE_OK;
+}
+
+static int run_distill(const v2vae_distill* d, const void* logits, const void* teacher, const void* index, const float* weight,
+                       float* loss, float* stats, void* grad, int mode, void* stream) {
+    const int rc = check_distill(d);
+    if (rc != V2VAE_OK) return rc;
+    if (d->rows == 0) return V2VAE_OK;
+    auto bytes = [](int t) { return t == V2VAE_F32 ? 4 : 2; };
+    auto off = [](const void* p, int n) { return ((uintptr_t)p % n) != 0; };
+    if (!logits || !teacher || !index || off(logits, bytes(d->dtype)) || off(teacher, bytes(d->teacher_dtype)) || off(index, d->index_bits / 8))
+        return V2VAE_EINVAL;
+    if ((mode & DO_LOSS) && (!loss || off(loss, 4))) return V2VAE_EINVAL;
+    if ((mode & DO_GRAD) && (!grad || !weight || off(grad, bytes(d->dtype)) || off(weight, 4))) return V2VAE_EINVAL;
+    if (off(stats, 4) || (mode == DO_GRAD && !stats)) return V2VAE_EINVAL;
+    DistillArgs a = {};
+    a.z = logits;
+    a.t = teacher;
+    a.index = index;
+    a.weight = weight;
+    a.loss = loss;
+    a.stats = stats;
+    a.grad = grad;
+    a.ld_z = d->ld_logits;
+    a.ld_t = d->ld_teacher;
+    a.ld_i = d->ld_index;
+    a.rows = d->rows;
+    a.V = (int)d->vocab;
+    a.k = d->k;
+    a.teacher_dtype = d->teacher_dtype;
+    a.wide_index = d->index_bits == 64;
+    a.T = d->temperature;
+    a.inv_t = 1.f / d->temperature;
+    if (d->dtype == V2VAE_F32) return distill<float>(a, mode, (hipStream_t)stream);
+    if (d->dtype == V2VAE_BF16) return distill<bf16_t>(a, mode, (hipStream_t)stream);
+    return distill<f16_t>(a, mode, (hipStream_t)stream);
+}
+
+}  // namespace v2vae
+
+using namespace v2vae;
+
+extern "C" {
+
+int v2vae_distill_fwd(const v2vae_distill* d, const void* logits, const void* teacher, const void* index, float* loss, float* stats,
+                      void* stream) {
+    return run_distill(d, logits, teacher, index, nullptr, loss, stats, nullptr, DO_LOSS, stream);
+}
+
+int v2vae_distill_bwd(const v2vae_distill* d, const void* logits, const void* teacher, const void* index, const float* stats,
+                      const float* weight, void* grad, void* stream) {
+    return run_distill(d, logits, teacher, index, weight, nullptr, const_cast<float*>(stats), grad, DO_GRAD, stream);
+}
+
+int v2vae_distill_step(const v2vae_distill* d, const void* logits, const void* teacher, const void* index, const float* weight,
+                       float* loss, void* grad, void* stream) {
+    return run_distill(d, logits, teacher, index, weight, loss, nullptr, grad, DO_LOSS | DO_GRAD, stream);
+}
+
+}  // extern "C"

@@ -1845,6 +1845,9 @@ static inline int allow_lds(K kernel, int bytes) {
     return V2VAE_ELAUNCH;
 }
 
+// for the launchers in other files
+int dense_launch_error(const char* where) { return launch_status_at(where); }
+
 }  // namespace v2vae
 
 using namespace v2vae;

@@ -1,0 +1,372 @@
+"""Layers and loss of a network equaliser: `linear`, `gated_linear` and `topk_distillation` over the HIP kernels.
+
+Tensors in, kernels enqueued on the current HIP stream of the tensors' device; float32, bfloat16 or float16, one type for all
+tensors of a call, on a GPU only.  Matrices need unit stride inside a row; rows may lie any distance apart, and rows of inputs
+may overlap (windows that slide over one received sequence are a matrix with the row stride `samples_per_symbol`).
+
+Two ways to train: the functions named above are differentiable; `linear_forward` / `linear_backward`, `gated_forward` /
+`gated_backward` and `topk_distillation_step` are the same passes with every gradient an explicit result, for training loops
+that run without autograd (and for HIP graphs, into which they can be captured).  `torch.ops.v2vae.linear`,
+`torch.ops.v2vae.gated_linear` and `torch.ops.v2vae.topk_distillation` are the differentiable forms as registered ops.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from ._lib import Dense, Distill, check, lib
+
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "tanh": 4}
+MAX_TEACHER_ENTRIES = 1024
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _check_tensor(t, name, dim, like=None, dtype=None):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor (got {type(t).__name__})")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must live on the GPU: these kernels have no CPU implementation")
+    if like is not None and t.device != like.device:
+        raise ValueError(f"{name} is on {t.device}, expected {like.device}")
+    want = dtype if dtype is not None else (like.dtype if like is not None else None)
+    if want is None:
+        if t.dtype not in _DTYPES:
+            raise NotImplementedError(f"{name}: float32, bfloat16 or float16 only (got {t.dtype})")
+    elif t.dtype != want:
+        raise ValueError(f"{name} is {t.dtype}, expected {want}")
+    if t.dim() != dim:
+        raise ValueError(f"{name} must have {dim} dimension{'s' if dim > 1 else ''} (got {t.dim()})")
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name} must have unit stride in its last dimension")
+
+
+def _row_stride(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _activation(kind):
+    try:
+        return ACTIVATIONS[kind]
+    except KeyError:
+        raise ValueError(f"activation {kind!r} is none of {', '.join(ACTIVATIONS)}") from None
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+class _On:
+    """The tensors' device made current around the calls, where it is not already."""
+
+    def __init__(self, device):
+        self.guard = torch.cuda.device(device) if device.index != torch.cuda.current_device() else None
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _workspace(n, device):
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+
+
+def _check_layer(x, weight, name, bias, bias_name):
+    _check_tensor(weight, name, 2, like=x)
+    if weight.shape[1] != x.shape[1]:
+        raise ValueError(f"{name}: {weight.shape[1]} columns, x has {x.shape[1]}")
+    if weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError(f"{name}: empty")
+    if bias is not None:
+        _check_tensor(bias, bias_name, 1, like=x)
+        if bias.shape[0] != weight.shape[0]:
+            raise ValueError(f"{bias_name}: {bias.shape[0]} values, {name} has {weight.shape[0]} rows")
+
+
+def _dense(x, w, act, w2=None, residual=None, dy=None):
+    return Dense(_DTYPES[x.dtype], act, x.shape[0], x.shape[1], w.shape[0], _row_stride(x), _row_stride(w),
+                 0 if w2 is None else _row_stride(w2), 0 if residual is None else _row_stride(residual),
+                 0 if dy is None else _row_stride(dy))
+
+
+def _check_grad(dy, name, x, n):
+    _check_tensor(dy, name, 2, like=x)
+    if tuple(dy.shape) != (x.shape[0], n):
+        raise ValueError(f"{name}: expected {(x.shape[0], n)}, got {tuple(dy.shape)}")
+
+
+def _check_kept(kept, shape, x):
+    _check_tensor(kept, "the kept pre-activations", len(shape), like=x, dtype=torch.float32)
+    if tuple(kept.shape) != shape or not kept.is_contiguous():
+        raise ValueError(f"the kept pre-activations: expected a contiguous {shape}, got {tuple(kept.shape)}")
+
+
+# ------------------------------------------------------------------------------------------------ linear
+def linear_forward(x, weight, bias=None, *, residual=None, activation="none",
+                   keep=False) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """(y, z) for x [M, K], weight [N, K]: y = activation(x weight^T + bias) + residual, and, if `keep` and there is an
+    activation, the float32 pre-activations z [M, N] that `linear_backward` wants (else None)."""
+    act = _activation(activation)
+    _check_tensor(x, "x", 2)
+    _check_layer(x, weight, "weight", bias, "bias")
+    m, n = x.shape[0], weight.shape[0]
+    if residual is not None:
+        _check_tensor(residual, "residual", 2, like=x)
+        if tuple(residual.shape) != (m, n):
+            raise ValueError(f"residual: expected {(m, n)}, got {tuple(residual.shape)}")
+    d = _dense(x, weight, act, residual=residual)
+    with _On(x.device) as stream:
+        y = torch.empty((m, n), dtype=x.dtype, device=x.device)
+        z = torch.empty((m, n), dtype=torch.float32, device=x.device) if keep and act else None
+        ws = _workspace(lib.v2vae_linear_workspace_bytes(d, 0), x.device)
+        check(lib.v2vae_linear_fwd(d, _p(x), _p(weight), _p(bias), _p(residual), _p(y), _p(z), _p(ws), stream), "v2vae_linear_fwd")
+    return y, z
+
+
+def linear_backward(dy, x, weight, z=None, *, activation="none", need=(True, True, True)):
+    """(dx, dweight, dbias) of `linear_forward` given dy [M, N] and the kept z; None where `need` says so.  The residual's
+    gradient is dy."""
+    act = _activation(activation)
+    _check_tensor(x, "x", 2)
+    _check_layer(x, weight, "weight", None, "")
+    m, k, n = x.shape[0], x.shape[1], weight.shape[0]
+    _check_grad(dy, "dy", x, n)
+    if act:
+        if z is None:
+            raise ValueError("z: the pre-activations of linear_forward(..., keep=True) are needed with an activation")
+        _check_kept(z, (m, n), x)
+    d = _dense(x, weight, act, dy=dy)
+    with _On(x.device) as stream:
+        new = lambda wanted, *shape: torch.empty(shape, dtype=x.dtype, device=x.device) if wanted else None  # noqa: E731
+        dx, dw, db = new(need[0], m, k), new(need[1], n, k), new(need[2], n)
+        ws = _workspace(max(256, lib.v2vae_linear_workspace_bytes(d, 1)), x.device)
+        check(lib.v2vae_linear_bwd(d, _p(x), _p(weight), _p(z) if act else None, _p(dy), _p(dx), _p(dw), _p(db), _p(ws), stream),
+              "v2vae_linear_bwd")
+    return dx, dw, db
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation):
+        y, z = linear_forward(x, weight, bias, residual=residual, activation=activation,
+                              keep=any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(x, weight, z)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, z = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx = dw = db = None
+        if any(need[:3]):
+            g = dy if dy.shape[1] <= 1 or dy.stride(1) == 1 else dy.contiguous()
+            dx, dw, db = linear_backward(g, x, weight, z, activation=ctx.activation, need=need[:3])
+        return dx, dw, db, dy if need[3] else None, None
+
+
+def _flat(t):
+    return t if t is None or t.dim() == 2 else t.reshape(-1, t.shape[-1])
+
+
+def _grads_wanted(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *, residual: Optional[torch.Tensor] = None,
+           activation: str = "none") -> torch.Tensor:
+    """activation(x weight^T + bias) + residual for x [..., K], weight [N, K], bias [N], residual [..., N], in one kernel.
+
+    activation: none, relu, silu, gelu (erf form) or tanh.  Differentiable in every tensor.  Sums are float32; the backward pass
+    works from float32 pre-activations and rounds dy * activation' to the tensors' type once before the two products."""
+    if not isinstance(x, torch.Tensor) or x.dim() < 1:
+        raise ValueError("x must be a tensor [..., K]")
+    if residual is not None and tuple(residual.shape[:-1]) != tuple(x.shape[:-1]):
+        raise ValueError(f"residual: expected {tuple(x.shape[:-1])} rows, got {tuple(residual.shape[:-1])}")
+    flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if _grads_wanted(x, weight, bias, residual):
+        y = _Linear.apply(flat, weight, bias, _flat(residual), activation)
+    else:
+        y = linear_forward(flat, weight, bias, residual=_flat(residual), activation=activation)[0]
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], y.shape[-1])
+
+
+# ------------------------------------------------------------------------------------------------ gated block
+def gated_forward(x, weight_gate, weight_up, bias_gate=None, bias_up=None, *, activation="silu",
+                  keep=False) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """(h, gu) for x [M, K], weights [N, K]: h = activation(x weight_gate^T + bias_gate) * (x weight_up^T + bias_up), and, if
+    `keep`, the float32 pre-activations gu [2, M, N] (gate, up) that `gated_backward` wants (else None)."""
+    act = _activation(activation)
+    _check_tensor(x, "x", 2)
+    _check_layer(x, weight_gate, "weight_gate", bias_gate, "bias_gate")
+    _check_layer(x, weight_up, "weight_up", bias_up, "bias_up")
+    if weight_up.shape != weight_gate.shape:
+        raise ValueError(f"weight_up: expected {tuple(weight_gate.shape)}, got {tuple(weight_up.shape)}")
+    m, n = x.shape[0], weight_gate.shape[0]
+    d = _dense(x, weight_gate, act, w2=weight_up)
+    with _On(x.device) as stream:
+        h = torch.empty((m, n), dtype=x.dtype, device=x.device)
+        gu = torch.empty((2, m, n), dtype=torch.float32, device=x.device) if keep else None
+        ws = _workspace(lib.v2vae_gated_workspace_bytes(d, 0), x.device)
+        check(lib.v2vae_gated_fwd(d, _p(x), _p(weight_gate), _p(weight_up), _p(bias_gate), _p(bias_up), _p(h), _p(gu), _p(ws), stream),
+              "v2vae_gated_fwd")
+    return h, gu
+
+
+def gated_backward(dh, x, weight_gate, weight_up, gu, *, activation="silu", need=(True, True, True, True, True)):
+    """(dx, dweight_gate, dweight_up, dbias_gate, dbias_up) of `gated_forward` given dh [M, N] and the kept gu; None where
+    `need` says so."""
+    act = _activation(activation)
+    _check_tensor(x, "x", 2)
+    _check_layer(x, weight_gate, "weight_gate", None, "")
+    _check_layer(x, weight_up, "weight_up", None, "")
+    if weight_up.shape != weight_gate.shape:
+        raise ValueError(f"weight_up: expected {tuple(weight_gate.shape)}, got {tuple(weight_up.shape)}")
+    m, k, n = x.shape[0], x.shape[1], weight_gate.shape[0]
+    _check_grad(dh, "dh", x, n)
+    _check_kept(gu, (2, m, n), x)
+    d = _dense(x, weight_gate, act, w2=weight_up, dy=dh)
+    with _On(x.device) as stream:
+        new = lambda wanted, *shape: torch.empty(shape, dtype=x.dtype, device=x.device) if wanted else None  # noqa: E731
+        out = [new(need[0], m, k), new(need[1], n, k), new(need[2], n, k), new(need[3], n), new(need[4], n)]
+        ws = _workspace(max(256, lib.v2vae_gated_workspace_bytes(d, 1)), x.device)
+        check(lib.v2vae_gated_bwd(d, _p(x), _p(weight_gate), _p(weight_up), _p(gu), _p(dh), *[_p(t) for t in out], _p(ws), stream),
+              "v2vae_gated_bwd")
+    return tuple(out)
+
+
+class _Gated(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight_gate, weight_up, bias_gate, bias_up, activation):
+        h, gu = gated_forward(x, weight_gate, weight_up, bias_gate, bias_up, activation=activation, keep=True)
+        ctx.save_for_backward(x, weight_gate, weight_up, gu)
+        ctx.activation = activation
+        return h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh):
+        x, weight_gate, weight_up, gu = ctx.saved_tensors
+        g = dh if dh.shape[1] <= 1 or dh.stride(1) == 1 else dh.contiguous()
+        return (*gated_backward(g, x, weight_gate, weight_up, gu, activation=ctx.activation, need=ctx.needs_input_grad[:5]), None)
+
+
+def gated_linear(x: torch.Tensor, weight_gate: torch.Tensor, weight_up: torch.Tensor, bias_gate: Optional[torch.Tensor] = None,
+                 bias_up: Optional[torch.Tensor] = None, *, activation: str = "silu") -> torch.Tensor:
+    """Gated feed-forward block: activation(x weight_gate^T + bias_gate) * (x weight_up^T + bias_up) for x [..., K], weights
+    [N, K], both projections, the activation and the product in one kernel.  Differentiable in every tensor."""
+    if not isinstance(x, torch.Tensor) or x.dim() < 1:
+        raise ValueError("x must be a tensor [..., K]")
+    flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if _grads_wanted(x, weight_gate, weight_up, bias_gate, bias_up):
+        h = _Gated.apply(flat, weight_gate, weight_up, bias_gate, bias_up, activation)
+    else:
+        h = gated_forward(flat, weight_gate, weight_up, bias_gate, bias_up, activation=activation)[0]
+    return h if x.dim() == 2 else h.view(*x.shape[:-1], h.shape[-1])
+
+
+# ------------------------------------------------------------------------------------------------ distillation
+def _distill(logits, teacher_logits, teacher_index, temperature):
+    _check_tensor(logits, "logits", 2)
+    if not isinstance(teacher_logits, torch.Tensor) or teacher_logits.dtype not in _DTYPES:
+        raise NotImplementedError("teacher_logits: a float32, bfloat16 or float16 tensor")
+    if not isinstance(teacher_index, torch.Tensor) or teacher_index.dtype not in (torch.int32, torch.int64):
+        raise ValueError("teacher_index: an int32 or int64 tensor")
+    _check_tensor(teacher_logits, "teacher_logits", 2, like=logits, dtype=teacher_logits.dtype)
+    _check_tensor(teacher_index, "teacher_index", 2, like=logits, dtype=teacher_index.dtype)
+    m, v = logits.shape
+    k = teacher_logits.shape[1]
+    if v < 1:
+        raise ValueError("logits: no classes")
+    if not 1 <= k <= MAX_TEACHER_ENTRIES:
+        raise ValueError(f"teacher_logits: 1 ... {MAX_TEACHER_ENTRIES} entries a row (got {k})")
+    if teacher_logits.shape[0] != m or tuple(teacher_index.shape) != (m, k):
+        raise ValueError(f"teacher_logits and teacher_index: expected {(m, k)}, got {tuple(teacher_logits.shape)} and "
+                         f"{tuple(teacher_index.shape)}")
+    if not (temperature > 0 and math.isfinite(temperature)):
+        raise ValueError(f"temperature must be positive and finite (got {temperature})")
+    return Distill(_DTYPES[logits.dtype], _DTYPES[teacher_logits.dtype], 32 if teacher_index.dtype == torch.int32 else 64, k, m, v,
+                   _row_stride(logits) if m > 1 else v, _row_stride(teacher_logits), _row_stride(teacher_index), temperature, 0)
+
+
+def _check_weight(weight, logits):
+    _check_tensor(weight, "row_weight", 1, like=logits, dtype=torch.float32)
+    if weight.shape[0] != logits.shape[0]:
+        raise ValueError(f"row_weight: expected {logits.shape[0]} values, got {weight.shape[0]}")
+
+
+def topk_distillation_step(logits, teacher_logits, teacher_index, row_weight, *, temperature: float = 1.0):
+    """(loss [M] float32, grad [M, V]): the losses of `topk_distillation` and d(sum of row_weight * loss) / d logits, one pass."""
+    d = _distill(logits, teacher_logits, teacher_index, temperature)
+    _check_weight(row_weight, logits)
+    with _On(logits.device) as stream:
+        loss = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        check(lib.v2vae_distill_step(d, _p(logits), _p(teacher_logits), _p(teacher_index), _p(row_weight), _p(loss), _p(grad), stream),
+              "v2vae_distill_step")
+    return loss, grad
+
+
+class _Distillation(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, teacher_logits, teacher_index, temperature):
+        loss, stats = _distill_forward(logits, teacher_logits, teacher_index, temperature, True)
+        ctx.save_for_backward(logits, teacher_logits, teacher_index, stats)
+        ctx.temperature = temperature
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, weight):
+        logits, teacher_logits, teacher_index, stats = ctx.saved_tensors
+        d = _distill(logits, teacher_logits, teacher_index, ctx.temperature)
+        weight = weight.contiguous()
+        with _On(logits.device) as stream:
+            grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+            check(lib.v2vae_distill_bwd(d, _p(logits), _p(teacher_logits), _p(teacher_index), _p(stats), _p(weight), _p(grad), stream),
+                  "v2vae_distill_bwd")
+        return grad, None, None, None
+
+
+def _distill_forward(logits, teacher_logits, teacher_index, temperature, keep):
+    d = _distill(logits, teacher_logits, teacher_index, temperature)
+    with _On(logits.device) as stream:
+        loss = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
+        stats = torch.empty((logits.shape[0], 2), dtype=torch.float32, device=logits.device) if keep else None
+        check(lib.v2vae_distill_fwd(d, _p(logits), _p(teacher_logits), _p(teacher_index), _p(loss), _p(stats), stream),
+              "v2vae_distill_fwd")
+    return loss, stats
+
+
+def topk_distillation(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor, *,
+                      temperature: float = 1.0) -> torch.Tensor:
+    """Per-row distillation losses [M] (float32) of student logits [M, V] against a teacher's top logits [M, k] at the classes
+    teacher_index [M, k] (int32 or int64):
+
+        p = softmax(teacher / T),  q = softmax(logits / T),  loss = T^2 sum_j p_j (log p_j - log q[index_j])
+
+    An entry with index < 0 or a teacher logit of -inf is absent; a row without present entries has loss and gradient 0; a class
+    that a row names twice counts twice.  An index >= V makes the row NaN.  Differentiable in `logits`; the teacher is not."""
+    if isinstance(teacher_logits, torch.Tensor) and teacher_logits.requires_grad and torch.is_grad_enabled():
+        raise ValueError("teacher_logits: the loss is not differentiable in the teacher (pass teacher_logits.detach())")
+    if isinstance(logits, torch.Tensor) and _grads_wanted(logits):
+        return _Distillation.apply(logits, teacher_logits, teacher_index, temperature)
+    return _distill_forward(logits, teacher_logits, teacher_index, temperature, False)[0]
+
+
+# ------------------------------------------------------------------------------------------------ registered ops
+_LIBRARY = torch.library.Library("v2vae", "FRAGMENT")
+_LIBRARY.define("linear(Tensor x, Tensor weight, Tensor? bias=None, *, Tensor? residual=None, str activation='none') -> Tensor")
+_LIBRARY.define("gated_linear(Tensor x, Tensor weight_gate, Tensor weight_up, Tensor? bias_gate=None, Tensor? bias_up=None, *, "
+                "str activation='silu') -> Tensor")
+_LIBRARY.define("topk_distillation(Tensor logits, Tensor teacher_logits, Tensor teacher_index, *, float temperature=1.0) -> Tensor")
+for _name, _fn in (("linear", linear), ("gated_linear", gated_linear), ("topk_distillation", topk_distillation)):
+    _LIBRARY.impl(_name, _fn, "CompositeImplicitAutograd")
