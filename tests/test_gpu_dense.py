@@ -225,6 +225,21 @@ def test_gated_block_through_autograd(dtype):
     assert torch.equal(g, leaves[2].grad)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16", "f16"])
+def test_shapes_of_many_tiles(dtype):
+    """Several tiles in both directions, ends that fill no tile, long contractions that are split, weights with different strides."""
+    from volterra_vae_amd.dense_ops import gated_backward, gated_forward, linear_backward, linear_forward
+    for m, k, n, act in ((4100, 1032, 520, "silu"), (300, 2056, 4104, "gelu"), (9000, 72, 136, "tanh"), (2304, 512, 2304, "none"), (70, 8192, 64, "none")):
+        x, w, b, r, dy = linear_case(m, k, n, dtype, act, True, True, "wide", m)
+        y, z = linear_forward(x, w, b, residual=r, activation=act, keep=True)
+        check_linear(x, w, b, r, dy, act, y, linear_backward(dy, x, w, z, activation=act), dtype)
+    for m, k, n in ((4100, 520, 1032), (600, 2048, 520), (5000, 64, 136)):
+        x, wg, wu, bg, bu, dh = gated_case(m, k, n, dtype, True, "plain", m)
+        for up in (wu, laid_out(wu, "wide"), laid_out(wu, "odd")):
+            h, gu = gated_forward(x, wg, up, bg, bu, keep=True)
+            check_gated(x, wg, up, bg, bu, dh, "silu", h, gated_backward(dh, x, wg, up, gu), dtype)
+
+
 def test_gradients_agree_with_differences():
     """Central differences of float64-accumulated losses through the float32 kernels: step h = 2^-6, truncation h^2 / 6 times the third
     derivative along the direction (of order 1) and rounding 2^-24 / h of the values: 2e-3 of the directional derivative's scale."""

@@ -65,6 +65,7 @@ struct GemmArgs {
     int M, N, K;            // rows of A, rows of B (output columns; gated forward: features), contraction length of a segment
     int segs, batch, splits, steps_per_split;
     int vec_a, vec_b;       // 16-byte loads allowed
+    int vec_c;              // eight columns at a time in the epilogue: N, strides and pointers allow it
     const void* bias[2];
     const void* residual;
     int64_t ldr;
@@ -72,23 +73,82 @@ struct GemmArgs {
     int act;
 };
 
-// What happens to a finished sum of row m, column n.
-template <typename T> __device__ __forceinline__ void finish_value(const GemmArgs& g, int64_t m, int n, float s) {
-    if (g.bias[0]) s += (float)((const T*)g.bias[0])[n];
-    if (g.z[0]) g.z[0][m * g.N + n] = s;
-    s = act_value(g.act, s);
-    if (g.residual) s += (float)((const T*)g.residual)[m * g.ldr + n];
-    ((T*)g.c[0])[m * g.ldc + n] = (T)s;
+// What happens to the finished sums of row m, columns n ... n + C - 1 (batch entry 1 has an output of its own, nothing else).
+// `whole`: all C columns exist and every pointer is aligned for them.
+template <typename T, int C> __device__ __forceinline__ void load_columns(const void* p, int64_t at, int count, bool whole, float v[C]) {
+    struct alignas(C * sizeof(T) > 16 ? 16 : C * sizeof(T)) TC { T e[C]; };
+    if (whole) {
+        const TC t = *reinterpret_cast<const TC*>((const T*)p + at);
+#pragma unroll
+        for (int e = 0; e < C; ++e) v[e] = (float)t.e[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < C; ++e) v[e] = e < count ? (float)((const T*)p)[at + e] : 0.f;
+    }
 }
-template <typename T> __device__ __forceinline__ void finish_gated(const GemmArgs& g, int64_t m, int n, float gate, float up) {
-    if (g.bias[0]) { gate += (float)((const T*)g.bias[0])[n]; }
-    if (g.bias[1]) { up += (float)((const T*)g.bias[1])[n]; }
-    if (g.z[0]) { g.z[0][m * g.N + n] = gate; g.z[1][m * g.N + n] = up; }
-    ((T*)g.c[0])[m * g.ldc + n] = (T)(act_value(g.act, gate) * up);
+template <typename T, int C> __device__ __forceinline__ void store_columns(void* p, int64_t at, int count, bool whole, const float v[C]) {
+    struct alignas(C * sizeof(T) > 16 ? 16 : C * sizeof(T)) TC { T e[C]; };
+    if (whole) {
+        TC t;
+#pragma unroll
+        for (int e = 0; e < C; ++e) t.e[e] = (T)v[e];
+        *reinterpret_cast<TC*>((T*)p + at) = t;
+    } else {
+#pragma unroll
+        for (int e = 0; e < C; ++e)
+            if (e < count) ((T*)p)[at + e] = (T)v[e];
+    }
 }
-
+template <int C> __device__ __forceinline__ void act_columns(int kind, float v[C]) {
+    if (kind == V2VAE_ACT_NONE) return;
+#pragma unroll
+    for (int e = 0; e < C; ++e) v[e] = act_value(kind, v[e]);
+}
+template <typename T, int C> __device__ __forceinline__ void finish_value(const GemmArgs& g, int64_t m, int n, float s[C], int bat, bool whole) {
+    const int count = g.N - n;
+    float v[C];
+    if (g.bias[0]) {
+        load_columns<T, C>(g.bias[0], n, count, whole, v);
+#pragma unroll
+        for (int e = 0; e < C; ++e) s[e] += v[e];
+    }
+    if (g.z[0]) store_columns<float, C>(g.z[0], m * g.N + n, count, whole, s);
+    act_columns<C>(g.act, s);
+    if (g.residual) {
+        load_columns<T, C>(g.residual, m * g.ldr + n, count, whole, v);
+#pragma unroll
+        for (int e = 0; e < C; ++e) s[e] += v[e];
+    }
+    store_columns<T, C>(g.c[bat], m * g.ldc + n, count, whole, s);
+}
+template <typename T, int C>
+__device__ __forceinline__ void finish_gated(const GemmArgs& g, int64_t m, int n, float gate[C], float up[C], bool whole) {
+    const int count = g.N - n;
+    float v[C];
+    if (g.bias[0]) {
+        load_columns<T, C>(g.bias[0], n, count, whole, v);
+#pragma unroll
+        for (int e = 0; e < C; ++e) gate[e] += v[e];
+    }
+    if (g.bias[1]) {
+        load_columns<T, C>(g.bias[1], n, count, whole, v);
+#pragma unroll
+        for (int e = 0; e < C; ++e) up[e] += v[e];
+    }
+    if (g.z[0]) {
+        store_columns<float, C>(g.z[0], m * g.N + n, count, whole, gate);
+        store_columns<float, C>(g.z[1], m * g.N + n, count, whole, up);
+    }
+    act_columns<C>(g.act, gate);
+#pragma unroll
+    for (int e = 0; e < C; ++e) gate[e] *= up[e];
+    store_columns<T, C>(g.c[0], m * g.ldc + n, count, whole, gate);
+}
 // launchers, one object file per element type; 0 or a V2VAE_E* code
 enum { LAYOUT_KK = 0, LAYOUT_KM = 1, LAYOUT_MM = 2 };  // A / B with the contraction (K) or the row index (M) contiguous
+enum { TILE_128 = 0, TILE_64 = 1, TILE_256 = 2 };
+int gemm_direct_bf16(const GemmArgs&, int layout, bool gated, int tile, hipStream_t);
+int gemm_direct_f16(const GemmArgs&, int layout, bool gated, int tile, hipStream_t);
 int gemm_staged_f32(const GemmArgs&, int layout, bool gated, int tile, hipStream_t);
 int gemm_staged_bf16(const GemmArgs&, int layout, bool gated, int tile, hipStream_t);
 int gemm_staged_f16(const GemmArgs&, int layout, bool gated, int tile, hipStream_t);

@@ -119,16 +119,24 @@ static int check_dense(const v2vae_dense* d, bool gated, bool backward, bool res
     return V2VAE_OK;
 }
 
-// How a product M x N x K is cut: tile size and the number of parts of the contraction.
+// How a product M x N x K is cut: tile size and the number of parts of the contraction.  `direct`: 16-bit operands, aligned.
+// The workspace does not know the alignment, so it is laid out for the larger of the two cuts.
 struct Cut { int tile, splits, per; };
-static Cut cut_product(int64_t M, int64_t N, int64_t K, int segs, int batch, int dtype, bool gated) {
+static Cut cut_product(int64_t M, int64_t N, int64_t K, int segs, int batch, int dtype, bool gated, bool direct) {
     const int64_t bk = dtype == V2VAE_F32 ? 32 : 64, steps = ((K + bk - 1) / bk) * segs;
-    const int64_t big = ((M + 127) / 128) * ((N + (gated ? 63 : 127)) / (gated ? 64 : 128)) * batch;
-    const int64_t small = ((M + 63) / 64) * ((N + 63) / 64) * batch;
+    auto tiles_of = [&](int64_t t) { return ((M + t - 1) / t) * ((N * (gated ? 2 : 1) + t - 1) / t) * batch; };
     Cut c;
-    int64_t tiles;
-    if (big >= 256 || (big * (steps / 8) >= 256)) { c.tile = 0; tiles = big; } else { c.tile = 1; tiles = small; }
-    int64_t s = 1;
+    int64_t tiles, s = 1;
+    if (direct && tiles_of(256) >= 200) {
+        c.tile = TILE_256;
+        tiles = tiles_of(256);
+    } else if (tiles_of(128) >= 256 || tiles_of(128) * (steps / 8) >= 256 || direct) {
+        c.tile = TILE_128;
+        tiles = tiles_of(128);
+    } else {
+        c.tile = TILE_64;
+        tiles = ((M + 63) / 64) * ((N + 63) / 64) * batch;
+    }
     if (tiles < 256) {
         s = 512 / (tiles < 1 ? 1 : tiles);
         if (s > steps / 8) s = steps / 8;
@@ -140,8 +148,13 @@ static Cut cut_product(int64_t M, int64_t N, int64_t K, int segs, int batch, int
     if (c.splits < 1) c.splits = 1;
     return c;
 }
-static size_t partial_bytes(const Cut& c, int64_t M, int64_t N, int batch, bool gated) {
-    return c.splits > 1 ? round_up((size_t)c.splits * batch * M * N * (gated ? 2 : 1) * 4) : 0;
+static size_t partial_bytes(int64_t M, int64_t N, int64_t K, int segs, int batch, int dtype, bool gated) {
+    int most = 1;
+    for (int direct = 0; direct < (dtype == V2VAE_F32 ? 1 : 2); ++direct) {
+        const Cut c = cut_product(M, N, K, segs, batch, dtype, gated, direct);
+        if (c.splits > most) most = c.splits;
+    }
+    return most > 1 ? round_up((size_t)most * batch * M * N * (gated ? 2 : 1) * 4) : 0;
 }
 
 static void slope_shape(int64_t M, int64_t N, int V, int* cx, int* gx, int* chunks) {
@@ -175,25 +188,34 @@ static BwdLayout bwd_layout(const v2vae_dense* d, bool gated) {
         if (i < n) o += round_up((size_t)(c1 > c4 ? c1 : c4) * d->out * 4);
     }
     l.prod = o;
-    const Cut cx_ = cut_product(d->rows, d->in, d->out, n, 1, d->dtype, false);
-    const Cut cw = cut_product(d->out, d->in, d->rows, 1, n, d->dtype, false);
-    const size_t a = partial_bytes(cx_, d->rows, d->in, 1, false), b = partial_bytes(cw, d->out, d->in, n, false);
+    const size_t a = partial_bytes(d->rows, d->in, d->out, n, 1, d->dtype, false);
+    const size_t b = partial_bytes(d->out, d->in, d->rows, 1, n, d->dtype, false);
     l.total = o + (a > b ? a : b);
     return l;
 }
 
 static int run_product(GemmArgs& g, int dtype, int layout, bool gated, float* partial, hipStream_t st) {
     if (g.M == 0 || g.N == 0) return V2VAE_OK;
-    const Cut c = cut_product(g.M, g.N, g.K, g.segs, g.batch, dtype, gated);
+    const int e = 16 / elem_bytes(dtype), bytes = elem_bytes(dtype);
+    auto aligned_rows = [&](const void* const p[2], int64_t ld0, int64_t ld1) {
+        return aligned_to(p[0], 16) && (p[1] == nullptr || aligned_to(p[1], 16)) && ld0 % e == 0 && ld1 % e == 0;
+    };
+    const bool rows_a = aligned_rows(g.a, g.lda, g.lda), rows_b = aligned_rows(g.b, g.ldb[0], g.ldb[1]);
+    const bool a_kc = layout != LAYOUT_MM, b_kc = layout == LAYOUT_KK;
+    g.vec_a = a_kc && rows_a && g.K % e == 0;
+    g.vec_b = b_kc && rows_b && g.K % e == 0;
+    auto fit = [&](const void* p, int64_t ld) { return aligned_to(p, 16) && (p == nullptr || ld % e == 0); };
+    g.vec_c = g.N % 8 == 0 && fit(g.c[0], g.ldc) && fit(g.c[1], g.ldc) && fit(g.bias[0], 0) && fit(g.bias[1], 0) && fit(g.residual, g.ldr) &&
+              fit(g.z[0], 0) && fit(g.z[1], 0);
+    // straight to LDS: 16-bit, every row of both operands whole 16-byte pieces, offsets inside a tile below 2^31, one stride
+    const int64_t ld_max = g.lda > g.ldb[0] ? (g.lda > g.ldb[1] ? g.lda : g.ldb[1]) : (g.ldb[0] > g.ldb[1] ? g.ldb[0] : g.ldb[1]);
+    const bool direct = dtype != V2VAE_F32 && (a_kc ? g.vec_a : rows_a && g.M % 8 == 0) && (b_kc ? g.vec_b : rows_b && g.N % 8 == 0) &&
+                        ld_max <= (1 << 21) && (gated || g.ldb[0] == g.ldb[1]);
+    const Cut c = cut_product(g.M, g.N, g.K, g.segs, g.batch, dtype, gated, direct);
     g.splits = c.splits;
     g.steps_per_split = c.per;
     g.partial = c.splits > 1 ? partial : nullptr;
-    const int e = 16 / elem_bytes(dtype), bytes = elem_bytes(dtype);
-    auto vec = [&](const void* p0, const void* p1, int64_t ld0, int64_t ld1) {
-        return aligned_to(p0, 16) && (p1 == nullptr || aligned_to(p1, 16)) && (ld0 * bytes) % 16 == 0 && (ld1 * bytes) % 16 == 0 && g.K % e == 0;
-    };
-    g.vec_a = layout != LAYOUT_MM && vec(g.a[0], g.a[1], g.lda, g.lda);
-    g.vec_b = layout == LAYOUT_KK && vec(g.b[0], g.b[1], g.ldb[0], g.ldb[1]);
+    if (direct) return dtype == V2VAE_BF16 ? gemm_direct_bf16(g, layout, gated, c.tile, st) : gemm_direct_f16(g, layout, gated, c.tile, st);
     if (dtype == V2VAE_F32) return gemm_staged_f32(g, layout, gated, c.tile, st);
     if (dtype == V2VAE_BF16) return gemm_staged_bf16(g, layout, gated, c.tile, st);
     return gemm_staged_f16(g, layout, gated, c.tile, st);
@@ -335,14 +357,14 @@ size_t v2vae_linear_workspace_bytes(const v2vae_dense* d, int backward) {
     if (check_dense(d, false, backward != 0, false) != V2VAE_OK) return 0;
     if (backward) return bwd_layout(d, false).total;
     if (d->rows <= ROWS_MAX) return 0;
-    return partial_bytes(cut_product(d->rows, d->out, d->in, 1, 1, d->dtype, false), d->rows, d->out, 1, false);
+    return partial_bytes(d->rows, d->out, d->in, 1, 1, d->dtype, false);
 }
 
 size_t v2vae_gated_workspace_bytes(const v2vae_dense* d, int backward) {
     if (check_dense(d, true, backward != 0, false) != V2VAE_OK) return 0;
     if (backward) return bwd_layout(d, true).total;
     if (d->rows <= ROWS_MAX) return 0;
-    return partial_bytes(cut_product(d->rows, d->out, d->in, 1, 1, d->dtype, true), d->rows, d->out, 1, true);
+    return partial_bytes(d->rows, d->out, d->in, 1, 1, d->dtype, true);
 }
 
 int v2vae_linear_fwd(const v2vae_dense* d, const void* x, const void* w, const void* bias, const void* residual, void* y, float* z,

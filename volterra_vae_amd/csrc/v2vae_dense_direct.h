@@ -1,0 +1,211 @@
+// Matrix product of the dense layers for 16-bit operands whose rows are 16-byte aligned: tiles go from memory to LDS directly.
+//
+// Mathematics and arguments as in v2vae_dense_gemm.h.  WM x WN waves own a tile of 32 TM WM x 32 TN WN outputs; a contraction step
+// is 64 elements, two steps' tiles live in LDS, and while one is multiplied the loads of the next (global_load_lds, 16 bytes a
+// lane, no registers) are in flight: one barrier a step.  Such a load writes its 64 pieces in lane order, so the order of pieces
+// in LDS is chosen by which piece a lane fetches:
+//  * contraction contiguous: a row is 8 pieces; row r holds piece p at position p ^ (r % 8), and the 16-byte reads of a
+//    fragment (32 rows, one piece each) spread over all banks;
+//  * rows contiguous: a contraction index is a line of 32 TM WM (or TN WN) elements, read as a transposed fragment by
+//    ds_read_b64_tr_b16 (16 lanes read 4 k x 16 rows and receive 4 k of one row each).  Line k holds its 64-byte blocks at
+//    position b ^ (k % 4 + 4 (k / 8 % 2)): the eight lines that one instruction reads then fall on different banks.
+// Rows beyond the matrix repeat its last row (or last 16 bytes): their products are not stored.  The last step of a contraction
+// that is not a multiple of 64 takes what lies beyond from a page of zeros.
+#ifndef V2VAE_DENSE_DIRECT_H
+#define V2VAE_DENSE_DIRECT_H
+#include "v2vae_dense_gemm.h"
+
+namespace v2vae {
+
+__device__ __align__(16) const unsigned g_zero_piece[4] = {0, 0, 0, 0};
+
+// 64 lanes' pieces of 16 bytes from base + off to LDS at lds + 16 lane; not tracked by the compiler, wait_tile() waits for them
+__device__ __forceinline__ void load_to_lds(const void* base, unsigned off, unsigned lds) {
+    lds = __builtin_amdgcn_readfirstlane(lds);
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
+}
+__device__ __forceinline__ void load_to_lds(const void* at, unsigned lds) {
+    lds = __builtin_amdgcn_readfirstlane(lds);
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(at), "s"(lds) : "memory", "m0");
+}
+// this wave's loads have landed and its LDS reads are done, then all waves'
+__device__ __forceinline__ void wait_tile() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+template <typename V> __device__ __forceinline__ V uniform64(V p) {
+    const uint64_t u = (uint64_t)p;
+    const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)u), hi = __builtin_amdgcn_readfirstlane((unsigned)(u >> 32));
+    return (V)(((uint64_t)hi << 32) | lo);
+}
+
+// One operand: ROWS rows of the tile, loaded by NW waves.
+template <typename T, int ROWS, int NW, bool KC, bool GATED> struct Tile {
+    static constexpr int LOADS = ROWS / 8 / NW, BYTES = ROWS * 128;
+    unsigned off[LOADS];  // byte offset of this lane's piece from the tile's corner
+    // corner: first row of the tile; R rows (features) in all
+    __device__ __forceinline__ void init(int lane, int wave, int64_t ld, int first, int R, const int64_t* ld2) {
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            const int i = j * NW + wave;
+            if constexpr (KC) {
+                const int r = i * 8 + (lane >> 3), piece = (lane & 7) ^ (r & 7);
+                int row = GATED ? (r >> 6) * 32 + (r & 31) : r;
+                row = first + row < R ? row : R - 1 - first;
+                off[j] = (unsigned)(row * (GATED ? ld2[(r >> 5) & 1] : ld) + piece * 8) * 2u;
+            } else {
+                const int k = (i * 64 + lane) / (ROWS / 8), p = (i * 64 + lane) % (ROWS / 8);
+                const int piece = p ^ (4 * ((k & 3) | (((k >> 3) & 1) << 2)) % (ROWS / 8));
+                const int row = first + piece * 8 < R ? piece * 8 : R - 8 - first;
+                off[j] = (unsigned)(k * ld + row) * 2u;
+            }
+        }
+    }
+    // base0 (base1): corner at contraction index k0; left = contraction elements from k0 on
+    __device__ __forceinline__ void fetch(const char* base0, const char* base1, int left, int lane, int wave, unsigned lds) const {
+        if (left >= 64) {
+#pragma unroll
+            for (int j = 0; j < LOADS; ++j) {
+                const int i = j * NW + wave;
+                const char* b = GATED && (((i * 8) >> 5) & 1) ? base1 : base0;
+                load_to_lds(b, off[j], lds + i * 1024);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < LOADS; ++j) {
+                const int i = j * NW + wave;
+                const char* b = GATED && (((i * 8) >> 5) & 1) ? base1 : base0;
+                int k;
+                if constexpr (KC) k = ((lane & 7) ^ ((i * 8 + (lane >> 3)) & 7)) * 8; else k = (i * 64 + lane) / (ROWS / 8);
+                load_to_lds(k < left ? (const void*)(b + off[j]) : (const void*)g_zero_piece, lds + i * 1024);
+            }
+        }
+    }
+};
+
+template <typename T, int WM, int WN, int TM, int TN, bool AKC, bool BKC, bool GATED>
+__global__ __launch_bounds__(64 * WM * WN, (WM * WN) / 4) void k_gemm_direct(GemmArgs g) {
+    typedef typename Elem<T>::frag frag;
+    typedef __attribute__((ext_vector_type(4))) short s16x4;
+    constexpr int NW = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, STAGE = (BM + BN) * 128;
+    static_assert(!GATED || TN == 2, "a gated wave holds one gate and one up block");
+    static_assert(NW * EPI_BYTES<TN> <= 2 * STAGE, "the epilogue's rows fit the tiles' memory");
+    __shared__ __align__(1024) char lds[2 * STAGE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
+    const int out_bn = GATED ? BN / 2 : BN;
+    const int tiles_m = (g.M + BM - 1) / BM, tiles_n = (g.N + out_bn - 1) / out_bn;
+    int tm, tn;
+    tile_of(blockIdx.x, tiles_m, tiles_n, &tm, &tn);
+    const int split = blockIdx.y, bat = blockIdx.z, m0 = tm * BM, n0 = tn * out_bn;
+    const int steps_seg = (g.K + 63) / 64, steps = steps_seg * g.segs;
+    const int s_lo = split * g.steps_per_split, s_hi = s_lo + g.steps_per_split < steps ? s_lo + g.steps_per_split : steps;
+    const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+
+    Tile<T, BM, NW, AKC, false> ta;
+    Tile<T, BN, NW, BKC, GATED> tb;
+    ta.init(lane, wave, g.lda, m0, g.M, nullptr);
+    tb.init(lane, wave, g.ldb[bat], n0, g.N, g.ldb);
+    auto fetch = [&](int s, int buf) {
+        const int seg = s >= steps_seg ? 1 : 0, k0 = (s - seg * steps_seg) * 64, sel = seg | bat, left = g.K - k0;
+        const char* a = (const char*)g.a[sel] + ((AKC ? (int64_t)m0 * g.lda + k0 : (int64_t)k0 * g.lda + m0) * 2);
+        const char *b0, *b1 = nullptr;
+        if constexpr (GATED) {
+            b0 = (const char*)g.b[0] + ((int64_t)n0 * g.ldb[0] + k0) * 2;
+            b1 = uniform64((const char*)g.b[1] + ((int64_t)n0 * g.ldb[1] + k0) * 2);
+        } else {
+            b0 = (const char*)g.b[sel] + ((BKC ? (int64_t)n0 * g.ldb[sel] + k0 : (int64_t)k0 * g.ldb[sel] + n0) * 2);
+        }
+        ta.fetch(uniform64(a), nullptr, left, lane, wave, lds0 + buf * STAGE);
+        tb.fetch(uniform64(b0), b1, left, lane, wave, lds0 + buf * STAGE + BM * 128);
+    };
+
+    f32x16 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+
+    // LDS byte offsets of this lane's fragments.  Contraction contiguous: row base + piece kk * 2 + lane / 32, one offset per kk.
+    // Rows contiguous: 4 k x 16 rows per 16 lanes; one offset per 32-row block, kk and the two halves as constants.
+    constexpr int OA = AKC ? 4 : TM, OB = BKC ? 4 : TN;
+    unsigned oa[OA], ob[OB];
+    const int g16 = lane >> 4, i16 = lane & 15, ks = (i16 >> 2) | ((g16 >> 1) << 2);
+    auto mn_offset = [&](int block, int rows) {
+        const int k = (g16 >> 1) * 8 + (i16 >> 2);
+        return (unsigned)(k * rows * 2 + (((block ^ ks) % (rows / 32)) * 64) + (g16 & 1) * 32 + (i16 & 3) * 8);
+    };
+#pragma unroll
+    for (int q = 0; q < OA; ++q) {
+        if constexpr (AKC) oa[q] = (unsigned)((wm * 32 * TM + (lane & 31)) * 128 + (((q * 2 + (lane >> 5)) ^ (lane & 7)) * 16));
+        else oa[q] = mn_offset(wm * TM + q, BM);
+    }
+#pragma unroll
+    for (int q = 0; q < OB; ++q) {
+        if constexpr (BKC) ob[q] = (unsigned)((wn * 32 * TN + (lane & 31)) * 128 + (((q * 2 + (lane >> 5)) ^ (lane & 7)) * 16));
+        else ob[q] = mn_offset(wn * TN + q, BN);
+    }
+    auto frag_mn = [&](unsigned at, int rows, int kk) {
+        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(at + kk * 32 * rows));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(at + kk * 32 * rows + 8 * rows));
+        union { s16x4 h[2]; frag f; } u;
+        u.h[0] = lo;
+        u.h[1] = hi;
+        return u.f;
+    };
+    typedef __attribute__((address_space(3))) frag lds_frag;
+
+    if (s_lo < s_hi) fetch(s_lo, 0);
+    for (int s = s_lo; s < s_hi; ++s) {
+        const int buf = (s - s_lo) & 1;
+        wait_tile();
+        if (s + 1 < s_hi) fetch(s + 1, buf ^ 1);
+        const unsigned la = lds0 + buf * STAGE, lb = la + BM * 128;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+            frag a[TM], b[TN];
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                if constexpr (AKC) a[i] = *(const lds_frag*)(uintptr_t)(la + oa[kk] + i * 4096);
+                else a[i] = frag_mn(la + oa[i], BM, kk);
+            }
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                if constexpr (BKC) b[j] = *(const lds_frag*)(uintptr_t)(lb + ob[kk] + j * 4096);
+                else b[j] = frag_mn(lb + ob[j], BN, kk);
+            }
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = mma32(b[j], a[i], acc[i][j]);
+        }
+    }
+
+    wait_tile();  // LDS is free
+    float* const part = g.partial ? g.partial + ((int64_t)bat * g.splits + split) * ((int64_t)g.M * (GATED ? 2 : 1) * g.N) : nullptr;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+        finish_block<T, TN, GATED>(g, acc[i], lds + wave * EPI_BYTES<TN>, lane, m0 + (wm * TM + i) * 32, n0 + wn * (GATED ? 32 : 32 * TN), part, bat);
+}
+
+template <typename T, int WM, int WN, int TM, int TN, bool AKC, bool BKC, bool GATED> void launch_direct(const GemmArgs& g, hipStream_t st) {
+    constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN / (GATED ? 2 : 1);
+    const int64_t tiles = (int64_t)((g.M + BM - 1) / BM) * ((g.N + BN - 1) / BN);
+    hipLaunchKernelGGL((k_gemm_direct<T, WM, WN, TM, TN, AKC, BKC, GATED>), dim3((unsigned)tiles, g.splits, g.batch), dim3(64 * WM * WN), 0,
+                       st, g);
+    if (g.partial) launch_join<T, GATED>(g, st);
+}
+template <typename T, bool AKC, bool BKC, bool GATED> void pick_direct(const GemmArgs& g, int tile, hipStream_t st) {
+    if (tile == TILE_256) launch_direct<T, 2, 4, 4, 2, AKC, BKC, GATED>(g, st);
+    else launch_direct<T, 2, 2, 2, 2, AKC, BKC, GATED>(g, st);
+}
+template <typename T> int gemm_direct(const GemmArgs& g, int layout, bool gated, int tile, hipStream_t st) {
+    if (gated) pick_direct<T, true, true, true>(g, tile, st);
+    else if (layout == LAYOUT_KK) pick_direct<T, true, true, false>(g, tile, st);
+    else if (layout == LAYOUT_KM) pick_direct<T, true, false, false>(g, tile, st);
+    else pick_direct<T, false, false, false>(g, tile, st);
+    return dense_launch_error("dense matrix product");
+}
+
+}  // namespace v2vae
+#endif

@@ -1,0 +1,8 @@
+// Matrix product of the dense layers straight from memory to LDS, f16 operands.
+#include "v2vae_dense_direct.h"
+
+namespace v2vae {
+int gemm_direct_f16(const GemmArgs& g, int layout, bool gated, int tile, hipStream_t st) {
+    return gemm_direct<f16_t>(g, layout, gated, tile, st);
+}
+}  // namespace v2vae

@@ -125,12 +125,61 @@ __device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int* t
     *tn = in / rows;
 }
 
+// The sums of one 32-row block of a wave, 32 TN columns, from matrix registers to memory.  The operands enter the matrix
+// instruction swapped, so a lane holds row lane % 32 and columns 32 j + 8 q + 4 (lane / 32) ... + 3.  They go through the wave's
+// own piece of LDS to become rows again: eight consecutive columns a lane, whole cache lines per row for every load and store of
+// the epilogue, and its code (bias, activation, residual) exists once per block instead of once per register.
+template <int TN> constexpr int EPI_ROWB = 32 * TN * 4 + 16;
+template <int TN> constexpr int EPI_BYTES = 32 * EPI_ROWB<TN>;
+template <typename T, int TN, bool GATED>
+__device__ __forceinline__ void finish_block(const GemmArgs& g, const f32x16 (&acc)[TN], char* lds, int lane, int m0, int n0, float* part, int bat) {
+    constexpr int ROWB = EPI_ROWB<TN>, COLS = GATED ? 32 : 32 * TN, PER = COLS / 8, ROWS = 64 / PER;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<f32x4*>(lds + (lane & 31) * ROWB + (32 * j + 8 * q + 4 * (lane >> 5)) * 4) =
+                f32x4{acc[j][4 * q], acc[j][4 * q + 1], acc[j][4 * q + 2], acc[j][4 * q + 3]};
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const int c = (lane % PER) * 8, n = n0 + c;
+    const bool whole = g.vec_c;  // N is a multiple of 8 then
+#pragma unroll 1
+    for (int r = lane / PER; r < 32; r += ROWS) {
+        const int64_t m = m0 + r;
+        if (m >= g.M || n >= g.N) continue;
+        float s[8], u[8];
+        const f32x4* p = reinterpret_cast<const f32x4*>(lds + r * ROWB + c * 4);
+        *reinterpret_cast<f32x4*>(s) = p[0];
+        *reinterpret_cast<f32x4*>(s + 4) = p[1];
+        if constexpr (GATED) {
+            const f32x4* p2 = reinterpret_cast<const f32x4*>(lds + r * ROWB + (c + 32) * 4);
+            *reinterpret_cast<f32x4*>(u) = p2[0];
+            *reinterpret_cast<f32x4*>(u + 4) = p2[1];
+        }
+        if (part) {
+            if constexpr (GATED) {
+                store_columns<float, 8>(part, m * 2 * g.N + n, g.N - n, whole, s);
+                store_columns<float, 8>(part, m * 2 * g.N + g.N + n, g.N - n, whole, u);
+            } else {
+                store_columns<float, 8>(part, m * g.N + n, g.N - n, whole, s);
+            }
+        } else if constexpr (GATED) {
+            finish_gated<T, 8>(g, m, n, s, u, whole);
+        } else {
+            finish_value<T, 8>(g, m, n, s, bat, whole);
+        }
+    }
+}
+
 template <typename T, int TM, int TN, bool AKC, bool BKC, bool GATED>
 __global__ __launch_bounds__(256, 2) void k_gemm_staged(GemmArgs g) {
     constexpr int NP = Elem<T>::NP, BK = Elem<T>::BK, ROWB = BK * 2 + 16, BM = 64 * TM, BN = 64 * TN;
     static_assert(!GATED || TN == 2, "a gated wave holds one gate and one up block");
     typedef typename Elem<T>::frag frag;
-    __shared__ __align__(16) char lds[NP * (BM + BN) * ROWB];
+    constexpr int TILES = NP * (BM + BN) * ROWB, EPI = 4 * EPI_BYTES<TN>;
+    __shared__ __align__(16) char lds[TILES > EPI ? TILES : EPI];
     char* const lds_a = lds;
     char* const lds_b = lds + NP * BM * ROWB;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
@@ -203,7 +252,7 @@ __global__ __launch_bounds__(256, 2) void k_gemm_staged(GemmArgs g) {
 #pragma unroll
                     for (int i = 0; i < TM; ++i)
 #pragma unroll
-                        for (int j = 0; j < TN; ++j) acc[i][j] = mma32(a[i][p], b[j][sum - p], acc[i][j]);
+                        for (int j = 0; j < TN; ++j) acc[i][j] = mma32(b[j][sum - p], a[i][p], acc[i][j]);
         }
         __syncthreads();
         if (s + 1 < s_hi) {
@@ -213,81 +262,63 @@ __global__ __launch_bounds__(256, 2) void k_gemm_staged(GemmArgs g) {
         __syncthreads();
     }
 
-    // lane: column lane % 32 of a block, rows 8 (e / 4) + 4 (lane / 32) + e % 4
     float* const part = g.partial ? g.partial + ((int64_t)bat * g.splits + split) * ((int64_t)g.M * (GATED ? 2 : 1) * g.N) : nullptr;
 #pragma unroll
     for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const int m = m0 + (wm * TM + i) * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-            if (m >= g.M) continue;
-            if constexpr (GATED) {
-                const int n = n0 + wn * 32 + (lane & 31);
-                if (n >= g.N) continue;
-                if (part) {
-                    part[(int64_t)m * 2 * g.N + n] = acc[i][0][e];
-                    part[(int64_t)m * 2 * g.N + g.N + n] = acc[i][1][e];
-                } else {
-                    finish_gated<T>(g, m, n, acc[i][0][e], acc[i][1][e]);
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < TN; ++j) {
-                    const int n = n0 + (wn * TN + j) * 32 + (lane & 31);
-                    if (n >= g.N) continue;
-                    if (part) part[(int64_t)m * g.N + n] = acc[i][j][e];
-                    else if (bat == 0) finish_value<T>(g, m, n, acc[i][j][e]);
-                    else ((T*)g.c[1])[(int64_t)m * g.ldc + n] = (T)acc[i][j][e];
-                }
-            }
-        }
+        finish_block<T, TN, GATED>(g, acc[i], lds + wave * EPI_BYTES<TN>, lane, m0 + (wm * TM + i) * 32, n0 + wn * (GATED ? 32 : 32 * TN), part, bat);
 }
 
-// Sums of a split contraction, added in the order of the splits, and the rest of the epilogue.
-template <typename T, bool GATED> __global__ __launch_bounds__(256) void k_gemm_join(GemmArgs g) {
-    const int64_t per = (int64_t)g.M * g.N * (GATED ? 2 : 1), count = (int64_t)g.M * g.N;
+// Sums of a split contraction, added in the order of the splits, and the rest of the epilogue; C columns a thread.
+template <typename T, int C, bool GATED> __global__ __launch_bounds__(256) void k_gemm_join(GemmArgs g) {
+    const int64_t per = (int64_t)g.M * g.N * (GATED ? 2 : 1), count = (int64_t)g.M * (g.N / C);
     const int bat = blockIdx.y;
     const float* base = g.partial + bat * (int64_t)g.splits * per;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
-        const int64_t m = i / g.N;
-        const int n = (int)(i - m * g.N);
-        if constexpr (GATED) {
-            float s0 = 0.f, s1 = 0.f;
-            for (int s = 0; s < g.splits; ++s) {
-                s0 += base[s * per + m * 2 * g.N + n];
-                s1 += base[s * per + m * 2 * g.N + g.N + n];
+        const int64_t m = i / (g.N / C);
+        const int n = (int)(i - m * (g.N / C)) * C;
+        float s[C], u[C], v[C];
+#pragma unroll
+        for (int e = 0; e < C; ++e) s[e] = u[e] = 0.f;
+#pragma unroll 4
+        for (int p = 0; p < g.splits; ++p) {
+            load_columns<float, C>(base, p * per + m * (GATED ? 2 : 1) * g.N + n, C, true, v);
+#pragma unroll
+            for (int e = 0; e < C; ++e) s[e] += v[e];
+            if constexpr (GATED) {
+                load_columns<float, C>(base, p * per + m * 2 * g.N + g.N + n, C, true, v);
+#pragma unroll
+                for (int e = 0; e < C; ++e) u[e] += v[e];
             }
-            finish_gated<T>(g, m, n, s0, s1);
-        } else {
-            float s0 = 0.f;
-            for (int s = 0; s < g.splits; ++s) s0 += base[s * per + i];
-            if (bat == 0) finish_value<T>(g, m, n, s0);
-            else ((T*)g.c[1])[m * g.ldc + n] = (T)s0;
         }
+        if constexpr (GATED) finish_gated<T, C>(g, m, n, s, u, true); else finish_value<T, C>(g, m, n, s, bat, true);
     }
+}
+
+template <typename T, bool GATED> void launch_join(const GemmArgs& g, hipStream_t st) {
+    const int c = g.vec_c ? 4 : 1;
+    int64_t blocks = ((int64_t)g.M * (g.N / c) + 255) / 256;
+    if (blocks > 4096) blocks = 4096;
+    if (c == 4) hipLaunchKernelGGL((k_gemm_join<T, 4, GATED>), dim3((unsigned)blocks, g.batch), dim3(256), 0, st, g);
+    else hipLaunchKernelGGL((k_gemm_join<T, 1, GATED>), dim3((unsigned)blocks, g.batch), dim3(256), 0, st, g);
 }
 
 template <typename T, int TM, int TN, bool AKC, bool BKC, bool GATED> void launch_staged(const GemmArgs& g, hipStream_t st) {
     const int bn = GATED ? 32 * TN : 64 * TN;
     const int64_t tiles = (int64_t)((g.M + 64 * TM - 1) / (64 * TM)) * ((g.N + bn - 1) / bn);
     hipLaunchKernelGGL((k_gemm_staged<T, TM, TN, AKC, BKC, GATED>), dim3((unsigned)tiles, g.splits, g.batch), dim3(256), 0, st, g);
-    if (g.partial) {
-        int64_t blocks = ((int64_t)g.M * g.N + 255) / 256;
-        if (blocks > 4096) blocks = 4096;
-        hipLaunchKernelGGL((k_gemm_join<T, GATED>), dim3((unsigned)blocks, g.batch), dim3(256), 0, st, g);
-    }
+    if (g.partial) launch_join<T, GATED>(g, st);
 }
 
-// tile: 0 = 128 x 128, 1 = 64 x 64 (gated: 64 rows x 64 features)
+// tile: TILE_128, or TILE_64 (gated: 64 rows x 64 features)
 template <typename T> int gemm_staged(const GemmArgs& g, int layout, bool gated, int tile, hipStream_t st) {
     if (gated) {
-        if (tile == 0) launch_staged<T, 2, 2, true, true, true>(g, st); else launch_staged<T, 1, 2, true, true, true>(g, st);
+        if (tile == TILE_128) launch_staged<T, 2, 2, true, true, true>(g, st); else launch_staged<T, 1, 2, true, true, true>(g, st);
     } else if (layout == LAYOUT_KK) {
-        if (tile == 0) launch_staged<T, 2, 2, true, true, false>(g, st); else launch_staged<T, 1, 1, true, true, false>(g, st);
+        if (tile == TILE_128) launch_staged<T, 2, 2, true, true, false>(g, st); else launch_staged<T, 1, 1, true, true, false>(g, st);
     } else if (layout == LAYOUT_KM) {
-        if (tile == 0) launch_staged<T, 2, 2, true, false, false>(g, st); else launch_staged<T, 1, 1, true, false, false>(g, st);
+        if (tile == TILE_128) launch_staged<T, 2, 2, true, false, false>(g, st); else launch_staged<T, 1, 1, true, false, false>(g, st);
     } else {
-        if (tile == 0) launch_staged<T, 2, 2, false, false, false>(g, st); else launch_staged<T, 1, 1, false, false, false>(g, st);
+        if (tile == TILE_128) launch_staged<T, 2, 2, false, false, false>(g, st); else launch_staged<T, 1, 1, false, false, false>(g, st);
     }
     return dense_launch_error("dense matrix product");
 }

@@ -67,7 +67,13 @@ template <typename T, int MR, int NR, bool GATED> __global__ __launch_bounds__(2
         const int m = i / FT, f = i % FT, n = n0 + f;
         if (m >= g.M || n >= g.N) continue;
         auto total = [&](int r) { return (s_sum[0][m * NR + r] + s_sum[1][m * NR + r]) + (s_sum[2][m * NR + r] + s_sum[3][m * NR + r]); };
-        if constexpr (GATED) finish_gated<T>(g, m, n, total(2 * f), total(2 * f + 1)); else finish_value<T>(g, m, n, total(f));
+        float s0 = total(GATED ? 2 * f : f);
+        if constexpr (GATED) {
+            float s1 = total(2 * f + 1);
+            finish_gated<T, 1>(g, m, n, &s0, &s1, true);
+        } else {
+            finish_value<T, 1>(g, m, n, &s0, 0, true);
+        }
     }
 }
 
