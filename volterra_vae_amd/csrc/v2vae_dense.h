@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/v2vae_hip.h"
 
 namespace v2vae {
@@ -23,36 +25,97 @@ template <typename T> struct Vec16 {
     union { u32x4 raw; T e[N]; };
 };
 
-// act(z); the kinds are V2VAE_ACT_*.  exp, erfc and tanh are the device library's float functions
-// (erfc rather than 1 + erf: no cancellation where z is far below zero).
-__device__ __forceinline__ float act_value(int kind, float z) {
-    switch (kind) {
-        case V2VAE_ACT_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
-        case V2VAE_ACT_SILU: return z / (1.f + expf(-z));
-        case V2VAE_ACT_GELU: return 0.5f * z * erfcf(z * -0.70710678118654752f);
-        case V2VAE_ACT_TANH: return tanhf(z);
-        default: return z;
+template <typename T> struct Elem;
+template <> struct Elem<float> { static constexpr int NP = 3, BK = 32; typedef bf16x8 frag; };
+template <> struct Elem<bf16_t> { static constexpr int NP = 1, BK = 64; typedef bf16x8 frag; };
+template <> struct Elem<f16_t> { static constexpr int NP = 1, BK = 64; typedef f16x8 frag; };
+
+__device__ __forceinline__ f32x16 mma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mma32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+// two floats -> their three bf16 pieces, each pair packed in a word
+__device__ __forceinline__ void split_pair(float x0, float x1, unsigned p[3]) {
+    typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        const bf16x2 h = {(__bf16)x0, (__bf16)x1};
+        const unsigned u = __builtin_bit_cast(unsigned, h);
+        p[i] = u;
+        x0 -= __uint_as_float(u << 16);
+        x1 -= __uint_as_float(u & 0xFFFF0000u);
     }
 }
-// act(z) and act'(z).  For |z| beyond 80 both soft activations are their asymptotes to the last bit of a float; the clamp keeps
-// z (1 - s) and z exp(-z^2 / 2) from becoming inf * 0 there.
-__device__ __forceinline__ float act_slope(int kind, float z, float* value) {
-    const float zc = fminf(fmaxf(z, -80.f), 80.f);
+
+// exp(x + lo) for |lo| far below |x|, x <= 88: x log2(e) is carried as a float and its remainder, so the result is off by about
+// two units however large |x| is; below exp(-87) it is 0.
+__device__ __forceinline__ float exp_with_rest(float x, float lo) {
+    constexpr float L = 1.44269502f, L_LO = 1.92596299e-8f, LN2 = 0.693147181f;
+    const float t = x * L;
+    const float r = fmaf(lo, L, fmaf(x, L_LO, fmaf(x, L, -t)));
+    const float e = __builtin_amdgcn_exp2f(t);
+    return fmaf(e, r * LN2, e);
+}
+// 1 / d to half a unit or so: the hardware's reciprocal and one Newton step (0 where it is subnormal)
+__device__ __forceinline__ float reciprocal(float d) {
+    const float r = __builtin_amdgcn_rcpf(d);
+    return fmaf(r, fmaf(-d, r, 1.f), r);
+}
+// Phi(z) and exp(-z^2 / 2), |z| <= 80.  With x = |z| / sqrt 2 and t = 1 / (1 + 0.42 x), erfc(x) = exp(-x^2) t P(t); P is a
+// least-squares fit of erfc(x) exp(x^2) / t in relative error (2.3e-9 at its worst over all x >= 0).  Both halves of the tail keep
+// their relative accuracy: nothing is subtracted for z < 0.
+__device__ __forceinline__ float normal_cdf(float z, float* gauss) {
+    const float q = z * z, rest = fmaf(z, z, -q);
+    const float e = exp_with_rest(-0.5f * q, -0.5f * rest);
+    const float t = reciprocal(fmaf(0.42f * 0.70710678118654752f, fabsf(z), 1.f));
+    float p = -0.04113757392246231f;
+    p = fmaf(p, t, 0.23070600708015587f);
+    p = fmaf(p, t, -0.4866447164102488f);
+    p = fmaf(p, t, 0.43715272615373146f);
+    p = fmaf(p, t, -0.19733165247973258f);
+    p = fmaf(p, t, 0.21373484799346232f);
+    p = fmaf(p, t, 0.15004025649345917f);
+    p = fmaf(p, t, 0.21989457161457882f);
+    p = fmaf(p, t, 0.23661220944910594f);
+    p = fmaf(p, t, 0.2369733217454039f);
+    const float half = 0.5f * (e * (t * p));
+    *gauss = e;
+    return z < 0.f ? half : 1.f - half;
+}
+
+// act(z) and act'(z); the kinds are V2VAE_ACT_*.  For |z| beyond 80 the soft activations are their asymptotes to the last bit of
+// a float; the clamp keeps z (1 - s) and z exp(-z^2 / 2) from becoming inf * 0 there.  A NaN stays one.
+template <bool SLOPE> __device__ __forceinline__ float act_both(int kind, float z, float* slope) {
     switch (kind) {
-        case V2VAE_ACT_RELU: *value = z > 0.f ? z : (z != z ? z : 0.f); return z > 0.f ? 1.f : (z != z ? z : 0.f);
+        case V2VAE_ACT_RELU:
+            if constexpr (SLOPE) *slope = z > 0.f ? 1.f : (z != z ? z : 0.f);
+            return z > 0.f ? z : (z != z ? z : 0.f);
         case V2VAE_ACT_SILU: {
-            const float s = 1.f / (1.f + expf(-zc));
-            *value = z != z ? z : (z < -80.f ? 0.f : z * s);
-            return z != z ? z : s * (1.f + zc * (1.f - s));
+            const float zc = fminf(fmaxf(z, -80.f), 80.f), e = exp_with_rest(-zc, 0.f), s = reciprocal(1.f + e);
+            if constexpr (SLOPE) *slope = z != z ? z : s * fmaf(zc, e * s, 1.f);
+            return z != z ? z : (z < -80.f ? 0.f : z * s);
         }
         case V2VAE_ACT_GELU: {
-            const float phi = 0.5f * erfcf(zc * -0.70710678118654752f);
-            *value = z != z ? z : (z < -80.f ? 0.f : z * phi);
-            return z != z ? z : phi + zc * (0.39894228040143268f * expf(-0.5f * zc * zc));
+            const float zc = fminf(fmaxf(z, -80.f), 80.f);
+            float gauss;
+            const float phi = normal_cdf(zc, &gauss);
+            if constexpr (SLOPE) *slope = z != z ? z : fmaf(zc, 0.39894228040143268f * gauss, phi);
+            return z != z ? z : (z < -80.f ? 0.f : z * phi);
         }
-        case V2VAE_ACT_TANH: { const float t = tanhf(z); *value = t; return 1.f - t * t; }
-        default: *value = z; return 1.f;
+        case V2VAE_ACT_TANH: {
+            const float t = tanhf(z);
+            if constexpr (SLOPE) *slope = fmaf(-t, t, 1.f);
+            return t;
+        }
+        default:
+            if constexpr (SLOPE) *slope = 1.f;
+            return z;
     }
+}
+__device__ __forceinline__ float act_value(int kind, float z) { return act_both<false>(kind, z, nullptr); }
+__device__ __forceinline__ float act_slope(int kind, float z, float* value) {
+    float slope;
+    *value = act_both<true>(kind, z, &slope);
+    return slope;
 }
 
 // One product D[m][n] = sum over segments and k of A(m, k) B(n, k), with what happens to D afterwards.
@@ -101,8 +164,17 @@ template <typename T, int C> __device__ __forceinline__ void store_columns(void*
 }
 template <int C> __device__ __forceinline__ void act_columns(int kind, float v[C]) {
     if (kind == V2VAE_ACT_NONE) return;
+    // one switch for all columns
+    auto all = [&](auto k) {
 #pragma unroll
-    for (int e = 0; e < C; ++e) v[e] = act_value(kind, v[e]);
+        for (int e = 0; e < C; ++e) v[e] = act_value(decltype(k)::value, v[e]);
+    };
+    switch (kind) {
+        case V2VAE_ACT_RELU: all(std::integral_constant<int, V2VAE_ACT_RELU>()); break;
+        case V2VAE_ACT_SILU: all(std::integral_constant<int, V2VAE_ACT_SILU>()); break;
+        case V2VAE_ACT_GELU: all(std::integral_constant<int, V2VAE_ACT_GELU>()); break;
+        case V2VAE_ACT_TANH: all(std::integral_constant<int, V2VAE_ACT_TANH>()); break;
+    }
 }
 template <typename T, int C> __device__ __forceinline__ void finish_value(const GemmArgs& g, int64_t m, int n, float s[C], int bat, bool whole) {
     const int count = g.N - n;

@@ -16,10 +16,10 @@ struct SlopeArgs {
     void* d[2];         // dz [M][N] (NULL: only the sums)
     float* part[2];     // [chunks][N] (NULL: no sums)
     int64_t M, rows_per_chunk;
-    int N, act, cx;     // cx threads along the columns, 256 / cx along the rows
+    int N, cx;          // cx threads along the columns, 256 / cx along the rows
 };
 
-template <typename T, int V, bool GATED> __global__ __launch_bounds__(256) void k_dense_slopes(SlopeArgs a) {
+template <typename T, int V, int ACT, bool GATED> __global__ __launch_bounds__(256) void k_dense_slopes(SlopeArgs a) {
     struct alignas(V * sizeof(T)) TV { T e[V]; };
     struct alignas(V * 4) FV { float e[V]; };
     __shared__ float s_sum[GATED ? 2 : 1][256 * V];
@@ -30,6 +30,7 @@ template <typename T, int V, bool GATED> __global__ __launch_bounds__(256) void 
 #pragma unroll
     for (int v = 0; v < V; ++v) s0[v] = s1[v] = 0.f;
     if (n < a.N) {
+#pragma unroll 2
         for (int64_t m = lo + ty; m < hi; m += ry) {
             const TV dy = *reinterpret_cast<const TV*>((const T*)a.dy + m * a.ld_dy + n);
             TV o0, o1;
@@ -38,7 +39,7 @@ template <typename T, int V, bool GATED> __global__ __launch_bounds__(256) void 
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     float val;
-                    const float slope = act_slope(a.act, gate.e[v], &val), d = (float)dy.e[v];
+                    const float slope = act_slope(ACT, gate.e[v], &val), d = (float)dy.e[v];
                     const float dg = d * up.e[v] * slope, du = d * val;
                     s0[v] += dg;
                     s1[v] += du;
@@ -53,7 +54,7 @@ template <typename T, int V, bool GATED> __global__ __launch_bounds__(256) void 
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     float val, d = (float)dy.e[v];
-                    if (a.z[0]) d *= act_slope(a.act, z.e[v], &val);
+                    if (a.z[0]) d *= act_slope(ACT, z.e[v], &val);
                     s0[v] += d;
                     o0.e[v] = (T)d;
                 }
@@ -80,21 +81,22 @@ template <typename T, int V, bool GATED> __global__ __launch_bounds__(256) void 
     }
 }
 
-// out[n] = sum of the chunks' partials, in a fixed order; 32 columns x 8 lanes a block
-template <typename T> __global__ __launch_bounds__(256) void k_column_join(const float* part0, const float* part1, void* out0, void* out1,
+// out[n] = sum of the chunks' partials, in a fixed order; 32 columns x 32 lanes a block
+template <typename T> __global__ __launch_bounds__(1024) void k_column_join(const float* part0, const float* part1, void* out0, void* out1,
                                                                            int chunks, int N) {
-    __shared__ float s_sum[8][33];
+    __shared__ float s_sum[32][33];
     const float* part = blockIdx.y ? part1 : part0;
     T* out = (T*)(blockIdx.y ? out1 : out0);
     const int c = threadIdx.x & 31, y = threadIdx.x >> 5, n = blockIdx.x * 32 + c;
     float s = 0.f;
     if (out && n < N)
-        for (int i = y; i < chunks; i += 8) s += part[(int64_t)i * N + n];
+#pragma unroll 4
+        for (int i = y; i < chunks; i += 32) s += part[(int64_t)i * N + n];
     s_sum[y][c] = s;
     __syncthreads();
     if (y == 0 && out && n < N) {
         float t = 0.f;
-        for (int i = 0; i < 8; ++i) t += s_sum[i][c];
+        for (int i = 0; i < 32; ++i) t += s_sum[i][c];
         out[n] = (T)t;
     }
 }
@@ -166,7 +168,7 @@ static void slope_shape(int64_t M, int64_t N, int V, int* cx, int* gx, int* chun
     int64_t n = 2048 / *gx;
     const int64_t most = M / ((256 / c) * 4);
     if (n > most) n = most;
-    if (n > 512) n = 512;
+    if (n > 1024) n = 1024;
     *chunks = (int)(n < 1 ? 1 : n);
 }
 
@@ -268,7 +270,6 @@ static int backward(const v2vae_dense* d, const void* x, const void* w0, const v
         s.ld_dy = d->ld_dy;
         s.M = M;
         s.N = (int)d->out;
-        s.act = d->activation;
         s.z[0] = act ? z : nullptr;
         s.z[1] = gated ? z + M * d->out : nullptr;
         if (act) {
@@ -288,17 +289,28 @@ static int backward(const v2vae_dense* d, const void* x, const void* w0, const v
         slope_shape(M, d->out, v4 ? 4 : 1, &s.cx, &gx, &chunks);
         s.rows_per_chunk = (M + chunks - 1) / chunks;
         const dim3 grid(gx, chunks);
+        auto slopes = [&](auto t, auto kind) {
+            typedef decltype(t) T;
+            constexpr int ACT = decltype(kind)::value;
+            if (gated) {
+                if (v4) hipLaunchKernelGGL((k_dense_slopes<T, 4, ACT, true>), grid, dim3(256), 0, st, s);
+                else hipLaunchKernelGGL((k_dense_slopes<T, 1, ACT, true>), grid, dim3(256), 0, st, s);
+            } else {
+                if (v4) hipLaunchKernelGGL((k_dense_slopes<T, 4, ACT, false>), grid, dim3(256), 0, st, s);
+                else hipLaunchKernelGGL((k_dense_slopes<T, 1, ACT, false>), grid, dim3(256), 0, st, s);
+            }
+        };
         auto go = [&](auto t) {
             typedef decltype(t) T;
-            if (gated) {
-                if (v4) hipLaunchKernelGGL((k_dense_slopes<T, 4, true>), grid, dim3(256), 0, st, s);
-                else hipLaunchKernelGGL((k_dense_slopes<T, 1, true>), grid, dim3(256), 0, st, s);
-            } else {
-                if (v4) hipLaunchKernelGGL((k_dense_slopes<T, 4, false>), grid, dim3(256), 0, st, s);
-                else hipLaunchKernelGGL((k_dense_slopes<T, 1, false>), grid, dim3(256), 0, st, s);
+            switch (d->activation) {
+                case V2VAE_ACT_RELU: slopes(t, std::integral_constant<int, V2VAE_ACT_RELU>()); break;
+                case V2VAE_ACT_SILU: slopes(t, std::integral_constant<int, V2VAE_ACT_SILU>()); break;
+                case V2VAE_ACT_GELU: slopes(t, std::integral_constant<int, V2VAE_ACT_GELU>()); break;
+                case V2VAE_ACT_TANH: slopes(t, std::integral_constant<int, V2VAE_ACT_TANH>()); break;
+                default: slopes(t, std::integral_constant<int, V2VAE_ACT_NONE>()); break;
             }
             if (want_b)
-                hipLaunchKernelGGL((k_column_join<T>), dim3((unsigned)((d->out + 31) / 32), gated ? 2 : 1), dim3(256), 0, st, s.part[0],
+                hipLaunchKernelGGL((k_column_join<T>), dim3((unsigned)((d->out + 31) / 32), gated ? 2 : 1), dim3(1024), 0, st, s.part[0],
                                    s.part[1], db0, db1, chunks, (int)d->out);
         };
         if (d->dtype == V2VAE_F32) go(float());

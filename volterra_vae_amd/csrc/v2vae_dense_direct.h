@@ -4,7 +4,7 @@
 // is 64 elements, two steps' tiles live in LDS, and while one is multiplied the loads of the next (global_load_lds, 16 bytes a
 // lane, no registers) are in flight: one barrier a step.  Such a load writes its 64 pieces in lane order, so the order of pieces
 // in LDS is chosen by which piece a lane fetches:
-//  * contraction contiguous: a row is 8 pieces; row r holds piece p at position p ^ (r % 8), and the 16-byte reads of a
+//  * contraction contiguous: a row is 8 pieces; row r holds piece p at position p ^ (r / 2 % 8), and the 16-byte reads of a
 //    fragment (32 rows, one piece each) spread over all banks;
 //  * rows contiguous: a contraction index is a line of 32 TM WM (or TN WN) elements, read as a transposed fragment by
 //    ds_read_b64_tr_b16 (16 lanes read 4 k x 16 rows and receive 4 k of one row each).  Line k holds its 64-byte blocks at
@@ -47,7 +47,7 @@ template <typename T, int ROWS, int NW, bool KC, bool GATED> struct Tile {
         for (int j = 0; j < LOADS; ++j) {
             const int i = j * NW + wave;
             if constexpr (KC) {
-                const int r = i * 8 + (lane >> 3), piece = (lane & 7) ^ (r & 7);
+                const int r = i * 8 + (lane >> 3), piece = (lane & 7) ^ ((r >> 1) & 7);
                 int row = GATED ? (r >> 6) * 32 + (r & 31) : r;
                 row = first + row < R ? row : R - 1 - first;
                 off[j] = (unsigned)(row * (GATED ? ld2[(r >> 5) & 1] : ld) + piece * 8) * 2u;
@@ -74,7 +74,7 @@ template <typename T, int ROWS, int NW, bool KC, bool GATED> struct Tile {
                 const int i = j * NW + wave;
                 const char* b = GATED && (((i * 8) >> 5) & 1) ? base1 : base0;
                 int k;
-                if constexpr (KC) k = ((lane & 7) ^ ((i * 8 + (lane >> 3)) & 7)) * 8; else k = (i * 64 + lane) / (ROWS / 8);
+                if constexpr (KC) k = ((lane & 7) ^ (((i * 8 + (lane >> 3)) >> 1) & 7)) * 8; else k = (i * 64 + lane) / (ROWS / 8);
                 load_to_lds(k < left ? (const void*)(b + off[j]) : (const void*)g_zero_piece, lds + i * 1024);
             }
         }
@@ -136,12 +136,12 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN) / 4) void k_gemm_direct(Gem
     };
 #pragma unroll
     for (int q = 0; q < OA; ++q) {
-        if constexpr (AKC) oa[q] = (unsigned)((wm * 32 * TM + (lane & 31)) * 128 + (((q * 2 + (lane >> 5)) ^ (lane & 7)) * 16));
+        if constexpr (AKC) oa[q] = (unsigned)((wm * 32 * TM + (lane & 31)) * 128 + (((q * 2 + (lane >> 5)) ^ ((lane >> 1) & 7)) * 16));
         else oa[q] = mn_offset(wm * TM + q, BM);
     }
 #pragma unroll
     for (int q = 0; q < OB; ++q) {
-        if constexpr (BKC) ob[q] = (unsigned)((wn * 32 * TN + (lane & 31)) * 128 + (((q * 2 + (lane >> 5)) ^ (lane & 7)) * 16));
+        if constexpr (BKC) ob[q] = (unsigned)((wn * 32 * TN + (lane & 31)) * 128 + (((q * 2 + (lane >> 5)) ^ ((lane >> 1) & 7)) * 16));
         else ob[q] = mn_offset(wn * TN + q, BN);
     }
     auto frag_mn = [&](unsigned at, int rows, int kk) {

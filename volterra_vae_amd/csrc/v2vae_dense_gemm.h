@@ -17,27 +17,6 @@
 
 namespace v2vae {
 
-template <typename T> struct Elem;
-template <> struct Elem<float> { static constexpr int NP = 3, BK = 32; typedef bf16x8 frag; };
-template <> struct Elem<bf16_t> { static constexpr int NP = 1, BK = 64; typedef bf16x8 frag; };
-template <> struct Elem<f16_t> { static constexpr int NP = 1, BK = 64; typedef f16x8 frag; };
-
-__device__ __forceinline__ f32x16 mma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ f32x16 mma32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
-
-// two floats -> their three bf16 pieces, each pair packed in a word
-__device__ __forceinline__ void split_pair(float x0, float x1, unsigned p[3]) {
-    typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        const bf16x2 h = {(__bf16)x0, (__bf16)x1};
-        const unsigned u = __builtin_bit_cast(unsigned, h);
-        p[i] = u;
-        x0 -= __uint_as_float(u << 16);
-        x1 -= __uint_as_float(u & 0xFFFF0000u);
-    }
-}
-
 // One operand's tile of one contraction step: ROWS rows x BK, held by 256 threads between the global load and the LDS store.
 template <typename T, int ROWS, bool KC> struct Stage;
 

@@ -1,98 +1,121 @@
 // One to sixteen rows through a dense layer or a gated block: the form that answers single symbols.
 //
-// The weights are read once and nothing else counts, so the kernel is a stream over them: a workgroup owns NR weight rows, its
-// 256 threads run along the contraction in 16-byte pieces (all NR pieces of a step in flight together), every piece is multiplied
-// with the MR input rows (held by the caches) into MR x NR float sums per thread, and the sums are joined over the lanes by
-// shuffles and over the four waves through LDS, in a fixed order.
+// The weights are read once and nothing else counts, so the kernel is a stream over them.  A workgroup of eight waves owns 16
+// weight rows (gated block: 16 gate and 16 up rows of the same features); the waves take turns along the contraction, 128 elements
+// each, and multiply on v_mfma_f32_16x16x32 with the input rows as the other operand (rows beyond the last repeat it): the matrix
+// instruction sums over lanes, which costs a vector kernel six shuffles per output and wave.  The fragments come straight from
+// memory (16 bytes a lane, any alignment); float operands are split into three bf16 pieces in registers (six products).  The
+// eight waves' sums are joined through LDS in a fixed order.
 #include "v2vae_dense.h"
 
 namespace v2vae {
 
-template <typename T, int MR, int NR, bool GATED> __global__ __launch_bounds__(256) void k_dense_rows(GemmArgs g) {
-    constexpr int E = Vec16<T>::N, FT = GATED ? NR / 2 : NR;  // features of the workgroup
-    __shared__ float s_sum[4][MR * NR];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int n0 = blockIdx.x * FT;
-    const T* w[NR];
+typedef __attribute__((ext_vector_type(4))) float acc4;
+__device__ __forceinline__ acc4 mma16(bf16x8 a, bf16x8 b, acc4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ acc4 mma16(f16x8 a, f16x8 b, acc4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+// eight consecutive elements of a row, at any alignment; TAIL: some may lie beyond K, zeros there
+template <typename T> struct Eight { T e[8]; };
+template <typename T, bool TAIL> __device__ __forceinline__ Eight<T> load_eight(const T* p, int k, int K) {
+    struct __attribute__((packed, aligned(sizeof(T)))) Loose { T e[8]; };
+    Eight<T> v;
+    if constexpr (!TAIL) {
+        const Loose t = *reinterpret_cast<const Loose*>(p + k);
 #pragma unroll
-    for (int r = 0; r < NR; ++r) {
-        const int n = n0 + (GATED ? r >> 1 : r), nc = n < g.N ? n : g.N - 1, which = GATED ? r & 1 : 0;
-        w[r] = (const T*)g.b[which] + (int64_t)nc * g.ldb[which];
-    }
-    const T* const x = (const T*)g.a[0];
-    float acc[MR][NR];
-#pragma unroll
-    for (int m = 0; m < MR; ++m)
-#pragma unroll
-        for (int r = 0; r < NR; ++r) acc[m][r] = 0.f;
-    if (g.vec_a && g.vec_b) {
-        for (int k = tid * E; k < g.K; k += 256 * E) {
-            Vec16<T> wv[NR];
-#pragma unroll
-            for (int r = 0; r < NR; ++r) wv[r].raw = *reinterpret_cast<const u32x4*>(w[r] + k);
-#pragma unroll
-            for (int m = 0; m < MR; ++m) {
-                Vec16<T> xv;
-                xv.raw = *reinterpret_cast<const u32x4*>(x + (int64_t)(m < g.M ? m : g.M - 1) * g.lda + k);
-#pragma unroll
-                for (int r = 0; r < NR; ++r)
-#pragma unroll
-                    for (int e = 0; e < E; ++e) acc[m][r] = fmaf((float)wv[r].e[e], (float)xv.e[e], acc[m][r]);
-            }
-        }
+        for (int e = 0; e < 8; ++e) v.e[e] = t.e[e];
     } else {
-        for (int k = tid; k < g.K; k += 256) {
-            float wv[NR];
 #pragma unroll
-            for (int r = 0; r < NR; ++r) wv[r] = (float)w[r][k];
-#pragma unroll
-            for (int m = 0; m < MR; ++m) {
-                const float xv = (float)x[(int64_t)(m < g.M ? m : g.M - 1) * g.lda + k];
-#pragma unroll
-                for (int r = 0; r < NR; ++r) acc[m][r] = fmaf(wv[r], xv, acc[m][r]);
-            }
-        }
+        for (int e = 0; e < 8; ++e) v.e[e] = k + e < K ? p[k + e] : (T)0.f;
     }
+    return v;
+}
+template <typename T> __device__ __forceinline__ void pieces_of(const Eight<T>& v, typename Elem<T>::frag f[Elem<T>::NP]) {
+    if constexpr (sizeof(T) == 4) {
+        union { unsigned u[4]; bf16x8 f; } w[3];
 #pragma unroll
-    for (int m = 0; m < MR; ++m)
+        for (int i = 0; i < 4; ++i) {
+            unsigned p[3];
+            split_pair(v.e[2 * i], v.e[2 * i + 1], p);
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
-            float s = acc[m][r];
-#pragma unroll
-            for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
-            if (lane == 0) s_sum[wave][m * NR + r] = s;
+            for (int q = 0; q < 3; ++q) w[q].u[i] = p[q];
         }
-    __syncthreads();
-    for (int i = tid; i < MR * FT; i += 256) {
-        const int m = i / FT, f = i % FT, n = n0 + f;
-        if (m >= g.M || n >= g.N) continue;
-        auto total = [&](int r) { return (s_sum[0][m * NR + r] + s_sum[1][m * NR + r]) + (s_sum[2][m * NR + r] + s_sum[3][m * NR + r]); };
-        float s0 = total(GATED ? 2 * f : f);
-        if constexpr (GATED) {
-            float s1 = total(2 * f + 1);
-            finish_gated<T, 1>(g, m, n, &s0, &s1, true);
-        } else {
-            finish_value<T, 1>(g, m, n, &s0, 0, true);
-        }
+#pragma unroll
+        for (int q = 0; q < 3; ++q) f[q] = w[q].f;
+    } else {
+        f[0] = __builtin_bit_cast(typename Elem<T>::frag, v);
     }
 }
 
-template <typename T, int MR, bool GATED> static void launch_rows(const GemmArgs& g, hipStream_t st) {
-    constexpr int NR = 4, FT = GATED ? NR / 2 : NR;
-    hipLaunchKernelGGL((k_dense_rows<T, MR, NR, GATED>), dim3((g.N + FT - 1) / FT), dim3(256), 0, st, g);
+template <typename T, bool GATED> __global__ __launch_bounds__(512) void k_dense_rows(GemmArgs g) {
+    constexpr int NP = Elem<T>::NP, NB = GATED ? 2 : 1;
+    typedef typename Elem<T>::frag frag;
+    __shared__ float s_sum[NB][8][16][17];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, kl = (lane >> 4) * 8, n0 = blockIdx.x * 16;
+    const int nc = n0 + r < g.N ? n0 + r : g.N - 1, mc = r < g.M ? r : g.M - 1;
+    const T* w[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) w[b] = (const T*)g.b[b] + (int64_t)nc * g.ldb[b];
+    const T* const x = (const T*)g.a[0] + (int64_t)mc * g.lda;
+    acc4 acc[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) acc[b] = acc4{0.f, 0.f, 0.f, 0.f};
+    auto chunk = [&](int k0, auto tail) {
+        Eight<T> wv[NB][4], xv[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int k = k0 + i * 32 + kl;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) wv[b][i] = load_eight<T, decltype(tail)::value>(w[b], k, g.K);
+            xv[i] = load_eight<T, decltype(tail)::value>(x, k, g.K);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            frag xf[NP];
+            pieces_of<T>(xv[i], xf);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                frag wf[NP];
+                pieces_of<T>(wv[b][i], wf);
+#pragma unroll
+                for (int sum = NP - 1; sum >= 0; --sum)
+#pragma unroll
+                    for (int p = 0; p <= sum; ++p) acc[b] = mma16(wf[p], xf[sum - p], acc[b]);
+            }
+        }
+    };
+    const int whole = g.K / 128 * 128;
+#pragma unroll 2
+    for (int k0 = wave * 128; k0 < whole; k0 += 8 * 128) chunk(k0, std::false_type());
+    if (whole < g.K && (whole / 128) % 8 == wave) chunk(whole, std::true_type());
+    // lane: input row lane % 16, weight rows 4 (lane / 16) ... + 3
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s_sum[b][wave][r][4 * (lane >> 4) + e] = acc[b][e];
+    __syncthreads();
+    if (tid >= 256) return;
+    const int m = tid >> 4, f = tid & 15, n = n0 + f;
+    if (m >= g.M || n >= g.N) return;
+    float s[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        s[b] = 0.f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) s[b] += s_sum[b][q][m][f];
+    }
+    if constexpr (GATED) finish_gated<T, 1>(g, m, n, &s[0], &s[1], true); else finish_value<T, 1>(g, m, n, &s[0], 0, true);
 }
-template <typename T, bool GATED> static void pick_rows(const GemmArgs& g, hipStream_t st) {
-    if (g.M <= 1) launch_rows<T, 1, GATED>(g, st);
-    else if (g.M <= 2) launch_rows<T, 2, GATED>(g, st);
-    else if (g.M <= 4) launch_rows<T, 4, GATED>(g, st);
-    else if (g.M <= 8) launch_rows<T, 8, GATED>(g, st);
-    else launch_rows<T, 16, GATED>(g, st);
+
+template <typename T> static void launch_rows(const GemmArgs& g, bool gated, hipStream_t st) {
+    const dim3 grid((g.N + 15) / 16);
+    if (gated) hipLaunchKernelGGL((k_dense_rows<T, true>), grid, dim3(512), 0, st, g);
+    else hipLaunchKernelGGL((k_dense_rows<T, false>), grid, dim3(512), 0, st, g);
 }
 
 int dense_rows(const GemmArgs& g, int dtype, bool gated, hipStream_t st) {
-    if (dtype == V2VAE_F32) gated ? pick_rows<float, true>(g, st) : pick_rows<float, false>(g, st);
-    else if (dtype == V2VAE_BF16) gated ? pick_rows<bf16_t, true>(g, st) : pick_rows<bf16_t, false>(g, st);
-    else gated ? pick_rows<f16_t, true>(g, st) : pick_rows<f16_t, false>(g, st);
+    if (dtype == V2VAE_F32) launch_rows<float>(g, gated, st);
+    else if (dtype == V2VAE_BF16) launch_rows<bf16_t>(g, gated, st);
+    else launch_rows<f16_t>(g, gated, st);
     return dense_launch_error("dense layer, few rows");
 }
 

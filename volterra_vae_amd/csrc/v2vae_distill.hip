@@ -81,8 +81,8 @@ constexpr float LOG2E = 1.4426950408889634f;
 __device__ __forceinline__ float exp_diff(float z, float zmax, float c) { return __builtin_amdgcn_exp2f((z - zmax) * c); }
 
 // G lanes a row, NV 16-byte pieces of the row held by each lane (HELD), or the row read once per pass.  MODE: DO_LOSS | DO_GRAD.
-// A DO_GRAD pass alone takes maximum and sum from `stats`.
-template <typename T, int G, int NV, bool HELD, int MODE>
+// A DO_GRAD pass alone takes maximum and sum from `stats`.  ONE: k <= G, every lane has at most one teacher entry and keeps it.
+template <typename T, int G, int NV, bool HELD, int MODE, bool ONE>
 __global__ __launch_bounds__(G > 64 ? G : 256) void k_distill(DistillArgs a) {
     constexpr int E = Vec16<T>::N, ROWS = G > 64 ? 1 : 256 / G;
     constexpr bool STATS_GIVEN = MODE == DO_GRAD;
@@ -109,6 +109,17 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void k_distill(DistillArgs a) {
         }
         return v;
     };
+
+    // entry and its logit, asked for before the row so that they arrive with it
+    int my_cls = -1;
+    float my_t = 0.f, my_z = 0.f;
+    if constexpr (ONE) {
+        if (tid < a.k) {
+            my_cls = class_at(a, row, tid);
+            my_t = teacher_at(a, row, tid);
+            if (my_cls >= 0) my_z = (float)z[my_cls];
+        }
+    }
 
     const float c = a.inv_t * LOG2E;
     Vec16<T> held[HELD ? NV : 1];
@@ -169,41 +180,45 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void k_distill(DistillArgs a) {
     float tmax = -INFINITY;
     int bad = 0;
     for (int j = tid; j < a.k; j += G) {
-        const int cls = class_at(a, row, j);
-        const float t = teacher_at(a, row, j);
+        const int cls = ONE ? my_cls : class_at(a, row, j);
+        const float t = ONE ? my_t : teacher_at(a, row, j);
         bad |= cls == -2 || (cls >= 0 && t != t);  // a class beyond the vocabulary, a NaN
         if (cls >= 0) tmax = fmaxf(tmax, t);
+        if (ONE) break;
     }
-    const float any_bad = lanes.max(bad ? 1.f : 0.f);
-    tmax = lanes.max(tmax);
-    float mass = 0.f;
-    if (tmax != -INFINITY) {
-        for (int j = tid; j < a.k; j += G) {
-            const int cls = class_at(a, row, j);
-            if (cls >= 0) mass += expf((teacher_at(a, row, j) - tmax) * a.inv_t);
-        }
+    tmax = lanes.max(bad ? INFINITY : tmax);       // +inf, from here or among the logits: the row is NaN
+    const bool any_bad = tmax == INFINITY;
+    float mass = 0.f, my_p = 0.f;
+    const bool there = tmax != -INFINITY;
+    for (int j = tid; j < a.k && there; j += G) {
+        const int cls = ONE ? my_cls : class_at(a, row, j);
+        const float e = cls >= 0 ? expf(((ONE ? my_t : teacher_at(a, row, j)) - tmax) * a.inv_t) : 0.f;
+        mass += e;
+        if (ONE) { my_p = e; break; }
     }
     mass = lanes.sum(mass);
-    const bool some = mass != 0.f;  // inf among the teacher's logits: NaN, present
+    const bool some = there && !any_bad;
     const float inv_mass = some ? 1.f / mass : 0.f, log_mass = logf(some ? mass : 1.f), log_l = logf(l);
+    my_p *= inv_mass;
 
     if constexpr (MODE & DO_LOSS) {
         float part = 0.f;
-        for (int j = tid; j < a.k; j += G) {
-            const int cls = class_at(a, row, j);
-            if (cls < 0 || !some) continue;
-            const float lt = (teacher_at(a, row, j) - tmax) * a.inv_t, p = expf(lt) * inv_mass;
-            if (p == 0.f) continue;
-            const float zj = (float)z[cls];
-            const float log_q = zj == -INFINITY ? -INFINITY : (zj - zm) * a.inv_t - log_l;
-            part += p * (lt - log_mass - log_q);
+        for (int j = tid; j < a.k && some; j += G) {
+            const int cls = ONE ? my_cls : class_at(a, row, j);
+            const float lt = ((ONE ? my_t : teacher_at(a, row, j)) - tmax) * a.inv_t, p = ONE ? my_p : cls >= 0 ? expf(lt) * inv_mass : 0.f;
+            if (p != 0.f) {
+                const float zj = ONE ? my_z : (float)z[cls];
+                const float log_q = zj == -INFINITY ? -INFINITY : (zj - zm) * a.inv_t - log_l;
+                part += p * (lt - log_mass - log_q);
+            }
+            if (ONE) break;
         }
         part = lanes.sum(part);
-        if (tid == 0) a.loss[row] = any_bad != 0.f ? NAN : a.T * a.T * part;
+        if (tid == 0) a.loss[row] = any_bad ? NAN : a.T * a.T * part;
     }
     if constexpr (MODE & DO_GRAD) {
-        const float wt = any_bad != 0.f ? NAN : a.weight[row] * a.T;
-        const bool live = some || any_bad != 0.f;
+        const float wt = any_bad ? NAN : a.weight[row] * a.T;
+        const bool live = some || any_bad;
         const float inv_l = l == 0.f ? 0.f : 1.f / l, scale = wt * inv_l;
         T* const out = (T*)a.grad + row * a.V;
         const bool same_phase = (int)(((uintptr_t)out & 15) / sizeof(T)) == off;
@@ -229,48 +244,69 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void k_distill(DistillArgs a) {
         }
         if constexpr (G > 64) {
             for (int j = tid; j < a.k; j += G) {
-                const int cls = class_at(a, row, j);
+                const int cls = ONE ? my_cls : class_at(a, row, j);
                 s_c[j] = cls;
-                s_p[j] = cls >= 0 && some ? expf((teacher_at(a, row, j) - tmax) * a.inv_t) * inv_mass : 0.f;
+                s_p[j] = ONE ? my_p : cls >= 0 && some ? expf((teacher_at(a, row, j) - tmax) * a.inv_t) * inv_mass : 0.f;
+                if (ONE) break;
             }
         }
         lanes.sync();
-        for (int j = tid; j < a.k; j += G) {
-            const int cls = G > 64 ? s_c[j] : class_at(a, row, j);
-            if (cls < 0 || !some) continue;
+        if constexpr (ONE && G <= 64) {
             float p = 0.f;
             bool first = true;
-            for (int i = 0; i < a.k; ++i) {
-                if (G > 64) {
-                    if (s_c[i] == cls) { p += s_p[i]; first &= i >= j; }
-                } else if (class_at(a, row, i) == cls) {
-                    p += expf((teacher_at(a, row, i) - tmax) * a.inv_t) * inv_mass;
-                    first &= i >= j;
+            for (int i = 0; i < a.k; ++i) {  // all lanes of the group, entry or not
+                const int c = __shfl(my_cls, i, G);
+                const float q = __shfl(my_p, i, G);
+                if (c == my_cls) {
+                    p += q;
+                    first &= i >= tid;
                 }
             }
-            if (first) out[cls] = (T)(wt * (exp_diff((float)z[cls], zm, c) * inv_l - p));
+            if (my_cls >= 0 && some && first) out[my_cls] = (T)(wt * (exp_diff(my_z, zm, c) * inv_l - p));
+        } else {
+            for (int j = tid; j < a.k; j += G) {
+                const int cls = G > 64 ? s_c[j] : class_at(a, row, j);
+                if (cls < 0 || !some) continue;
+                float p = 0.f;
+                bool first = true;
+                for (int i = 0; i < a.k; ++i) {
+                    if (G > 64) {
+                        if (s_c[i] == cls) { p += s_p[i]; first &= i >= j; }
+                    } else if (class_at(a, row, i) == cls) {
+                        p += expf((teacher_at(a, row, i) - tmax) * a.inv_t) * inv_mass;
+                        first &= i >= j;
+                    }
+                }
+                if (first) out[cls] = (T)(wt * (exp_diff((float)z[cls], zm, c) * inv_l - p));
+            }
         }
     }
 }
 
-template <typename T, int G, int NV, bool HELD> static void go(const DistillArgs& a, int mode, hipStream_t st) {
+template <typename T, int G, int NV, bool HELD, bool ONE> static void go_mode(const DistillArgs& a, int mode, hipStream_t st) {
     constexpr int ROWS = G > 64 ? 1 : 256 / G, NT = G > 64 ? G : 256;
     const dim3 grid((unsigned)((a.rows + ROWS - 1) / ROWS));
-    if (mode == DO_LOSS) hipLaunchKernelGGL((k_distill<T, G, NV, HELD, DO_LOSS>), grid, dim3(NT), 0, st, a);
-    else if (mode == DO_GRAD) hipLaunchKernelGGL((k_distill<T, G, NV, HELD, DO_GRAD>), grid, dim3(NT), 0, st, a);
-    else hipLaunchKernelGGL((k_distill<T, G, NV, HELD, DO_LOSS | DO_GRAD>), grid, dim3(NT), 0, st, a);
+    if (mode == DO_LOSS) hipLaunchKernelGGL((k_distill<T, G, NV, HELD, DO_LOSS, ONE>), grid, dim3(NT), 0, st, a);
+    else if (mode == DO_GRAD) hipLaunchKernelGGL((k_distill<T, G, NV, HELD, DO_GRAD, ONE>), grid, dim3(NT), 0, st, a);
+    else hipLaunchKernelGGL((k_distill<T, G, NV, HELD, DO_LOSS | DO_GRAD, ONE>), grid, dim3(NT), 0, st, a);
+}
+template <typename T, int G, int NV, bool HELD> static void go(const DistillArgs& a, int mode, hipStream_t st) {
+    if (a.k <= G) go_mode<T, G, NV, HELD, true>(a, mode, st); else go_mode<T, G, NV, HELD, false>(a, mode, st);
 }
 
 template <typename T> static int distill(const DistillArgs& a, int mode, hipStream_t st) {
     constexpr int E = Vec16<T>::N;
-    const int64_t pieces = (a.V + 2 * E - 2) / E;  // of a row that starts anywhere in a piece
+    // pieces of a row: V / E if every row starts at one, else of a row that starts anywhere
+    const bool aligned = ((uintptr_t)a.z & 15) == 0 && (a.ld_z % E == 0 || a.rows == 1);
+    const int64_t pieces = aligned ? (a.V + E - 1) / E : (a.V + 2 * E - 2) / E;
     if (pieces <= 8) go<T, 8, 1, true>(a, mode, st);
     else if (pieces <= 16) go<T, 16, 1, true>(a, mode, st);
     else if (pieces <= 32) go<T, 16, 2, true>(a, mode, st);
     else if (pieces <= 64) go<T, 32, 2, true>(a, mode, st);
     else if (pieces <= 256) go<T, 64, 4, true>(a, mode, st);
     else if (pieces <= 1024) go<T, 256, 4, true>(a, mode, st);
-    else if (pieces <= 4096) go<T, 1024, 4, true>(a, mode, st);
+    else if (pieces <= 2048) go<T, 256, 8, true>(a, mode, st);
+    else if (pieces <= 4096) go<T, 512, 8, true>(a, mode, st);
     else if (pieces <= 8192) go<T, 1024, 8, true>(a, mode, st);
     else go<T, 1024, 1, false>(a, mode, st);
     return dense_launch_error("distillation");

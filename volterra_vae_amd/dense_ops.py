@@ -11,6 +11,7 @@ that run without autograd (and for HIP graphs, into which they can be captured).
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional, Tuple
 
@@ -25,22 +26,28 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 def _check_tensor(t, name, dim, like=None, dtype=None):
+    try:  # what passes, first: these checks run before every launch
+        want = dtype if dtype is not None else (like.dtype if like is not None else t.dtype)
+        index = t.get_device()
+        if (t.dtype is want and (like is not None or want in _DTYPES) and index >= 0 and (like is None or index == like.get_device())
+                and t.dim() == dim and (t.stride(-1) == 1 or t.shape[-1] <= 1)):
+            return
+    except (AttributeError, IndexError):
+        pass
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor (got {type(t).__name__})")
     if not t.is_cuda:
         raise RuntimeError(f"{name} must live on the GPU: these kernels have no CPU implementation")
     if like is not None and t.device != like.device:
         raise ValueError(f"{name} is on {t.device}, expected {like.device}")
-    want = dtype if dtype is not None else (like.dtype if like is not None else None)
-    if want is None:
+    if dtype is None and like is None:
         if t.dtype not in _DTYPES:
             raise NotImplementedError(f"{name}: float32, bfloat16 or float16 only (got {t.dtype})")
     elif t.dtype != want:
         raise ValueError(f"{name} is {t.dtype}, expected {want}")
     if t.dim() != dim:
         raise ValueError(f"{name} must have {dim} dimension{'s' if dim > 1 else ''} (got {t.dim()})")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{name} must have unit stride in its last dimension")
+    raise ValueError(f"{name} must have unit stride in its last dimension")
 
 
 def _row_stride(t):
@@ -59,23 +66,34 @@ def _p(t):
 
 
 class _On:
-    """The tensors' device made current around the calls, where it is not already."""
+    """The tensors' device made current around the calls, where it is not already; gives its current stream."""
+    __slots__ = ("index", "guard")
 
-    def __init__(self, device):
-        self.guard = torch.cuda.device(device) if device.index != torch.cuda.current_device() else None
+    def __init__(self, t):
+        self.index = t.get_device()
+        self.guard = None
 
     def __enter__(self):
-        if self.guard is not None:
+        if self.index != torch._C._cuda_getDevice():
+            self.guard = torch.cuda.device(self.index)
             self.guard.__enter__()
-        return torch.cuda.current_stream().cuda_stream
+        return torch._C._cuda_getCurrentRawStream(self.index)
 
     def __exit__(self, *exc):
         if self.guard is not None:
             self.guard.__exit__(*exc)
 
 
-def _workspace(n, device):
-    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(gated, backward, dtype, act, rows, columns, out):
+    f = lib.v2vae_gated_workspace_bytes if gated else lib.v2vae_linear_workspace_bytes
+    return f(Dense(dtype, act, rows, columns, out, columns, columns, columns, out, out), backward)
+
+
+def _workspace(gated, backward, act, x, n):
+    """Scratch memory of one call, from torch's allocator: of the current stream, or of the graph that is being captured."""
+    size = _workspace_bytes(gated, backward, _DTYPES[x.dtype], act, x.shape[0], x.shape[1], n)
+    return torch.empty(max(size, 256), dtype=torch.uint8, device=x.device) if size or backward else None
 
 
 def _check_layer(x, weight, name, bias, bias_name):
@@ -122,10 +140,10 @@ def linear_forward(x, weight, bias=None, *, residual=None, activation="none",
         if tuple(residual.shape) != (m, n):
             raise ValueError(f"residual: expected {(m, n)}, got {tuple(residual.shape)}")
     d = _dense(x, weight, act, residual=residual)
-    with _On(x.device) as stream:
-        y = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    with _On(x) as stream:
+        y = x.new_empty((m, n))
         z = torch.empty((m, n), dtype=torch.float32, device=x.device) if keep and act else None
-        ws = _workspace(lib.v2vae_linear_workspace_bytes(d, 0), x.device)
+        ws = _workspace(False, 0, act, x, n)
         check(lib.v2vae_linear_fwd(d, _p(x), _p(weight), _p(bias), _p(residual), _p(y), _p(z), _p(ws), stream), "v2vae_linear_fwd")
     return y, z
 
@@ -143,10 +161,10 @@ def linear_backward(dy, x, weight, z=None, *, activation="none", need=(True, Tru
             raise ValueError("z: the pre-activations of linear_forward(..., keep=True) are needed with an activation")
         _check_kept(z, (m, n), x)
     d = _dense(x, weight, act, dy=dy)
-    with _On(x.device) as stream:
+    with _On(x) as stream:
         new = lambda wanted, *shape: torch.empty(shape, dtype=x.dtype, device=x.device) if wanted else None  # noqa: E731
         dx, dw, db = new(need[0], m, k), new(need[1], n, k), new(need[2], n)
-        ws = _workspace(max(256, lib.v2vae_linear_workspace_bytes(d, 1)), x.device)
+        ws = _workspace(False, 1, act, x, n)
         check(lib.v2vae_linear_bwd(d, _p(x), _p(weight), _p(z) if act else None, _p(dy), _p(dx), _p(dw), _p(db), _p(ws), stream),
               "v2vae_linear_bwd")
     return dx, dw, db
@@ -212,10 +230,10 @@ def gated_forward(x, weight_gate, weight_up, bias_gate=None, bias_up=None, *, ac
         raise ValueError(f"weight_up: expected {tuple(weight_gate.shape)}, got {tuple(weight_up.shape)}")
     m, n = x.shape[0], weight_gate.shape[0]
     d = _dense(x, weight_gate, act, w2=weight_up)
-    with _On(x.device) as stream:
-        h = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    with _On(x) as stream:
+        h = x.new_empty((m, n))
         gu = torch.empty((2, m, n), dtype=torch.float32, device=x.device) if keep else None
-        ws = _workspace(lib.v2vae_gated_workspace_bytes(d, 0), x.device)
+        ws = _workspace(True, 0, act, x, n)
         check(lib.v2vae_gated_fwd(d, _p(x), _p(weight_gate), _p(weight_up), _p(bias_gate), _p(bias_up), _p(h), _p(gu), _p(ws), stream),
               "v2vae_gated_fwd")
     return h, gu
@@ -234,10 +252,10 @@ def gated_backward(dh, x, weight_gate, weight_up, gu, *, activation="silu", need
     _check_grad(dh, "dh", x, n)
     _check_kept(gu, (2, m, n), x)
     d = _dense(x, weight_gate, act, w2=weight_up, dy=dh)
-    with _On(x.device) as stream:
+    with _On(x) as stream:
         new = lambda wanted, *shape: torch.empty(shape, dtype=x.dtype, device=x.device) if wanted else None  # noqa: E731
         out = [new(need[0], m, k), new(need[1], n, k), new(need[2], n, k), new(need[3], n), new(need[4], n)]
-        ws = _workspace(max(256, lib.v2vae_gated_workspace_bytes(d, 1)), x.device)
+        ws = _workspace(True, 1, act, x, n)
         check(lib.v2vae_gated_bwd(d, _p(x), _p(weight_gate), _p(weight_up), _p(gu), _p(dh), *[_p(t) for t in out], _p(ws), stream),
               "v2vae_gated_bwd")
     return tuple(out)
@@ -307,7 +325,7 @@ def topk_distillation_step(logits, teacher_logits, teacher_index, row_weight, *,
     """(loss [M] float32, grad [M, V]): the losses of `topk_distillation` and d(sum of row_weight * loss) / d logits, one pass."""
     d = _distill(logits, teacher_logits, teacher_index, temperature)
     _check_weight(row_weight, logits)
-    with _On(logits.device) as stream:
+    with _On(logits) as stream:
         loss = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         check(lib.v2vae_distill_step(d, _p(logits), _p(teacher_logits), _p(teacher_index), _p(row_weight), _p(loss), _p(grad), stream),
@@ -329,7 +347,7 @@ class _Distillation(torch.autograd.Function):
         logits, teacher_logits, teacher_index, stats = ctx.saved_tensors
         d = _distill(logits, teacher_logits, teacher_index, ctx.temperature)
         weight = weight.contiguous()
-        with _On(logits.device) as stream:
+        with _On(logits) as stream:
             grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
             check(lib.v2vae_distill_bwd(d, _p(logits), _p(teacher_logits), _p(teacher_index), _p(stats), _p(weight), _p(grad), stream),
                   "v2vae_distill_bwd")
@@ -338,7 +356,7 @@ class _Distillation(torch.autograd.Function):
 
 def _distill_forward(logits, teacher_logits, teacher_index, temperature, keep):
     d = _distill(logits, teacher_logits, teacher_index, temperature)
-    with _On(logits.device) as stream:
+    with _On(logits) as stream:
         loss = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
         stats = torch.empty((logits.shape[0], 2), dtype=torch.float32, device=logits.device) if keep else None
         check(lib.v2vae_distill_fwd(d, _p(logits), _p(teacher_logits), _p(teacher_index), _p(loss), _p(stats), stream),
