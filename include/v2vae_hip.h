@@ -358,9 +358,9 @@ typedef struct v2vae_dense {
     int32_t dtype;      /* V2VAE_F32, V2VAE_BF16 or V2VAE_F16 */
     int32_t activation; /* V2VAE_ACT_* */
     int64_t rows;       /* rows of x and y, 0 ... 2^30 */
-    int64_t in;         /* columns of x and of the weights, 1 ... 2^30 */
-    int64_t out;        /* rows of the weights, columns of y, 1 ... 2^30 */
-    int64_t ld_x;       /* >= 0, as all of these */
+    int64_t in;         /* columns of x and of the weights, 1 ... 2^22 */
+    int64_t out;        /* rows of the weights, columns of y, 1 ... 2^22 */
+    int64_t ld_x;       /* 0 ... 2^22, as all of these */
     int64_t ld_w;       /* gated block: of the gate weights */
     int64_t ld_w2;      /* gated block: of the up weights; otherwise ignored */
     int64_t ld_res;     /* where a residual is passed */

@@ -37,7 +37,8 @@ def test_bad_descriptions_are_refused(over):
 
 
 def test_sizes_beyond_the_limits_are_refused():
-    for over in (dict(rows=(1 << 30) + 1), dict(in_=(1 << 30) + 1), dict(out=1 << 31), dict(rows=1 << 30, out=1 << 30)):
+    for over in (dict(rows=(1 << 30) + 1), dict(in_=(1 << 22) + 1), dict(out=1 << 31), dict(rows=1 << 30, out=1 << 22),
+                 dict(ld_x=(1 << 22) + 1), dict(ld_w=(1 << 22) + 1)):
         assert _lib.lib.v2vae_linear_fwd(dense(**over), P, P, None, None, P, None, P, None) == _lib.ESIZE
         assert _lib.lib.v2vae_linear_workspace_bytes(dense(**over), 1) == 0
     assert _lib.lib.v2vae_distill_fwd(distill(k=1025, ld_teacher=1025, ld_index=1025), P, P, P, P, None, None) == _lib.ESIZE

@@ -39,7 +39,8 @@ __device__ __forceinline__ void split_pair(float x0, float x1, unsigned p[3]) {
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
         const bf16x2 h = {(__bf16)x0, (__bf16)x1};
-        const unsigned u = __builtin_bit_cast(unsigned, h);
+        unsigned u = __builtin_bit_cast(unsigned, h);
+        asm("" : "+v"(u));  // no instruction: keeps the compiler from converting each float again to get at its half of the pair
         p[i] = u;
         x0 -= __uint_as_float(u << 16);
         x1 -= __uint_as_float(u & 0xFFFF0000u);
@@ -82,6 +83,19 @@ __device__ __forceinline__ float normal_cdf(float z, float* gauss) {
     return z < 0.f ? half : 1.f - half;
 }
 
+// tanh z: below 0.55 an odd polynomial (least-squares fit of tanh(z) / z - 1 in z^2, 1e-9 at its worst), else from exp(-2 |z|)
+__device__ __forceinline__ float tanh_of(float z) {
+    const float u = z * z, y = fabsf(z);
+    float p = -0.006282466723832369f;
+    p = fmaf(p, u, 0.02107775339065489f);
+    p = fmaf(p, u, -0.053853856641005726f);
+    p = fmaf(p, u, 0.13332601672040642f);
+    p = fmaf(p, u, -0.33333318045245297f);
+    const float e = exp_with_rest(-2.f * fminf(y, 20.f), 0.f);
+    const float large = copysignf((1.f - e) * reciprocal(1.f + e), z);
+    return y < 0.55f ? fmaf(z * u, p, z) : (z != z ? z : large);
+}
+
 // act(z) and act'(z); the kinds are V2VAE_ACT_*.  For |z| beyond 80 the soft activations are their asymptotes to the last bit of
 // a float; the clamp keeps z (1 - s) and z exp(-z^2 / 2) from becoming inf * 0 there.  A NaN stays one.
 template <bool SLOPE> __device__ __forceinline__ float act_both(int kind, float z, float* slope) {
@@ -102,7 +116,7 @@ template <bool SLOPE> __device__ __forceinline__ float act_both(int kind, float 
             return z != z ? z : (z < -80.f ? 0.f : z * phi);
         }
         case V2VAE_ACT_TANH: {
-            const float t = tanhf(z);
+            const float t = tanh_of(z);
             if constexpr (SLOPE) *slope = fmaf(-t, t, 1.f);
             return t;
         }
@@ -134,6 +148,10 @@ struct GemmArgs {
     int64_t ldr;
     float* z[2];            // pre-activations kept for the backward pass, [M][N]; may be NULL
     int act;
+    // float32: the weights as three planes [plane_rows][plane_ld] of bf16 pieces (NULL: split on the way into LDS)
+    const void* planes;
+    int64_t plane_bytes;
+    int plane_rows, plane_ld;
 };
 
 // What happens to the finished sums of row m, columns n ... n + C - 1 (batch entry 1 has an output of its own, nothing else).
@@ -221,7 +239,8 @@ enum { LAYOUT_KK = 0, LAYOUT_KM = 1, LAYOUT_MM = 2 };  // A / B with the contrac
 enum { TILE_128 = 0, TILE_64 = 1, TILE_256 = 2 };
 int gemm_direct_bf16(const GemmArgs&, int layout, bool gated, int tile, hipStream_t);
 int gemm_direct_f16(const GemmArgs&, int layout, bool gated, int tile, hipStream_t);
-int gemm_staged_f32(const GemmArgs&, int layout, bool gated, int tile, hipStream_t);
+int split_planes(const GemmArgs&, bool transposed, bool gated, int N, int K, hipStream_t);  // b[], ldb[]: N x K weights
+int gemm_split(const GemmArgs&, int layout, bool gated, int tile, hipStream_t);  // float32
 int gemm_staged_bf16(const GemmArgs&, int layout, bool gated, int tile, hipStream_t);
 int gemm_staged_f16(const GemmArgs&, int layout, bool gated, int tile, hipStream_t);
 

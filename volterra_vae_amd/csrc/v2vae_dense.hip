@@ -106,15 +106,18 @@ static int elem_bytes(int dtype) { return dtype == V2VAE_F32 ? 4 : 2; }
 static bool aligned_to(const void* p, int n) { return ((uintptr_t)p % n) == 0; }
 static size_t round_up(size_t n) { return (n + 255) & ~(size_t)255; }
 
-constexpr int64_t DENSE_MAX = (int64_t)1 << 30;
+constexpr int64_t ROWS_LIMIT = (int64_t)1 << 30, WIDTH_LIMIT = (int64_t)1 << 22;  // columns and strides: 32-bit offsets inside a tile
 
 static int check_dense(const v2vae_dense* d, bool gated, bool backward, bool residual) {
     if (!d || d->dtype < V2VAE_F32 || d->dtype > V2VAE_F16) return V2VAE_EINVAL;
     if (d->activation < V2VAE_ACT_NONE || d->activation > V2VAE_ACT_TANH) return V2VAE_EINVAL;
     if (d->rows < 0 || d->in < 1 || d->out < 1) return V2VAE_EINVAL;
-    if (d->rows > DENSE_MAX || d->in > DENSE_MAX || d->out > DENSE_MAX) return V2VAE_ESIZE;
+    if (d->rows > ROWS_LIMIT || d->in > WIDTH_LIMIT || d->out > WIDTH_LIMIT) return V2VAE_ESIZE;
     if (d->ld_x < 0 || d->ld_w < 0 || (gated && d->ld_w2 < 0)) return V2VAE_EINVAL;
     if ((residual && d->ld_res < 0) || (backward && d->ld_dy < 0)) return V2VAE_EINVAL;
+    if (d->ld_x > WIDTH_LIMIT || d->ld_w > WIDTH_LIMIT || (gated && d->ld_w2 > WIDTH_LIMIT) || (residual && d->ld_res > WIDTH_LIMIT) ||
+        (backward && d->ld_dy > WIDTH_LIMIT))
+        return V2VAE_ESIZE;
     // tiles of 64 x 64 (gated forward: 64 x 64 features) are counted in 31 bits
     const int64_t m = (d->rows + 63) / 64, n = (d->out + 63) / 64, k = (d->in + 63) / 64;
     if (m * n >= INT32_MAX || m * k >= INT32_MAX || n * k >= INT32_MAX) return V2VAE_ESIZE;
@@ -129,7 +132,16 @@ static Cut cut_product(int64_t M, int64_t N, int64_t K, int segs, int batch, int
     auto tiles_of = [&](int64_t t) { return ((M + t - 1) / t) * ((N * (gated ? 2 : 1) + t - 1) / t) * batch; };
     Cut c;
     int64_t tiles, s = 1;
-    if (direct && tiles_of(256) >= 200) {
+    if (dtype == V2VAE_F32) {
+        const int64_t rows = (M + 127) / 128, wide = rows * ((N * (gated ? 2 : 1) + 127) / 128) * batch;
+        const int64_t narrow = rows * ((N * (gated ? 2 : 1) + 63) / 64) * batch;
+        // 128 columns a tile unless that leaves workgroups or a half-empty last column of tiles
+        c.tile = (wide >= 256 || wide * (steps / 8) >= 256) && wide * 2 == narrow ? TILE_128 : TILE_64;
+#ifdef FORCE_TILE
+        c.tile = FORCE_TILE;
+#endif
+        tiles = c.tile == TILE_128 ? wide : narrow;
+    } else if (direct && tiles_of(256) >= 200) {
         c.tile = TILE_256;
         tiles = tiles_of(256);
     } else if (tiles_of(128) >= 256 || tiles_of(128) * (steps / 8) >= 256 || direct) {
@@ -159,6 +171,23 @@ static size_t partial_bytes(int64_t M, int64_t N, int64_t K, int segs, int batch
     return most > 1 ? round_up((size_t)most * batch * M * N * (gated ? 2 : 1) * 4) : 0;
 }
 
+// float32: planes of split weights, for a forward (plane rows = weight rows) or a dx product (plane rows = weight columns).
+// From 1024 rows on: then at least eight row blocks share every weight, and splitting it once saves more vector work in the
+// product than the pass over the weights costs.
+struct Planes { int rows, ld; size_t plane, bytes; };
+static Planes planes_of(const v2vae_dense* d, bool gated, bool transposed) {
+    Planes p = {};
+    if (d->dtype != V2VAE_F32 || d->rows < 1024) return p;
+    auto pad = [](int64_t n) { return (n + 31) / 32 * 32; };
+    p.rows = (int)(transposed ? d->in : gated ? 2 * pad(d->out) : d->out);
+    p.ld = (int)(transposed ? pad(d->out) * (gated ? 2 : 1) : pad(d->in));
+    p.plane = (size_t)p.rows * p.ld * 2;
+    // a tile's lane offsets span all three planes in 32 bits, and its columns are counted in 31
+    if (2 * p.plane + (size_t)128 * p.ld * 2 >= (size_t)0xFFFF0000u) return Planes{};
+    p.bytes = round_up(3 * p.plane);
+    return p;
+}
+
 static void slope_shape(int64_t M, int64_t N, int V, int* cx, int* gx, int* chunks) {
     const int64_t cols = (N + V - 1) / V;
     int c = 1;
@@ -173,7 +202,7 @@ static void slope_shape(int64_t M, int64_t N, int V, int* cx, int* gx, int* chun
 }
 
 // workspace of the backward pass: dz (two for the gated block), the column partials, the partials of the two products
-struct BwdLayout { size_t dz[2], part[2], prod, total; };
+struct BwdLayout { size_t dz[2], part[2], planes, prod, total; };
 static BwdLayout bwd_layout(const v2vae_dense* d, bool gated) {
     BwdLayout l;
     const int n = gated ? 2 : 1;
@@ -189,6 +218,8 @@ static BwdLayout bwd_layout(const v2vae_dense* d, bool gated) {
         l.part[i] = o;
         if (i < n) o += round_up((size_t)(c1 > c4 ? c1 : c4) * d->out * 4);
     }
+    l.planes = o;
+    o += planes_of(d, gated, true).bytes;
     l.prod = o;
     const size_t a = partial_bytes(d->rows, d->in, d->out, n, 1, d->dtype, false);
     const size_t b = partial_bytes(d->out, d->in, d->rows, 1, n, d->dtype, false);
@@ -218,9 +249,17 @@ static int run_product(GemmArgs& g, int dtype, int layout, bool gated, float* pa
     g.steps_per_split = c.per;
     g.partial = c.splits > 1 ? partial : nullptr;
     if (direct) return dtype == V2VAE_BF16 ? gemm_direct_bf16(g, layout, gated, c.tile, st) : gemm_direct_f16(g, layout, gated, c.tile, st);
-    if (dtype == V2VAE_F32) return gemm_staged_f32(g, layout, gated, c.tile, st);
+    if (dtype == V2VAE_F32) return gemm_split(g, layout, gated, c.tile, st);
     if (dtype == V2VAE_BF16) return gemm_staged_bf16(g, layout, gated, c.tile, st);
     return gemm_staged_f16(g, layout, gated, c.tile, st);
+}
+
+static int use_planes(GemmArgs& g, const Planes& p, bool transposed, bool gated, char* at, hipStream_t st) {
+    g.planes = at;
+    g.plane_bytes = (int64_t)p.plane;
+    g.plane_rows = p.rows;
+    g.plane_ld = p.ld;
+    return split_planes(g, transposed, gated, transposed ? g.K : g.N, transposed ? g.N : g.K, st);
 }
 
 static int forward(const v2vae_dense* d, const void* x, const void* w0, const void* w1, const void* b0, const void* b1,
@@ -246,13 +285,18 @@ static int forward(const v2vae_dense* d, const void* x, const void* w0, const vo
     g.z[0] = z;
     g.z[1] = z ? z + (int64_t)d->rows * d->out : nullptr;
     g.act = d->activation;
+    const Planes p = planes_of(d, gated, false);
+    if (p.bytes) {
+        const int rc = use_planes(g, p, false, gated, (char*)ws, st);
+        if (rc != V2VAE_OK) return rc;
+    }
     if (d->rows <= ROWS_MAX) {
         const int e = 16 / elem_bytes(d->dtype);
         g.vec_a = aligned_to(x, 16) && d->ld_x % e == 0 && d->in % e == 0;
         g.vec_b = aligned_to(w0, 16) && d->ld_w % e == 0 && (!gated || (aligned_to(w1, 16) && d->ld_w2 % e == 0)) && d->in % e == 0;
         return dense_rows(g, d->dtype, gated, st);
     }
-    return run_product(g, d->dtype, LAYOUT_KK, gated, (float*)ws, st);
+    return run_product(g, d->dtype, LAYOUT_KK, gated, (float*)((char*)ws + p.bytes), st);
 }
 
 static int backward(const v2vae_dense* d, const void* x, const void* w0, const void* w1, const float* z, const void* dy, void* dx,
@@ -336,6 +380,11 @@ static int backward(const v2vae_dense* d, const void* x, const void* w0, const v
         g.K = (int)d->out;
         g.segs = gated ? 2 : 1;
         g.batch = 1;
+        const Planes p = planes_of(d, gated, true);
+        if (p.bytes && M > 0) {
+            const int rc = use_planes(g, p, true, gated, base + l.planes, st);
+            if (rc != V2VAE_OK) return rc;
+        }
         const int rc = run_product(g, d->dtype, LAYOUT_KM, false, prod, st);
         if (rc != V2VAE_OK) return rc;
     }
@@ -369,14 +418,14 @@ size_t v2vae_linear_workspace_bytes(const v2vae_dense* d, int backward) {
     if (check_dense(d, false, backward != 0, false) != V2VAE_OK) return 0;
     if (backward) return bwd_layout(d, false).total;
     if (d->rows <= ROWS_MAX) return 0;
-    return partial_bytes(d->rows, d->out, d->in, 1, 1, d->dtype, false);
+    return planes_of(d, false, false).bytes + partial_bytes(d->rows, d->out, d->in, 1, 1, d->dtype, false);
 }
 
 size_t v2vae_gated_workspace_bytes(const v2vae_dense* d, int backward) {
     if (check_dense(d, true, backward != 0, false) != V2VAE_OK) return 0;
     if (backward) return bwd_layout(d, true).total;
     if (d->rows <= ROWS_MAX) return 0;
-    return partial_bytes(d->rows, d->out, d->in, 1, 1, d->dtype, true);
+    return planes_of(d, true, false).bytes + partial_bytes(d->rows, d->out, d->in, 1, 1, d->dtype, true);
 }
 
 int v2vae_linear_fwd(const v2vae_dense* d, const void* x, const void* w, const void* bias, const void* residual, void* y, float* z,

@@ -28,8 +28,14 @@ __device__ __forceinline__ void load_to_lds(const void* at, unsigned lds) {
     lds = __builtin_amdgcn_readfirstlane(lds);
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(at), "s"(lds) : "memory", "m0");
 }
-// this wave's loads have landed and its LDS reads are done, then all waves'
-__device__ __forceinline__ void wait_tile() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// this wave's loads have landed and its LDS reads are done, then all waves' (the builtin, so that the compiler knows that its own
+// loads have arrived as well and asks for no wait of its own after the next ones are under way)
+__device__ __forceinline__ void wait_tile() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
 
 template <typename V> __device__ __forceinline__ V uniform64(V p) {
     const uint64_t u = (uint64_t)p;
@@ -97,6 +103,9 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN) / 4) void k_gemm_direct(Gem
     const int split = blockIdx.y, bat = blockIdx.z, m0 = tm * BM, n0 = tn * out_bn;
     const int steps_seg = (g.K + 63) / 64, steps = steps_seg * g.segs;
     const int s_lo = split * g.steps_per_split, s_hi = s_lo + g.steps_per_split < steps ? s_lo + g.steps_per_split : steps;
+    // operands of the two segments (a batch entry has one)
+    const void *const a_0 = g.a[bat], *const a_1 = g.a[1], *const b_0 = g.b[bat], *const b_1 = g.b[1];
+    const int64_t ldb_0 = g.ldb[bat], ldb_1 = g.ldb[1];
     const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
 
     Tile<T, BM, NW, AKC, false> ta;
@@ -104,14 +113,14 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN) / 4) void k_gemm_direct(Gem
     ta.init(lane, wave, g.lda, m0, g.M, nullptr);
     tb.init(lane, wave, g.ldb[bat], n0, g.N, g.ldb);
     auto fetch = [&](int s, int buf) {
-        const int seg = s >= steps_seg ? 1 : 0, k0 = (s - seg * steps_seg) * 64, sel = seg | bat, left = g.K - k0;
-        const char* a = (const char*)g.a[sel] + ((AKC ? (int64_t)m0 * g.lda + k0 : (int64_t)k0 * g.lda + m0) * 2);
+        const int seg = s >= steps_seg ? 1 : 0, k0 = (s - seg * steps_seg) * 64, left = g.K - k0;
+        const char* a = (const char*)(seg ? a_1 : a_0) + ((AKC ? (int64_t)m0 * g.lda + k0 : (int64_t)k0 * g.lda + m0) * 2);
         const char *b0, *b1 = nullptr;
         if constexpr (GATED) {
             b0 = (const char*)g.b[0] + ((int64_t)n0 * g.ldb[0] + k0) * 2;
             b1 = uniform64((const char*)g.b[1] + ((int64_t)n0 * g.ldb[1] + k0) * 2);
         } else {
-            b0 = (const char*)g.b[sel] + ((BKC ? (int64_t)n0 * g.ldb[sel] + k0 : (int64_t)k0 * g.ldb[sel] + n0) * 2);
+            b0 = (const char*)(seg ? b_1 : b_0) + ((BKC ? (int64_t)n0 * (seg ? ldb_1 : ldb_0) + k0 : (int64_t)k0 * (seg ? ldb_1 : ldb_0) + n0) * 2);
         }
         ta.fetch(uniform64(a), nullptr, left, lane, wave, lds0 + buf * STAGE);
         tb.fetch(uniform64(b0), b1, left, lane, wave, lds0 + buf * STAGE + BM * 128);

@@ -25,15 +25,16 @@ template <typename T, int ROWS> struct Stage<T, ROWS, true> {
     static constexpr int E = 16 / sizeof(T), PASS = ROWS / 32, BK = Elem<T>::BK, ROWB = BK * 2 + 16;
     Vec16<T> v[PASS];
     // row_of(r): pointer of tile row r at k = 0, or NULL beyond the matrix
-    template <typename F> __device__ __forceinline__ void load(int tid, int k0, int K, bool vec, F row_of) {
+    template <typename F> __device__ __forceinline__ void load(int tid, int k0, int K, F row_of) {
         const int k = k0 + (tid & 7) * E;
 #pragma unroll
         for (int j = 0; j < PASS; ++j) {
             const T* p = row_of((tid >> 3) + 32 * j);
             v[j].raw = u32x4{0, 0, 0, 0};
             if (p == nullptr) continue;
-            if (vec) {
-                if (k < K) v[j].raw = *reinterpret_cast<const u32x4*>(p + k);
+            struct __attribute__((packed, aligned(sizeof(T)))) Loose { u32x4 raw; };
+            if (k + E <= K) {
+                v[j].raw = reinterpret_cast<const Loose*>(p + k)->raw;
             } else {
 #pragma unroll
                 for (int e = 0; e < E; ++e)
@@ -191,8 +192,8 @@ __global__ __launch_bounds__(256, 2) void k_gemm_staged(GemmArgs g) {
                 return n < g.N ? b + (BKC ? (int64_t)n * g.ldb[sel] : (int64_t)n) : nullptr;
             }
         };
-        if constexpr (AKC) sa.load(tid, k0, g.K, g.vec_a != 0, row_a); else sa.load(tid, k0, g.K, g.lda, row_a);
-        if constexpr (BKC) sb.load(tid, k0, g.K, g.vec_b != 0, row_b); else sb.load(tid, k0, g.K, g.ldb[sel], row_b);
+        if constexpr (AKC) sa.load(tid, k0, g.K, row_a); else sa.load(tid, k0, g.K, g.lda, row_a);
+        if constexpr (BKC) sb.load(tid, k0, g.K, row_b); else sb.load(tid, k0, g.K, g.ldb[sel], row_b);
     };
 
     f32x16 acc[TM][TN];

@@ -1,11 +1,11 @@
 // One to sixteen rows through a dense layer or a gated block: the form that answers single symbols.
 //
-// The weights are read once and nothing else counts, so the kernel is a stream over them.  A workgroup of eight waves owns 16
-// weight rows (gated block: 16 gate and 16 up rows of the same features); the waves take turns along the contraction, 128 elements
-// each, and multiply on v_mfma_f32_16x16x32 with the input rows as the other operand (rows beyond the last repeat it): the matrix
+// The weights are read once and nothing else counts, so the kernel is a stream over them.  A workgroup owns 16 weight rows (gated
+// block: 8 gate and 8 up rows of the same features); its 16 waves (8 up to 1024 columns) take turns along the contraction, 128
+// elements each, and multiply on v_mfma_f32_16x16x32 with the input rows as the other operand (rows beyond the last repeat it): the matrix
 // instruction sums over lanes, which costs a vector kernel six shuffles per output and wave.  The fragments come straight from
 // memory (16 bytes a lane, any alignment); float operands are split into three bf16 pieces in registers (six products).  The
-// eight waves' sums are joined through LDS in a fixed order.
+// waves' sums are joined through LDS in a fixed order.
 #include "v2vae_dense.h"
 
 namespace v2vae {
@@ -46,70 +46,66 @@ template <typename T> __device__ __forceinline__ void pieces_of(const Eight<T>& 
     }
 }
 
-template <typename T, bool GATED> __global__ __launch_bounds__(512) void k_dense_rows(GemmArgs g) {
-    constexpr int NP = Elem<T>::NP, NB = GATED ? 2 : 1;
+template <typename T, int W, bool GATED> __global__ __launch_bounds__(64 * W) void k_dense_rows(GemmArgs g) {
+    constexpr int NP = Elem<T>::NP, FT = GATED ? 8 : 16;  // features of the workgroup
     typedef typename Elem<T>::frag frag;
-    __shared__ float s_sum[NB][8][16][17];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, kl = (lane >> 4) * 8, n0 = blockIdx.x * 16;
-    const int nc = n0 + r < g.N ? n0 + r : g.N - 1, mc = r < g.M ? r : g.M - 1;
-    const T* w[NB];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) w[b] = (const T*)g.b[b] + (int64_t)nc * g.ldb[b];
+    __shared__ float s_sum[W][16][17];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, kl = (lane >> 4) * 8, n0 = blockIdx.x * FT;
+    const int n = n0 + r % FT, nc = n < g.N ? n : g.N - 1, mc = r < g.M ? r : g.M - 1, which = GATED ? r >> 3 : 0;
+    const T* const w = (const T*)g.b[which] + (int64_t)nc * g.ldb[which];
     const T* const x = (const T*)g.a[0] + (int64_t)mc * g.lda;
-    acc4 acc[NB];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) acc[b] = acc4{0.f, 0.f, 0.f, 0.f};
+    acc4 acc = acc4{0.f, 0.f, 0.f, 0.f};
     auto chunk = [&](int k0, auto tail) {
-        Eight<T> wv[NB][4], xv[4];
+        Eight<T> wv[4], xv[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int k = k0 + i * 32 + kl;
-#pragma unroll
-            for (int b = 0; b < NB; ++b) wv[b][i] = load_eight<T, decltype(tail)::value>(w[b], k, g.K);
+            wv[i] = load_eight<T, decltype(tail)::value>(w, k, g.K);
             xv[i] = load_eight<T, decltype(tail)::value>(x, k, g.K);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            frag xf[NP];
+            frag xf[NP], wf[NP];
             pieces_of<T>(xv[i], xf);
+            pieces_of<T>(wv[i], wf);
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                frag wf[NP];
-                pieces_of<T>(wv[b][i], wf);
+            for (int sum = NP - 1; sum >= 0; --sum)
 #pragma unroll
-                for (int sum = NP - 1; sum >= 0; --sum)
-#pragma unroll
-                    for (int p = 0; p <= sum; ++p) acc[b] = mma16(wf[p], xf[sum - p], acc[b]);
-            }
+                for (int p = 0; p <= sum; ++p) acc = mma16(wf[p], xf[sum - p], acc);
         }
     };
     const int whole = g.K / 128 * 128;
 #pragma unroll 2
-    for (int k0 = wave * 128; k0 < whole; k0 += 8 * 128) chunk(k0, std::false_type());
-    if (whole < g.K && (whole / 128) % 8 == wave) chunk(whole, std::true_type());
+    for (int k0 = wave * 128; k0 < whole; k0 += W * 128) chunk(k0, std::false_type());
+    if (whole < g.K && (whole / 128) % W == wave) chunk(whole, std::true_type());
     // lane: input row lane % 16, weight rows 4 (lane / 16) ... + 3
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s_sum[b][wave][r][4 * (lane >> 4) + e] = acc[b][e];
+    for (int e = 0; e < 4; ++e) s_sum[wave][r][4 * (lane >> 4) + e] = acc[e];
     __syncthreads();
-    if (tid >= 256) return;
-    const int m = tid >> 4, f = tid & 15, n = n0 + f;
-    if (m >= g.M || n >= g.N) return;
-    float s[NB];
+    if (tid >= 16 * FT) return;
+    const int m = tid / FT, f = tid % FT;
+    if (m >= g.M || n0 + f >= g.N) return;
+    auto total = [&](int at) {
+        float s = 0.f;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        s[b] = 0.f;
-#pragma unroll
-        for (int q = 0; q < 8; ++q) s[b] += s_sum[b][q][m][f];
+        for (int q = 0; q < W; ++q) s += s_sum[q][m][at];
+        return s;
+    };
+    float s0 = total(f);
+    if constexpr (GATED) {
+        float s1 = total(f + 8);
+        finish_gated<T, 1>(g, m, n0 + f, &s0, &s1, true);
+    } else {
+        finish_value<T, 1>(g, m, n0 + f, &s0, 0, true);
     }
-    if constexpr (GATED) finish_gated<T, 1>(g, m, n, &s[0], &s[1], true); else finish_value<T, 1>(g, m, n, &s[0], 0, true);
 }
 
+template <typename T, int W> static void launch_waves(const GemmArgs& g, bool gated, hipStream_t st) {
+    if (gated) hipLaunchKernelGGL((k_dense_rows<T, W, true>), dim3((g.N + 7) / 8), dim3(64 * W), 0, st, g);
+    else hipLaunchKernelGGL((k_dense_rows<T, W, false>), dim3((g.N + 15) / 16), dim3(64 * W), 0, st, g);
+}
 template <typename T> static void launch_rows(const GemmArgs& g, bool gated, hipStream_t st) {
-    const dim3 grid((g.N + 15) / 16);
-    if (gated) hipLaunchKernelGGL((k_dense_rows<T, true>), grid, dim3(512), 0, st, g);
-    else hipLaunchKernelGGL((k_dense_rows<T, false>), grid, dim3(512), 0, st, g);
+    if (g.K > 1024) launch_waves<T, 16>(g, gated, st); else launch_waves<T, 8>(g, gated, st);
 }
 
 int dense_rows(const GemmArgs& g, int dtype, bool gated, hipStream_t st) {
