@@ -194,7 +194,8 @@ template <int C> __device__ __forceinline__ void act_columns(int kind, float v[C
         case V2VAE_ACT_TANH: all(std::integral_constant<int, V2VAE_ACT_TANH>()); break;
     }
 }
-template <typename T, int C> __device__ __forceinline__ void finish_value(const GemmArgs& g, int64_t m, int n, float s[C], int bat, bool whole) {
+template <typename T, int C> __device__ __forceinline__ void finish_value(const GemmArgs& g, int64_t m, int n, float s[C], int bat, bool whole,
+                                                                                       const T* res = nullptr) {
     const int count = g.N - n;
     float v[C];
     if (g.bias[0]) {
@@ -205,7 +206,12 @@ template <typename T, int C> __device__ __forceinline__ void finish_value(const 
     if (g.z[0]) store_columns<float, C>(g.z[0], m * g.N + n, count, whole, s);
     act_columns<C>(g.act, s);
     if (g.residual) {
-        load_columns<T, C>(g.residual, m * g.ldr + n, count, whole, v);
+        if (whole && res) {  // already here
+#pragma unroll
+            for (int e = 0; e < C; ++e) v[e] = (float)res[e];
+        } else {
+            load_columns<T, C>(g.residual, m * g.ldr + n, count, whole, v);
+        }
 #pragma unroll
         for (int e = 0; e < C; ++e) s[e] += v[e];
     }

@@ -19,14 +19,15 @@ namespace v2vae {
 
 __device__ __align__(16) const unsigned g_zero_piece[4] = {0, 0, 0, 0};
 
-// 64 lanes' pieces of 16 bytes from base + off to LDS at lds + 16 lane; not tracked by the compiler, wait_tile() waits for them
+// 64 lanes' pieces of 16 bytes from base + off to LDS at lds + 16 lane.  Not tracked by the compiler: wait_tile() waits for them and
+// is what LDS reads may not cross; between two of its calls reads and loads concern different tiles and may change places.
 __device__ __forceinline__ void load_to_lds(const void* base, unsigned off, unsigned lds) {
     lds = __builtin_amdgcn_readfirstlane(lds);
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "m0");
 }
 __device__ __forceinline__ void load_to_lds(const void* at, unsigned lds) {
     lds = __builtin_amdgcn_readfirstlane(lds);
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(at), "s"(lds) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(at), "s"(lds) : "m0");
 }
 // this wave's loads have landed and its LDS reads are done, then all waves' (the builtin, so that the compiler knows that its own
 // loads have arrived as well and asks for no wait of its own after the next ones are under way)
@@ -65,23 +66,20 @@ template <typename T, int ROWS, int NW, bool KC, bool GATED> struct Tile {
             }
         }
     }
-    // base0 (base1): corner at contraction index k0; left = contraction elements from k0 on
-    __device__ __forceinline__ void fetch(const char* base0, const char* base1, int left, int lane, int wave, unsigned lds) const {
-        if (left >= 64) {
+    // loads lo ... hi - 1 of this wave; base0 (base1): corner at contraction index k0, left = contraction elements from k0 on
+    template <bool TAIL> __device__ __forceinline__ void fetch(const char* base0, const char* base1, int left, int lane, int wave, unsigned lds,
+                                                               int lo, int hi) const {
 #pragma unroll
-            for (int j = 0; j < LOADS; ++j) {
-                const int i = j * NW + wave;
-                const char* b = GATED && (((i * 8) >> 5) & 1) ? base1 : base0;
-                load_to_lds(b, off[j], lds + i * 1024);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < LOADS; ++j) {
-                const int i = j * NW + wave;
-                const char* b = GATED && (((i * 8) >> 5) & 1) ? base1 : base0;
+        for (int j = 0; j < LOADS; ++j) {
+            if (j < lo || j >= hi) continue;
+            const int i = j * NW + wave;
+            const char* b = GATED && (((i * 8) >> 5) & 1) ? base1 : base0;
+            if constexpr (TAIL) {
                 int k;
                 if constexpr (KC) k = ((lane & 7) ^ (((i * 8 + (lane >> 3)) >> 1) & 7)) * 8; else k = (i * 64 + lane) / (ROWS / 8);
                 load_to_lds(k < left ? (const void*)(b + off[j]) : (const void*)g_zero_piece, lds + i * 1024);
+            } else {
+                load_to_lds(b, off[j], lds + i * 1024);
             }
         }
     }
@@ -92,8 +90,8 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN) / 4) void k_gemm_direct(Gem
     typedef typename Elem<T>::frag frag;
     typedef __attribute__((ext_vector_type(4))) short s16x4;
     constexpr int NW = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, STAGE = (BM + BN) * 128;
-    static_assert(!GATED || TN == 2, "a gated wave holds one gate and one up block");
-    static_assert(NW * EPI_BYTES<TN> <= 2 * STAGE, "the epilogue's rows fit the tiles' memory");
+    static_assert(TN % 2 == 0, "the epilogue takes blocks in pairs (gated: gate and up)");
+    static_assert(NW * EPI_BYTES<2> <= 2 * STAGE, "the epilogue's rows fit the tiles' memory");
     __shared__ __align__(1024) char lds[2 * STAGE];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
     const int out_bn = GATED ? BN / 2 : BN;
@@ -112,18 +110,45 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN) / 4) void k_gemm_direct(Gem
     Tile<T, BN, NW, BKC, GATED> tb;
     ta.init(lane, wave, g.lda, m0, g.M, nullptr);
     tb.init(lane, wave, g.ldb[bat], n0, g.N, g.ldb);
-    auto fetch = [&](int s, int buf) {
-        const int seg = s >= steps_seg ? 1 : 0, k0 = (s - seg * steps_seg) * 64, left = g.K - k0;
-        const char* a = (const char*)(seg ? a_1 : a_0) + ((AKC ? (int64_t)m0 * g.lda + k0 : (int64_t)k0 * g.lda + m0) * 2);
-        const char *b0, *b1 = nullptr;
-        if constexpr (GATED) {
-            b0 = (const char*)g.b[0] + ((int64_t)n0 * g.ldb[0] + k0) * 2;
-            b1 = uniform64((const char*)g.b[1] + ((int64_t)n0 * g.ldb[1] + k0) * 2);
+    // where the next tile comes from: corners of both operands at its contraction index, what is left of its segment
+    const int64_t step_a = (AKC ? 64 : 64 * g.lda) * 2;
+    const char *pa, *pb, *pb1 = nullptr;
+    int left, seg;
+    int64_t step_b;
+    auto enter = [&](int sg, int k0) {
+        seg = sg;
+        left = g.K - k0;
+        const int64_t ldb = sg ? ldb_1 : ldb_0;
+        step_b = (BKC ? 64 : 64 * ldb) * 2;
+        pa = uniform64((const char*)(sg ? a_1 : a_0) + (AKC ? (int64_t)m0 * g.lda + k0 : (int64_t)k0 * g.lda + m0) * 2);
+        pb = uniform64((const char*)(sg ? b_1 : b_0) + (BKC ? (int64_t)n0 * ldb + k0 : (int64_t)k0 * ldb + n0) * 2);
+        if constexpr (GATED) pb1 = uniform64((const char*)b_1 + ((int64_t)n0 * ldb_1 + k0) * 2);
+    };
+    int at_step = 0;  // step that the corners stand at
+    auto go_to = [&](int s) {
+        at_step = s;
+        enter(s >= steps_seg ? 1 : 0, (s >= steps_seg ? s - steps_seg : s) * 64);
+    };
+    auto advance = [&]() {
+        ++at_step;
+        if (at_step < s_hi && left > 64) {
+            left -= 64;
+            pa += step_a;
+            pb += step_b;
+            if constexpr (GATED) pb1 += step_b;
         } else {
-            b0 = (const char*)(seg ? b_1 : b_0) + ((BKC ? (int64_t)n0 * (seg ? ldb_1 : ldb_0) + k0 : (int64_t)k0 * (seg ? ldb_1 : ldb_0) + n0) * 2);
+            go_to(at_step < s_hi ? at_step : s_lo);
         }
-        ta.fetch(uniform64(a), nullptr, left, lane, wave, lds0 + buf * STAGE);
-        tb.fetch(uniform64(b0), b1, left, lane, wave, lds0 + buf * STAGE + BM * 128);
+    };
+    constexpr int LA = Tile<T, BM, NW, AKC, false>::LOADS, LB = Tile<T, BN, NW, BKC, GATED>::LOADS;
+    auto fetch = [&](int buf, int lo, int hi) {  // loads lo ... hi - 1 of the next tile, A's first
+        if (left >= 64) {
+            ta.template fetch<false>(pa, nullptr, left, lane, wave, lds0 + buf * STAGE, lo, hi);
+            tb.template fetch<false>(pb, pb1, left, lane, wave, lds0 + buf * STAGE + BM * 128, lo - LA, hi - LA);
+        } else {
+            ta.template fetch<true>(pa, nullptr, left, lane, wave, lds0 + buf * STAGE, lo, hi);
+            tb.template fetch<true>(pb, pb1, left, lane, wave, lds0 + buf * STAGE + BM * 128, lo - LA, hi - LA);
+        }
     };
 
     f32x16 acc[TM][TN];
@@ -164,37 +189,73 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN) / 4) void k_gemm_direct(Gem
     };
     typedef __attribute__((address_space(3))) frag lds_frag;
 
-    if (s_lo < s_hi) fetch(s_lo, 0);
-    for (int s = s_lo; s < s_hi; ++s) {
-        const int buf = (s - s_lo) & 1;
-        wait_tile();
-        if (s + 1 < s_hi) fetch(s + 1, buf ^ 1);
-        const unsigned la = lds0 + buf * STAGE, lb = la + BM * 128;
+    auto read = [&](unsigned la, int kk, frag (&a)[TM], frag (&b)[TN]) {
+        const unsigned lb = la + BM * 128;
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-            frag a[TM], b[TN];
-#pragma unroll
-            for (int i = 0; i < TM; ++i) {
-                if constexpr (AKC) a[i] = *(const lds_frag*)(uintptr_t)(la + oa[kk] + i * 4096);
-                else a[i] = frag_mn(la + oa[i], BM, kk);
-            }
-#pragma unroll
-            for (int j = 0; j < TN; ++j) {
-                if constexpr (BKC) b[j] = *(const lds_frag*)(uintptr_t)(lb + ob[kk] + j * 4096);
-                else b[j] = frag_mn(lb + ob[j], BN, kk);
-            }
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] = mma32(b[j], a[i], acc[i][j]);
+        for (int j = 0; j < TN; ++j) {
+            if constexpr (BKC) b[j] = *(const lds_frag*)(uintptr_t)(lb + ob[kk] + j * 4096);
+            else b[j] = frag_mn(lb + ob[j], BN, kk);
         }
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            if constexpr (AKC) a[i] = *(const lds_frag*)(uintptr_t)(la + oa[kk] + i * 4096);
+            else a[i] = frag_mn(la + oa[i], BM, kk);
+        }
+    };
+    // Neighbouring tiles start up to seven steps apart in the contraction and wrap round: rows a power of two apart would otherwise
+    // have every workgroup ask the same few cache channels for the same 128-byte column of the operands at a time.
+    const int n_steps = s_hi - s_lo;
+    frag a[2][TM], b[2][TN];
+    auto products = [&](int q) {
+        // reads that were just written down are issued before these products, not where their fragments are used
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] = mma32(b[q][j], a[q][i], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    if (n_steps > 0) {
+        go_to(s_lo + (n_steps >= 16 ? (int)((blockIdx.x >> 3) & 7) : 0));
+        fetch(0, 0, LA + LB);
+        wait_tile();
+        if (n_steps > 1) {
+            advance();
+            fetch(1, 0, LA + LB);
+        }
+        read(lds0, 0, a[0], b[0]);
+    }
+    for (int i = 0; i < n_steps; ++i) {
+        const int buf = i & 1;
+        const unsigned here = lds0 + buf * STAGE;
+        read(here, 1, a[1], b[1]);
+        products(0);
+        read(here, 2, a[0], b[0]);
+        products(1);
+        read(here, 3, a[1], b[1]);
+        products(0);
+        // The tile is read; while its last products run, the next one's first fragments come in and the one after it is asked for.
+        if (i + 1 < n_steps) {
+            wait_tile();
+            read(lds0 + (buf ^ 1) * STAGE, 0, a[0], b[0]);
+            if (i + 2 < n_steps) {
+                advance();
+                fetch(buf, 0, LA + LB);
+            }
+        }
+        products(1);
     }
 
     wait_tile();  // LDS is free
     float* const part = g.partial ? g.partial + ((int64_t)bat * g.splits + split) * ((int64_t)g.M * (GATED ? 2 : 1) * g.N) : nullptr;
 #pragma unroll
     for (int i = 0; i < TM; ++i)
-        finish_block<T, TN, GATED>(g, acc[i], lds + wave * EPI_BYTES<TN>, lane, m0 + (wm * TM + i) * 32, n0 + wn * (GATED ? 32 : 32 * TN), part, bat);
+#pragma unroll
+        for (int j = 0; j < TN; j += 2) {
+            const f32x16 pair[2] = {acc[i][j], acc[i][j + 1]};
+            finish_block<T, 2, GATED>(g, pair, lds + wave * EPI_BYTES<2>, lane, m0 + (wm * TM + i) * 32,
+                                      n0 + (wn * TN + j) * (GATED ? 16 : 32), part, bat);
+        }
 }
 
 template <typename T, int WM, int WN, int TM, int TN, bool AKC, bool BKC, bool GATED> void launch_direct(const GemmArgs& g, hipStream_t st) {

@@ -125,9 +125,20 @@ __device__ __forceinline__ void finish_block(const GemmArgs& g, const f32x16 (&a
     __builtin_amdgcn_wave_barrier();
     const int c = (lane % PER) * 8, n = n0 + c;
     const bool whole = g.vec_c;  // N is a multiple of 8 then
+    // the residual of a row is asked for while the row before it is finished
+    struct alignas(8 * sizeof(T) > 16 ? 16 : 8 * sizeof(T)) T8 { T e[8]; };
+    const bool fetched = !GATED && !part && g.residual && whole;
+    auto residual_at = [&](int r) {
+        const int64_t m = m0 + r < g.M ? m0 + r : g.M - 1;
+        return *reinterpret_cast<const T8*>((const T*)g.residual + m * g.ldr + (n < g.N ? n : 0));
+    };
+    T8 next;
+    if (fetched) next = residual_at(lane / PER);
 #pragma unroll 1
     for (int r = lane / PER; r < 32; r += ROWS) {
         const int64_t m = m0 + r;
+        const T8 res = next;
+        if (fetched && r + ROWS < 32) next = residual_at(r + ROWS);
         if (m >= g.M || n >= g.N) continue;
         float s[8], u[8];
         const f32x4* p = reinterpret_cast<const f32x4*>(lds + r * ROWB + c * 4);
@@ -148,7 +159,7 @@ __device__ __forceinline__ void finish_block(const GemmArgs& g, const f32x16 (&a
         } else if constexpr (GATED) {
             finish_gated<T, 8>(g, m, n, s, u, whole);
         } else {
-            finish_value<T, 8>(g, m, n, s, bat, whole);
+            finish_value<T, 8>(g, m, n, s, bat, whole, res.e);
         }
     }
 }

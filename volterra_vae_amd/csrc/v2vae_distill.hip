@@ -77,8 +77,9 @@ template <int G> struct Lanes {
 };
 
 constexpr float LOG2E = 1.4426950408889634f;
-// exp(s - m) for scaled values: the difference first (exact where it matters), then the base-2 exponential of the hardware
-__device__ __forceinline__ float exp_diff(float z, float zmax, float c) { return __builtin_amdgcn_exp2f((z - zmax) * c); }
+// exp((z - m) / T) for c = log2(e) / T: the difference first (exact where it matters, finite for the type's lowest values), then the
+// base-2 exponential of the hardware
+__device__ __forceinline__ float exp_diff(float z, float m, float c) { return __builtin_amdgcn_exp2f((z - m) * c); }
 
 // G lanes a row, NV 16-byte pieces of the row held by each lane (HELD), or the row read once per pass.  MODE: DO_LOSS | DO_GRAD.
 // A DO_GRAD pass alone takes maximum and sum from `stats`.  ONE: k <= G, every lane has at most one teacher entry and keeps it.
@@ -122,30 +123,35 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void k_distill(DistillArgs a) {
     }
 
     const float c = a.inv_t * LOG2E;
-    Vec16<T> held[HELD ? NV : 1];
+    auto finite = [](float m) { return m == -INFINITY ? 0.f : m; };
+    // the row in registers: logits, then their exponentials in place
+    float held[HELD ? NV : 1][E];
     float zmax = -INFINITY, l = 0.f;
     if constexpr (HELD) {
+        Vec16<T> raw[NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            if (tid + i * G < pieces) held[i] = get(tid + i * G);
-            else {
+        for (int i = 0; i < NV; ++i)
+            if (tid + i * G < pieces) raw[i] = get(tid + i * G);
 #pragma unroll
-                for (int e = 0; e < E; ++e) held[i].e[e] = (T)(-INFINITY);
-            }
-        }
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < E; ++e) held[i][e] = tid + i * G < pieces ? (float)raw[i].e[e] : -INFINITY;
     }
     if constexpr (!STATS_GIVEN) {
         if constexpr (HELD) {
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll
-                for (int e = 0; e < E; ++e) zmax = fmaxf(zmax, (float)held[i].e[e]);
+                for (int e = 0; e < E; ++e) zmax = fmaxf(zmax, held[i][e]);
             zmax = lanes.max(zmax);
-            const float zm = zmax == -INFINITY ? 0.f : zmax;
+            const float zm = finite(zmax);
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll
-                for (int e = 0; e < E; ++e) l += exp_diff((float)held[i].e[e], zm, c);
+                for (int e = 0; e < E; ++e) {
+                    held[i][e] = exp_diff(held[i][e], zm, c);
+                    l += held[i][e];
+                }
             l = lanes.sum(l);
         } else {
             // one pass with a running maximum per thread, joined at the end
@@ -159,9 +165,8 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void k_distill(DistillArgs a) {
                     l *= exp_diff(mine, top, c);
                     mine = top;
                 }
-                const float zm = mine == -INFINITY ? 0.f : mine;
 #pragma unroll
-                for (int e = 0; e < E; ++e) l += exp_diff((float)v.e[e], zm, c);
+                for (int e = 0; e < E; ++e) l += exp_diff((float)v.e[e], finite(mine), c);
             }
             zmax = lanes.max(mine);
             l = lanes.sum(mine == -INFINITY ? l : l * exp_diff(mine, zmax, c));
@@ -174,7 +179,7 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void k_distill(DistillArgs a) {
         zmax = a.stats[2 * row];
         l = a.stats[2 * row + 1];
     }
-    const float zm = zmax == -INFINITY ? 0.f : zmax;
+    const float zm = finite(zmax);
 
     // the teacher's entries: probabilities over the present ones
     float tmax = -INFINITY;
@@ -222,10 +227,10 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void k_distill(DistillArgs a) {
         const float inv_l = l == 0.f ? 0.f : 1.f / l, scale = wt * inv_l;
         T* const out = (T*)a.grad + row * a.V;
         const bool same_phase = (int)(((uintptr_t)out & 15) / sizeof(T)) == off;
-        auto put = [&](int i, const Vec16<T>& v) {
+        auto put = [&](int i, const float (&v)[E]) {  // exponentials of piece i
             Vec16<T> o;
 #pragma unroll
-            for (int e = 0; e < E; ++e) o.e[e] = (T)(live ? exp_diff((float)v.e[e], zm, c) * scale : 0.f);
+            for (int e = 0; e < E; ++e) o.e[e] = (T)(live ? v[e] * scale : 0.f);
             const int lo = i * E - off;
             if (same_phase && lo >= 0 && lo + E <= a.V) {
                 *reinterpret_cast<u32x4*>(out + lo) = o.raw;
@@ -236,11 +241,23 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void k_distill(DistillArgs a) {
             }
         };
         if constexpr (HELD) {
+            if constexpr (STATS_GIVEN) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) held[i][e] = exp_diff(held[i][e], zm, c);
+            }
 #pragma unroll
             for (int i = 0; i < NV; ++i)
                 if (tid + i * G < pieces) put(tid + i * G, held[i]);
         } else {
-            for (int i = tid; i < pieces; i += G) put(i, get(i));
+            for (int i = tid; i < pieces; i += G) {
+                const Vec16<T> v = get(i);
+                float ev[E];
+#pragma unroll
+                for (int e = 0; e < E; ++e) ev[e] = exp_diff((float)v.e[e], zm, c);
+                put(i, ev);
+            }
         }
         if constexpr (G > 64) {
             for (int j = tid; j < a.k; j += G) {

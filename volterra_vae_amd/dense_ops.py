@@ -154,15 +154,20 @@ def linear_backward(dy, x, weight, z=None, *, activation="none", need=(True, Tru
     act = _activation(activation)
     _check_tensor(x, "x", 2)
     _check_layer(x, weight, "weight", None, "")
-    m, k, n = x.shape[0], x.shape[1], weight.shape[0]
+    m, n = x.shape[0], weight.shape[0]
     _check_grad(dy, "dy", x, n)
     if act:
         if z is None:
             raise ValueError("z: the pre-activations of linear_forward(..., keep=True) are needed with an activation")
         _check_kept(z, (m, n), x)
+    return _linear_backward(dy, x, weight, z, act, need)
+
+
+def _linear_backward(dy, x, weight, z, act, need):
+    m, k, n = x.shape[0], x.shape[1], weight.shape[0]
     d = _dense(x, weight, act, dy=dy)
     with _On(x) as stream:
-        new = lambda wanted, *shape: torch.empty(shape, dtype=x.dtype, device=x.device) if wanted else None  # noqa: E731
+        new = lambda wanted, *shape: x.new_empty(shape) if wanted else None  # noqa: E731
         dx, dw, db = new(need[0], m, k), new(need[1], n, k), new(need[2], n)
         ws = _workspace(False, 1, act, x, n)
         check(lib.v2vae_linear_bwd(d, _p(x), _p(weight), _p(z) if act else None, _p(dy), _p(dx), _p(dw), _p(db), _p(ws), stream),
@@ -187,7 +192,7 @@ class _Linear(torch.autograd.Function):
         dx = dw = db = None
         if any(need[:3]):
             g = dy if dy.shape[1] <= 1 or dy.stride(1) == 1 else dy.contiguous()
-            dx, dw, db = linear_backward(g, x, weight, z, activation=ctx.activation, need=need[:3])
+            dx, dw, db = _linear_backward(g, x, weight, z, ACTIVATIONS[ctx.activation], need)
         return dx, dw, db, dy if need[3] else None, None
 
 
@@ -248,12 +253,17 @@ def gated_backward(dh, x, weight_gate, weight_up, gu, *, activation="silu", need
     _check_layer(x, weight_up, "weight_up", None, "")
     if weight_up.shape != weight_gate.shape:
         raise ValueError(f"weight_up: expected {tuple(weight_gate.shape)}, got {tuple(weight_up.shape)}")
-    m, k, n = x.shape[0], x.shape[1], weight_gate.shape[0]
+    m, n = x.shape[0], weight_gate.shape[0]
     _check_grad(dh, "dh", x, n)
     _check_kept(gu, (2, m, n), x)
+    return _gated_backward(dh, x, weight_gate, weight_up, gu, act, need)
+
+
+def _gated_backward(dh, x, weight_gate, weight_up, gu, act, need):
+    m, k, n = x.shape[0], x.shape[1], weight_gate.shape[0]
     d = _dense(x, weight_gate, act, w2=weight_up, dy=dh)
     with _On(x) as stream:
-        new = lambda wanted, *shape: torch.empty(shape, dtype=x.dtype, device=x.device) if wanted else None  # noqa: E731
+        new = lambda wanted, *shape: x.new_empty(shape) if wanted else None  # noqa: E731
         out = [new(need[0], m, k), new(need[1], n, k), new(need[2], n, k), new(need[3], n), new(need[4], n)]
         ws = _workspace(True, 1, act, x, n)
         check(lib.v2vae_gated_bwd(d, _p(x), _p(weight_gate), _p(weight_up), _p(gu), _p(dh), *[_p(t) for t in out], _p(ws), stream),
@@ -274,7 +284,7 @@ class _Gated(torch.autograd.Function):
     def backward(ctx, dh):
         x, weight_gate, weight_up, gu = ctx.saved_tensors
         g = dh if dh.shape[1] <= 1 or dh.stride(1) == 1 else dh.contiguous()
-        return (*gated_backward(g, x, weight_gate, weight_up, gu, activation=ctx.activation, need=ctx.needs_input_grad[:5]), None)
+        return (*_gated_backward(g, x, weight_gate, weight_up, gu, ACTIVATIONS[ctx.activation], ctx.needs_input_grad), None)
 
 
 def gated_linear(x: torch.Tensor, weight_gate: torch.Tensor, weight_up: torch.Tensor, bias_gate: Optional[torch.Tensor] = None,
@@ -327,7 +337,7 @@ def topk_distillation_step(logits, teacher_logits, teacher_index, row_weight, *,
     _check_weight(row_weight, logits)
     with _On(logits) as stream:
         loss = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        grad = logits.new_empty(logits.shape)
         check(lib.v2vae_distill_step(d, _p(logits), _p(teacher_logits), _p(teacher_index), _p(row_weight), _p(loss), _p(grad), stream),
               "v2vae_distill_step")
     return loss, grad
@@ -336,26 +346,24 @@ def topk_distillation_step(logits, teacher_logits, teacher_index, row_weight, *,
 class _Distillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher_logits, teacher_index, temperature):
-        loss, stats = _distill_forward(logits, teacher_logits, teacher_index, temperature, True)
+        ctx.d = _distill(logits, teacher_logits, teacher_index, temperature)
+        loss, stats = _distill_forward(ctx.d, logits, teacher_logits, teacher_index, True)
         ctx.save_for_backward(logits, teacher_logits, teacher_index, stats)
-        ctx.temperature = temperature
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, weight):
         logits, teacher_logits, teacher_index, stats = ctx.saved_tensors
-        d = _distill(logits, teacher_logits, teacher_index, ctx.temperature)
         weight = weight.contiguous()
         with _On(logits) as stream:
-            grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-            check(lib.v2vae_distill_bwd(d, _p(logits), _p(teacher_logits), _p(teacher_index), _p(stats), _p(weight), _p(grad), stream),
+            grad = logits.new_empty(logits.shape)
+            check(lib.v2vae_distill_bwd(ctx.d, _p(logits), _p(teacher_logits), _p(teacher_index), _p(stats), _p(weight), _p(grad), stream),
                   "v2vae_distill_bwd")
         return grad, None, None, None
 
 
-def _distill_forward(logits, teacher_logits, teacher_index, temperature, keep):
-    d = _distill(logits, teacher_logits, teacher_index, temperature)
+def _distill_forward(d, logits, teacher_logits, teacher_index, keep):
     with _On(logits) as stream:
         loss = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
         stats = torch.empty((logits.shape[0], 2), dtype=torch.float32, device=logits.device) if keep else None
@@ -377,7 +385,8 @@ def topk_distillation(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
         raise ValueError("teacher_logits: the loss is not differentiable in the teacher (pass teacher_logits.detach())")
     if isinstance(logits, torch.Tensor) and _grads_wanted(logits):
         return _Distillation.apply(logits, teacher_logits, teacher_index, temperature)
-    return _distill_forward(logits, teacher_logits, teacher_index, temperature, False)[0]
+    d = _distill(logits, teacher_logits, teacher_index, temperature)
+    return _distill_forward(d, logits, teacher_logits, teacher_index, False)[0]
 
 
 # ------------------------------------------------------------------------------------------------ registered ops
