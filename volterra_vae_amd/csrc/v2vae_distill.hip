@@ -40,35 +40,28 @@ __device__ __forceinline__ int class_at(const DistillArgs& a, int64_t row, int j
     return c < 0 ? -1 : c >= a.V ? -2 : (int)c;
 }
 
-// Reductions over the lanes of a group: G lanes of a wave, or all 1024 / 256 threads of a workgroup through LDS.  Every lane
-// gets the result; the order is fixed.
+// Reductions over the lanes of a group: G lanes of a wave, or all threads of a workgroup through LDS (one barrier: every reduction of
+// a kernel has a slot of its own).  Every lane gets the result; the order is fixed.
 template <int G> struct Lanes {
     float* scratch;
-    __device__ __forceinline__ float max(float v) const {
+    template <typename F> __device__ __forceinline__ float join(float v, int slot, F f) const {
 #pragma unroll
-        for (int d = (G < 64 ? G : 64) / 2; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
+        for (int d = (G < 64 ? G : 64) / 2; d > 0; d >>= 1) v = f(v, __shfl_xor(v, d));
         if constexpr (G > 64) {
+            float* const at = scratch + slot * (G / 64);
+            if ((threadIdx.x & 63) == 0) at[threadIdx.x >> 6] = v;
             __syncthreads();
-            if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
-            __syncthreads();
-            v = scratch[0];
+            v = at[0];
 #pragma unroll
-            for (int i = 1; i < G / 64; ++i) v = fmaxf(v, scratch[i]);
+            for (int i = 1; i < G / 64; ++i) v = f(v, at[i]);
         }
         return v;
     }
-    __device__ __forceinline__ float sum(float v) const {
-#pragma unroll
-        for (int d = (G < 64 ? G : 64) / 2; d > 0; d >>= 1) v += __shfl_xor(v, d);
-        if constexpr (G > 64) {
-            __syncthreads();
-            if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
-            __syncthreads();
-            v = scratch[0];
-#pragma unroll
-            for (int i = 1; i < G / 64; ++i) v += scratch[i];
-        }
-        return v;
+    __device__ __forceinline__ float max(float v, int slot) const {
+        return join(v, slot, [](float x, float y) { return fmaxf(x, y); });
+    }
+    __device__ __forceinline__ float sum(float v, int slot) const {
+        return join(v, slot, [](float x, float y) { return x + y; });
     }
     __device__ __forceinline__ void sync() const {
         if constexpr (G > 64) __syncthreads();
@@ -82,15 +75,18 @@ constexpr float LOG2E = 1.4426950408889634f;
 __device__ __forceinline__ float exp_diff(float z, float m, float c) { return __builtin_amdgcn_exp2f((z - m) * c); }
 
 // G lanes a row, NV 16-byte pieces of the row held by each lane (HELD), or the row read once per pass.  MODE: DO_LOSS | DO_GRAD.
-// A DO_GRAD pass alone takes maximum and sum from `stats`.  ONE: k <= G, every lane has at most one teacher entry and keeps it.
+// A DO_GRAD pass alone takes maximum and sum from `stats`.  ONE: the teacher's entries fit the lanes of one wave (k <= G and
+// k <= 64): each of them keeps one, and everything about them happens there while the row is on its way.
 template <typename T, int G, int NV, bool HELD, int MODE, bool ONE>
 __global__ __launch_bounds__(G > 64 ? G : 256) void k_distill(DistillArgs a) {
-    constexpr int E = Vec16<T>::N, ROWS = G > 64 ? 1 : 256 / G;
-    constexpr bool STATS_GIVEN = MODE == DO_GRAD;
-    __shared__ float s_red[16];
-    __shared__ float s_p[V2VAE_DISTILL_MAX_K > 0 ? (G > 64 ? V2VAE_DISTILL_MAX_K : 1) : 1];
-    __shared__ int s_c[G > 64 ? V2VAE_DISTILL_MAX_K : 1];
+    constexpr int E = Vec16<T>::N, ROWS = G > 64 ? 1 : 256 / G, GE = G > 64 ? 64 : G;
+    constexpr bool STATS_GIVEN = MODE == DO_GRAD, LISTS = G > 64 && !ONE;
+    __shared__ float s_red[G > 64 ? 5 * (G / 64) : 1];
+    __shared__ int s_state;
+    __shared__ float s_p[LISTS ? V2VAE_DISTILL_MAX_K : 1];
+    __shared__ int s_c[LISTS ? V2VAE_DISTILL_MAX_K : 1];
     const Lanes<G> lanes{s_red};
+    const Lanes<GE> wave{nullptr};
     const int tid = G > 64 ? threadIdx.x : threadIdx.x % G;
     const int64_t row = (int64_t)blockIdx.x * ROWS + (G > 64 ? 0 : threadIdx.x / G);
     if (row >= a.rows) return;  // G > 64: a workgroup has one row; G <= 64: whole groups leave, shuffles stay within a group
@@ -110,28 +106,57 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void k_distill(DistillArgs a) {
         }
         return v;
     };
-
-    // entry and its logit, asked for before the row so that they arrive with it
-    int my_cls = -1;
-    float my_t = 0.f, my_z = 0.f;
-    if constexpr (ONE) {
-        if (tid < a.k) {
-            my_cls = class_at(a, row, tid);
-            my_t = teacher_at(a, row, tid);
-            if (my_cls >= 0) my_z = (float)z[my_cls];
-        }
-    }
-
     const float c = a.inv_t * LOG2E;
     auto finite = [](float m) { return m == -INFINITY ? 0.f : m; };
-    // the row in registers: logits, then their exponentials in place
-    float held[HELD ? NV : 1][E];
-    float zmax = -INFINITY, l = 0.f;
+
+    Vec16<T> raw[HELD ? NV : 1];
     if constexpr (HELD) {
-        Vec16<T> raw[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i)
             if (tid + i * G < pieces) raw[i] = get(tid + i * G);
+    }
+
+    // The teacher's entries: p = softmax over the present ones.  ONE: lane j has entry j; p_all and `first` merge what names one
+    // class twice.
+    enum { NOTHING, SOME, BAD };
+    int state = NOTHING, my_cls = -1;
+    float my_p = 0.f, my_lp = 0.f, my_z = 0.f, p_all = 0.f, tmax = -INFINITY, inv_mass = 0.f, log_mass = 0.f;
+    bool first = true;
+    if constexpr (ONE) {
+        if (tid < GE) {
+            float t = -INFINITY;
+            if (tid < a.k) {
+                my_cls = class_at(a, row, tid);
+                t = teacher_at(a, row, tid);
+                if (my_cls >= 0) my_z = (float)z[my_cls];
+            }
+            // a class beyond the vocabulary, a NaN: as +inf, which makes the row NaN
+            tmax = wave.max(my_cls == -2 || (my_cls >= 0 && t != t) ? INFINITY : my_cls >= 0 ? t : -INFINITY, 0);
+            state = tmax == INFINITY ? BAD : tmax == -INFINITY ? NOTHING : SOME;
+            const float lt = (t - tmax) * a.inv_t, e = my_cls >= 0 && state == SOME ? expf(lt) : 0.f;
+            const float mass = wave.sum(e, 0);
+            if (state == SOME) {
+                my_p = e / mass;
+                my_lp = lt - logf(mass);
+            }
+            if constexpr (MODE & DO_GRAD) {
+                for (int i = 0; i < a.k; ++i) {  // all lanes of the group, entry or not
+                    const int ci = __shfl(my_cls, i, GE);
+                    const float pi = __shfl(my_p, i, GE);
+                    if (ci == my_cls) {
+                        p_all += pi;
+                        first &= i >= tid;
+                    }
+                }
+            }
+            if (G > 64 && tid == 0) s_state = state;  // read behind the barriers below
+        }
+    }
+
+    // the row: logits, then their exponentials in place
+    float held[HELD ? NV : 1][E];
+    float zmax = -INFINITY, l = 0.f;
+    if constexpr (HELD) {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -143,7 +168,7 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void k_distill(DistillArgs a) {
             for (int i = 0; i < NV; ++i)
 #pragma unroll
                 for (int e = 0; e < E; ++e) zmax = fmaxf(zmax, held[i][e]);
-            zmax = lanes.max(zmax);
+            zmax = lanes.max(zmax, 0);
             const float zm = finite(zmax);
 #pragma unroll
             for (int i = 0; i < NV; ++i)
@@ -152,7 +177,7 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void k_distill(DistillArgs a) {
                     held[i][e] = exp_diff(held[i][e], zm, c);
                     l += held[i][e];
                 }
-            l = lanes.sum(l);
+            l = lanes.sum(l, 1);
         } else {
             // one pass with a running maximum per thread, joined at the end
             float mine = -INFINITY;
@@ -168,8 +193,8 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void k_distill(DistillArgs a) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) l += exp_diff((float)v.e[e], finite(mine), c);
             }
-            zmax = lanes.max(mine);
-            l = lanes.sum(mine == -INFINITY ? l : l * exp_diff(mine, zmax, c));
+            zmax = lanes.max(mine, 0);
+            l = lanes.sum(mine == -INFINITY ? l : l * exp_diff(mine, zmax, c), 1);
         }
         if (a.stats && tid == 0) {
             a.stats[2 * row] = zmax;
@@ -178,52 +203,52 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void k_distill(DistillArgs a) {
     } else {
         zmax = a.stats[2 * row];
         l = a.stats[2 * row + 1];
+        if constexpr (G > 64 && ONE) __syncthreads();
     }
-    const float zm = finite(zmax);
+    const float zm = finite(zmax), log_l = logf(l);
+    if constexpr (G > 64 && ONE) state = s_state;
 
-    // the teacher's entries: probabilities over the present ones
-    float tmax = -INFINITY;
-    int bad = 0;
-    for (int j = tid; j < a.k; j += G) {
-        const int cls = ONE ? my_cls : class_at(a, row, j);
-        const float t = ONE ? my_t : teacher_at(a, row, j);
-        bad |= cls == -2 || (cls >= 0 && t != t);  // a class beyond the vocabulary, a NaN
-        if (cls >= 0) tmax = fmaxf(tmax, t);
-        if (ONE) break;
+    if constexpr (!ONE) {
+        int bad = 0;
+        for (int j = tid; j < a.k; j += G) {
+            const int cls = class_at(a, row, j);
+            const float t = teacher_at(a, row, j);
+            bad |= cls == -2 || (cls >= 0 && t != t);
+            if (cls >= 0) tmax = fmaxf(tmax, t);
+        }
+        tmax = lanes.max(bad ? INFINITY : tmax, 2);
+        state = tmax == INFINITY ? BAD : tmax == -INFINITY ? NOTHING : SOME;
+        float mass = 0.f;
+        for (int j = tid; j < a.k && state == SOME; j += G)
+            if (class_at(a, row, j) >= 0) mass += expf((teacher_at(a, row, j) - tmax) * a.inv_t);
+        mass = lanes.sum(mass, 3);
+        if (state == SOME) {
+            inv_mass = 1.f / mass;
+            log_mass = logf(mass);
+        }
     }
-    tmax = lanes.max(bad ? INFINITY : tmax);       // +inf, from here or among the logits: the row is NaN
-    const bool any_bad = tmax == INFINITY;
-    float mass = 0.f, my_p = 0.f;
-    const bool there = tmax != -INFINITY;
-    for (int j = tid; j < a.k && there; j += G) {
-        const int cls = ONE ? my_cls : class_at(a, row, j);
-        const float e = cls >= 0 ? expf(((ONE ? my_t : teacher_at(a, row, j)) - tmax) * a.inv_t) : 0.f;
-        mass += e;
-        if (ONE) { my_p = e; break; }
-    }
-    mass = lanes.sum(mass);
-    const bool some = there && !any_bad;
-    const float inv_mass = some ? 1.f / mass : 0.f, log_mass = logf(some ? mass : 1.f), log_l = logf(l);
-    my_p *= inv_mass;
+    auto entry_p = [&](int j, int cls) { return cls >= 0 && state == SOME ? expf((teacher_at(a, row, j) - tmax) * a.inv_t) * inv_mass : 0.f; };
+    auto entry_loss = [&](float p, float lp, float zj) {  // p (log p - log q)
+        return p == 0.f ? 0.f : p * (lp - (zj == -INFINITY ? -INFINITY : (zj - zm) * a.inv_t - log_l));
+    };
 
     if constexpr (MODE & DO_LOSS) {
-        float part = 0.f;
-        for (int j = tid; j < a.k && some; j += G) {
-            const int cls = ONE ? my_cls : class_at(a, row, j);
-            const float lt = ((ONE ? my_t : teacher_at(a, row, j)) - tmax) * a.inv_t, p = ONE ? my_p : cls >= 0 ? expf(lt) * inv_mass : 0.f;
-            if (p != 0.f) {
-                const float zj = ONE ? my_z : (float)z[cls];
-                const float log_q = zj == -INFINITY ? -INFINITY : (zj - zm) * a.inv_t - log_l;
-                part += p * (lt - log_mass - log_q);
+        float loss = 0.f;
+        if constexpr (ONE) {
+            if (tid < GE) loss = wave.sum(entry_loss(my_p, my_lp, my_z), 0);
+        } else {
+            for (int j = tid; j < a.k && state == SOME; j += G) {
+                const int cls = class_at(a, row, j);
+                const float p = entry_p(j, cls);
+                if (p != 0.f) loss += entry_loss(p, (teacher_at(a, row, j) - tmax) * a.inv_t - log_mass, (float)z[cls]);
             }
-            if (ONE) break;
+            loss = lanes.sum(loss, 4);
         }
-        part = lanes.sum(part);
-        if (tid == 0) a.loss[row] = any_bad ? NAN : a.T * a.T * part;
+        if (tid == 0) a.loss[row] = state == BAD ? NAN : a.T * a.T * loss;
     }
     if constexpr (MODE & DO_GRAD) {
-        const float wt = any_bad ? NAN : a.weight[row] * a.T;
-        const bool live = some || any_bad;
+        const float wt = state == BAD ? NAN : a.weight[row] * a.T;
+        const bool live = state != NOTHING;
         const float inv_l = l == 0.f ? 0.f : 1.f / l, scale = wt * inv_l;
         T* const out = (T*)a.grad + row * a.V;
         const bool same_phase = (int)(((uintptr_t)out & 15) / sizeof(T)) == off;
@@ -259,42 +284,28 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void k_distill(DistillArgs a) {
                 put(i, ev);
             }
         }
-        if constexpr (G > 64) {
+        if constexpr (LISTS) {
             for (int j = tid; j < a.k; j += G) {
-                const int cls = ONE ? my_cls : class_at(a, row, j);
-                s_c[j] = cls;
-                s_p[j] = ONE ? my_p : cls >= 0 && some ? expf((teacher_at(a, row, j) - tmax) * a.inv_t) * inv_mass : 0.f;
-                if (ONE) break;
+                s_c[j] = class_at(a, row, j);
+                s_p[j] = entry_p(j, s_c[j]);
             }
         }
         lanes.sync();
-        if constexpr (ONE && G <= 64) {
-            float p = 0.f;
-            bool first = true;
-            for (int i = 0; i < a.k; ++i) {  // all lanes of the group, entry or not
-                const int c = __shfl(my_cls, i, G);
-                const float q = __shfl(my_p, i, G);
-                if (c == my_cls) {
-                    p += q;
-                    first &= i >= tid;
-                }
-            }
-            if (my_cls >= 0 && some && first) out[my_cls] = (T)(wt * (exp_diff(my_z, zm, c) * inv_l - p));
+        if constexpr (ONE) {
+            if (my_cls >= 0 && state == SOME && first) out[my_cls] = (T)(wt * (exp_diff(my_z, zm, c) * inv_l - p_all));
         } else {
             for (int j = tid; j < a.k; j += G) {
-                const int cls = G > 64 ? s_c[j] : class_at(a, row, j);
-                if (cls < 0 || !some) continue;
+                const int cls = LISTS ? s_c[j] : class_at(a, row, j);
+                if (cls < 0 || state != SOME) continue;
                 float p = 0.f;
-                bool first = true;
+                bool one = true;
                 for (int i = 0; i < a.k; ++i) {
-                    if (G > 64) {
-                        if (s_c[i] == cls) { p += s_p[i]; first &= i >= j; }
-                    } else if (class_at(a, row, i) == cls) {
-                        p += expf((teacher_at(a, row, i) - tmax) * a.inv_t) * inv_mass;
-                        first &= i >= j;
+                    if ((LISTS ? s_c[i] : class_at(a, row, i)) == cls) {
+                        p += LISTS ? s_p[i] : entry_p(i, cls);
+                        one &= i >= j;
                     }
                 }
-                if (first) out[cls] = (T)(wt * (exp_diff((float)z[cls], zm, c) * inv_l - p));
+                if (one) out[cls] = (T)(wt * (exp_diff((float)z[cls], zm, c) * inv_l - p));
             }
         }
     }
@@ -308,7 +319,7 @@ template <typename T, int G, int NV, bool HELD, bool ONE> static void go_mode(co
     else hipLaunchKernelGGL((k_distill<T, G, NV, HELD, DO_LOSS | DO_GRAD, ONE>), grid, dim3(NT), 0, st, a);
 }
 template <typename T, int G, int NV, bool HELD> static void go(const DistillArgs& a, int mode, hipStream_t st) {
-    if (a.k <= G) go_mode<T, G, NV, HELD, true>(a, mode, st); else go_mode<T, G, NV, HELD, false>(a, mode, st);
+    if (a.k <= (G > 64 ? 64 : G)) go_mode<T, G, NV, HELD, true>(a, mode, st); else go_mode<T, G, NV, HELD, false>(a, mode, st);
 }
 
 template <typename T> static int distill(const DistillArgs& a, int mode, hipStream_t st) {
