@@ -169,6 +169,29 @@ class VAESecondVolterraForward(GenericTorchBlindEqualizer):
             q = self.forward_probs(y)
         return q.cpu().numpy()
 
+    @property
+    def joint_constellation(self):
+        """Complex points in the order of the classes that `top_logits` names: I level outer, Q level inner."""
+        re, im = self._levels[0].cpu().numpy(), self._levels[1].cpu().numpy()
+        return (re[:, None] + 1j * im[None, :]).reshape(-1)
+
+    def top_logits(self, y_input, k, chunk=1 << 18):
+        """The k largest logits of every symbol over the joint constellation (the sum of both axes' soft-demapper logits,
+        :808-817), largest first, and their classes: (float32 [N, k], int32 [N, k]) on the device.  What a student learns from
+        (`distilled_equalization.DistilledEqualiser`)."""
+        y = torch.from_numpy(self.to_real_stacked(y_input)).type(self.dtype).to(device=self.torch_device)
+        values, classes = [], []
+        with torch.no_grad():
+            xhat = self.forward(y)
+            spread = self._noise_var * self.noise_scaling.detach()                 # [2, M]
+            for part in xhat.split(chunk, dim=1):
+                axis = -(part[:, :, None] - self._levels[:, None, :]) ** 2 / spread[:, None, :]   # [2, n, M]
+                joint = (axis[0][:, :, None] + axis[1][:, None, :]).reshape(part.shape[1], -1)
+                top = joint.topk(min(k, joint.shape[1]), dim=1)
+                values.append(top.values)
+                classes.append(top.indices.to(torch.int32))
+        return torch.cat(values), torch.cat(classes)
+
     def _calculate_loss(self, xhat, y):
         n = y.shape[-1]
         loss, E = ElboLossFn.apply(self._plan(n), xhat, y.to(self.dtype).contiguous(), self.channel_h1, self.channel_h2,

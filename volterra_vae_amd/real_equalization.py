@@ -278,6 +278,22 @@ class VAESecondVolterraForward(GenericTorchBlindProbabilisticEqualizer):
                            self._noise_var, q_out=q)
         return q[0]
 
+    @property
+    def joint_constellation(self):
+        """Points in the order of the classes that `top_logits` names."""
+        return self.constellation.cpu().numpy()
+
+    def top_logits(self, y_input, k):
+        """The soft demapper's k largest logits -(xhat - a)^2 / (noise variance * scaling) (:816-823) of every symbol, largest first,
+        and the classes they belong to: (float32 [N, k], int32 [N, k]) on the device.  What a student learns from
+        (`distilled_equalization.DistilledEqualiser`)."""
+        y = torch.from_numpy(np.ascontiguousarray(y_input)).type(self.dtype).to(device=self.torch_device)
+        with torch.no_grad():
+            xhat = self.forward(y).reshape(-1)
+            logits = -(xhat[:, None] - self.constellation[None, :]) ** 2 / (self._noise_var * self.noise_scaling.detach()[None, :])
+            top = logits.topk(min(k, logits.shape[1]), dim=1)
+        return top.values.contiguous(), top.indices.to(torch.int32).contiguous()
+
     def _calculate_loss(self, xhat, y):
         """ELBO (:836-925) incl. the noise-variance side effect (:921-923); 0-d tensor with grad_fn."""
         n = y.shape[-1]
