@@ -138,11 +138,9 @@ static Cut cut_product(int64_t M, int64_t N, int64_t K, int segs, int batch, int
     if (dtype == V2VAE_F32) {
         const int64_t rows = (M + 127) / 128, wide = rows * ((N * (gated ? 2 : 1) + 127) / 128) * batch;
         const int64_t narrow = rows * ((N * (gated ? 2 : 1) + 63) / 64) * batch;
-        // 128 columns a tile unless that leaves workgroups or a half-empty last column of tiles
+        // 128 columns a tile unless that leaves too few workgroups or a half-empty last column of tiles (130 columns, 65536 rows: the
+        // two gradient products take 60 and 55 us with 64 columns a tile, 66 and 76 us with 128)
         c.tile = (wide >= 256 || wide * (steps / 8) >= 256) && wide * 2 == narrow ? TILE_128 : TILE_64;
-#ifdef FORCE_TILE
-        c.tile = FORCE_TILE;
-#endif
         tiles = c.tile == TILE_128 ? wide : narrow;
     } else if (direct && tiles_of(256) >= 128 && full(tiles_of(256), 256) >= 0.88 * full(tiles_of(128), 512)) {
         c.tile = TILE_256;

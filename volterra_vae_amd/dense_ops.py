@@ -65,23 +65,16 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
-class _On:
-    """The tensors' device made current around the calls, where it is not already; gives its current stream."""
-    __slots__ = ("index", "guard")
-
-    def __init__(self, t):
-        self.index = t.get_device()
-        self.guard = None
-
-    def __enter__(self):
-        if self.index != torch._C._cuda_getDevice():
-            self.guard = torch.cuda.device(self.index)
-            self.guard.__enter__()
-        return torch._C._cuda_getCurrentRawStream(self.index)
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _enqueue(fn, name, t, *args):
+    """fn(*args, stream) with t's device current and its current stream."""
+    index = t.get_device()
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc, name)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -97,6 +90,16 @@ def _workspace(gated, backward, act, x, n):
 
 
 def _check_layer(x, weight, name, bias, bias_name):
+    try:  # what passes, first
+        dtype, index = x.dtype, x.get_device()
+        n, k = weight.shape
+        if (weight.dtype is dtype and weight.get_device() == index and k == x.shape[1] and n > 0 and k > 0
+                and (weight.stride(1) == 1 or k == 1)
+                and (bias is None or (bias.dtype is dtype and bias.get_device() == index and bias.shape == (n,)
+                                      and (bias.stride(0) == 1 or n == 1)))):
+            return
+    except (AttributeError, ValueError, IndexError):
+        pass
     _check_tensor(weight, name, 2, like=x)
     if weight.shape[1] != x.shape[1]:
         raise ValueError(f"{name}: {weight.shape[1]} columns, x has {x.shape[1]}")
@@ -140,11 +143,11 @@ def linear_forward(x, weight, bias=None, *, residual=None, activation="none",
         if tuple(residual.shape) != (m, n):
             raise ValueError(f"residual: expected {(m, n)}, got {tuple(residual.shape)}")
     d = _dense(x, weight, act, residual=residual)
-    with _On(x) as stream:
-        y = x.new_empty((m, n))
-        z = torch.empty((m, n), dtype=torch.float32, device=x.device) if keep and act else None
-        ws = _workspace(False, 0, act, x, n)
-        check(lib.v2vae_linear_fwd(d, _p(x), _p(weight), _p(bias), _p(residual), _p(y), _p(z), _p(ws), stream), "v2vae_linear_fwd")
+    y = x.new_empty((m, n))
+    z = torch.empty((m, n), dtype=torch.float32, device=x.device) if keep and act else None
+    ws = _workspace(False, 0, act, x, n)
+    _enqueue(lib.v2vae_linear_fwd, "v2vae_linear_fwd", x, d, x.data_ptr(), weight.data_ptr(), _p(bias), _p(residual), y.data_ptr(), _p(z),
+             _p(ws))
     return y, z
 
 
@@ -166,12 +169,10 @@ def linear_backward(dy, x, weight, z=None, *, activation="none", need=(True, Tru
 def _linear_backward(dy, x, weight, z, act, need):
     m, k, n = x.shape[0], x.shape[1], weight.shape[0]
     d = _dense(x, weight, act, dy=dy)
-    with _On(x) as stream:
-        new = lambda wanted, *shape: x.new_empty(shape) if wanted else None  # noqa: E731
-        dx, dw, db = new(need[0], m, k), new(need[1], n, k), new(need[2], n)
-        ws = _workspace(False, 1, act, x, n)
-        check(lib.v2vae_linear_bwd(d, _p(x), _p(weight), _p(z) if act else None, _p(dy), _p(dx), _p(dw), _p(db), _p(ws), stream),
-              "v2vae_linear_bwd")
+    new = lambda wanted, *shape: x.new_empty(shape) if wanted else None  # noqa: E731
+    dx, dw, db = new(need[0], m, k), new(need[1], n, k), new(need[2], n)
+    ws = _workspace(False, 1, act, x, n)
+    _enqueue(lib.v2vae_linear_bwd, "v2vae_linear_bwd", x, d, _p(x), _p(weight), _p(z) if act else None, _p(dy), _p(dx), _p(dw), _p(db), _p(ws))
     return dx, dw, db
 
 
@@ -235,12 +236,11 @@ def gated_forward(x, weight_gate, weight_up, bias_gate=None, bias_up=None, *, ac
         raise ValueError(f"weight_up: expected {tuple(weight_gate.shape)}, got {tuple(weight_up.shape)}")
     m, n = x.shape[0], weight_gate.shape[0]
     d = _dense(x, weight_gate, act, w2=weight_up)
-    with _On(x) as stream:
-        h = x.new_empty((m, n))
-        gu = torch.empty((2, m, n), dtype=torch.float32, device=x.device) if keep else None
-        ws = _workspace(True, 0, act, x, n)
-        check(lib.v2vae_gated_fwd(d, _p(x), _p(weight_gate), _p(weight_up), _p(bias_gate), _p(bias_up), _p(h), _p(gu), _p(ws), stream),
-              "v2vae_gated_fwd")
+    h = x.new_empty((m, n))
+    gu = torch.empty((2, m, n), dtype=torch.float32, device=x.device) if keep else None
+    ws = _workspace(True, 0, act, x, n)
+    _enqueue(lib.v2vae_gated_fwd, "v2vae_gated_fwd", x, d, x.data_ptr(), weight_gate.data_ptr(), weight_up.data_ptr(), _p(bias_gate),
+             _p(bias_up), h.data_ptr(), _p(gu), _p(ws))
     return h, gu
 
 
@@ -262,12 +262,10 @@ def gated_backward(dh, x, weight_gate, weight_up, gu, *, activation="silu", need
 def _gated_backward(dh, x, weight_gate, weight_up, gu, act, need):
     m, k, n = x.shape[0], x.shape[1], weight_gate.shape[0]
     d = _dense(x, weight_gate, act, w2=weight_up, dy=dh)
-    with _On(x) as stream:
-        new = lambda wanted, *shape: x.new_empty(shape) if wanted else None  # noqa: E731
-        out = [new(need[0], m, k), new(need[1], n, k), new(need[2], n, k), new(need[3], n), new(need[4], n)]
-        ws = _workspace(True, 1, act, x, n)
-        check(lib.v2vae_gated_bwd(d, _p(x), _p(weight_gate), _p(weight_up), _p(gu), _p(dh), *[_p(t) for t in out], _p(ws), stream),
-              "v2vae_gated_bwd")
+    new = lambda wanted, *shape: x.new_empty(shape) if wanted else None  # noqa: E731
+    out = [new(need[0], m, k), new(need[1], n, k), new(need[2], n, k), new(need[3], n), new(need[4], n)]
+    ws = _workspace(True, 1, act, x, n)
+    _enqueue(lib.v2vae_gated_bwd, "v2vae_gated_bwd", x, d, _p(x), _p(weight_gate), _p(weight_up), _p(gu), _p(dh), *[_p(t) for t in out], _p(ws))
     return tuple(out)
 
 
@@ -304,9 +302,9 @@ def gated_linear(x: torch.Tensor, weight_gate: torch.Tensor, weight_up: torch.Te
 # ------------------------------------------------------------------------------------------------ distillation
 def _distill(logits, teacher_logits, teacher_index, temperature):
     _check_tensor(logits, "logits", 2)
-    if not isinstance(teacher_logits, torch.Tensor) or teacher_logits.dtype not in _DTYPES:
+    if getattr(teacher_logits, "dtype", None) not in _DTYPES:
         raise NotImplementedError("teacher_logits: a float32, bfloat16 or float16 tensor")
-    if not isinstance(teacher_index, torch.Tensor) or teacher_index.dtype not in (torch.int32, torch.int64):
+    if getattr(teacher_index, "dtype", None) not in (torch.int32, torch.int64):
         raise ValueError("teacher_index: an int32 or int64 tensor")
     _check_tensor(teacher_logits, "teacher_logits", 2, like=logits, dtype=teacher_logits.dtype)
     _check_tensor(teacher_index, "teacher_index", 2, like=logits, dtype=teacher_index.dtype)
@@ -335,11 +333,9 @@ def topk_distillation_step(logits, teacher_logits, teacher_index, row_weight, *,
     """(loss [M] float32, grad [M, V]): the losses of `topk_distillation` and d(sum of row_weight * loss) / d logits, one pass."""
     d = _distill(logits, teacher_logits, teacher_index, temperature)
     _check_weight(row_weight, logits)
-    with _On(logits) as stream:
-        loss = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
-        grad = logits.new_empty(logits.shape)
-        check(lib.v2vae_distill_step(d, _p(logits), _p(teacher_logits), _p(teacher_index), _p(row_weight), _p(loss), _p(grad), stream),
-              "v2vae_distill_step")
+    loss, grad = row_weight.new_empty(row_weight.shape), logits.new_empty(logits.shape)
+    _enqueue(lib.v2vae_distill_step, "v2vae_distill_step", logits, d, _p(logits), _p(teacher_logits), _p(teacher_index), _p(row_weight),
+             _p(loss), _p(grad))
     return loss, grad
 
 
@@ -355,20 +351,17 @@ class _Distillation(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, weight):
         logits, teacher_logits, teacher_index, stats = ctx.saved_tensors
-        weight = weight.contiguous()
-        with _On(logits) as stream:
-            grad = logits.new_empty(logits.shape)
-            check(lib.v2vae_distill_bwd(ctx.d, _p(logits), _p(teacher_logits), _p(teacher_index), _p(stats), _p(weight), _p(grad), stream),
-                  "v2vae_distill_bwd")
+        weight, grad = weight.contiguous(), logits.new_empty(logits.shape)
+        _enqueue(lib.v2vae_distill_bwd, "v2vae_distill_bwd", logits, ctx.d, _p(logits), _p(teacher_logits), _p(teacher_index), _p(stats),
+                 _p(weight), _p(grad))
         return grad, None, None, None
 
 
 def _distill_forward(d, logits, teacher_logits, teacher_index, keep):
-    with _On(logits) as stream:
-        loss = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
-        stats = torch.empty((logits.shape[0], 2), dtype=torch.float32, device=logits.device) if keep else None
-        check(lib.v2vae_distill_fwd(d, _p(logits), _p(teacher_logits), _p(teacher_index), _p(loss), _p(stats), stream),
-              "v2vae_distill_fwd")
+    m = logits.shape[0]
+    loss = torch.empty(m, dtype=torch.float32, device=logits.device)
+    stats = loss.new_empty((m, 2)) if keep else None
+    _enqueue(lib.v2vae_distill_fwd, "v2vae_distill_fwd", logits, d, _p(logits), _p(teacher_logits), _p(teacher_index), _p(loss), _p(stats))
     return loss, stats
 
 
