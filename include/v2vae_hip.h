@@ -406,7 +406,7 @@ typedef struct v2vae_distill {
     int64_t ld_logits;     /* >= vocab */
     int64_t ld_teacher;    /* >= k */
     int64_t ld_index;      /* >= k */
-    float temperature;     /* > 0, finite */
+    float temperature;     /* 1e-4 ... 1e4 */
     int32_t reserved;      /* must be 0 */
 } v2vae_distill;
 #define V2VAE_DISTILL_MAX_K 1024

@@ -37,12 +37,15 @@ def test_bad_descriptions_are_refused(over):
 
 
 def test_sizes_beyond_the_limits_are_refused():
-    for over in (dict(rows=(1 << 30) + 1), dict(in_=(1 << 22) + 1), dict(out=1 << 31), dict(rows=1 << 30, out=1 << 22),
+    for over in (dict(rows=(1 << 30) + 1), dict(in_=(1 << 22) + 1), dict(out=1 << 31), dict(rows=1 << 30, out=1 << 22), dict(rows=1 << 30), dict(rows=1 << 26, out=1024, ld_res=1024),
                  dict(ld_x=(1 << 22) + 1), dict(ld_w=(1 << 22) + 1)):
         assert _lib.lib.v2vae_linear_fwd(dense(**over), P, P, None, None, P, None, P, None) == _lib.ESIZE
         assert _lib.lib.v2vae_linear_workspace_bytes(dense(**over), 1) == 0
     assert _lib.lib.v2vae_distill_fwd(distill(k=1025, ld_teacher=1025, ld_index=1025), P, P, P, P, None, None) == _lib.ESIZE
     assert _lib.lib.v2vae_distill_fwd(distill(rows=(1 << 30) + 1), P, P, P, P, None, None) == _lib.ESIZE
+    # more rows than a launch has threads for
+    assert _lib.lib.v2vae_distill_fwd(distill(rows=1 << 30), P, P, P, P, None, None) == _lib.ESIZE
+    assert _lib.lib.v2vae_distill_fwd(distill(rows=1 << 23, vocab=20000, ld_logits=20000), P, P, P, P, None, None) == _lib.ESIZE
 
 
 def test_missing_and_misaligned_pointers_are_refused():
@@ -69,7 +72,7 @@ def test_missing_and_misaligned_pointers_are_refused():
 @pytest.mark.parametrize("over", [dict(dtype=3), dict(teacher_dtype=-1), dict(index_bits=16), dict(k=0), dict(rows=-1), dict(vocab=0),
                                   dict(ld_logits=99), dict(ld_teacher=3), dict(ld_index=3), dict(temperature=0.0),
                                   dict(temperature=-1.0), dict(temperature=float("nan")), dict(temperature=float("inf")),
-                                  dict(temperature=1e-44), dict(reserved=1)], ids=str)
+                                  dict(temperature=9e-5), dict(temperature=2e4), dict(reserved=1)], ids=str)
 def test_bad_distillations_are_refused(over):
     d = distill(**over)
     assert _lib.lib.v2vae_distill_fwd(d, P, P, P, P, None, None) == _lib.EINVAL

@@ -274,6 +274,68 @@ def test_rows_of_an_input_may_overlap():
                 assert torch.equal(p, q)
 
 
+@pytest.mark.parametrize("act", ["none", "relu"])
+def test_gated_block_with_the_other_activations(act):
+    from volterra_vae_amd.dense_ops import gated_backward, gated_forward
+    for dtype in DTYPES:
+        x, wg, wu, bg, bu, dh = gated_case(90, 56, 48, dtype, True, "plain", 21)
+        h, gu = gated_forward(x, wg, wu, bg, bu, activation=act, keep=True)
+        check_gated(x, wg, wu, bg, bu, dh, act, h, gated_backward(dh, x, wg, wu, gu, activation=act), dtype)
+
+
+def test_one_row_repeated_and_one_tensor_in_two_places():
+    """Rows with stride 0, the input as its own residual, one weight as gate and up: values and summed gradients."""
+    from volterra_vae_amd.dense_ops import gated_linear, linear
+    gen = torch.Generator().manual_seed(6)
+    for dtype in DTYPES:
+        row, w = normal(gen, 1, 64, dtype=dtype), normal(gen, 64, 64, scale=0.1, dtype=dtype)
+        for m in (5, 40, 1500):
+            assert torch.equal(linear(row.expand(m, 64), w), linear(row.repeat(m, 1), w))
+            assert torch.equal(gated_linear(row.expand(m, 64), w, w), gated_linear(row.repeat(m, 1), w, w))
+        x = normal(gen, 33, 64, dtype=dtype).requires_grad_(True)
+        w.requires_grad_(True)
+        x2, w2 = x.detach().clone().requires_grad_(True), w.detach().clone().requires_grad_(True)
+        dy = normal(gen, 33, 64, dtype=dtype)
+        got = torch.autograd.grad(linear(x, w, residual=x, activation="tanh"), (x, w), dy)
+        r2 = x.detach().clone().requires_grad_(True)
+        dx, dw, dr = torch.autograd.grad(linear(x2, w2, residual=r2, activation="tanh"), (x2, w2, r2), dy)
+        assert torch.equal(got[0], dx + dr) and torch.equal(got[1], dw)
+        got = torch.autograd.grad(gated_linear(x, w, w), w, dy)[0]
+        wa, wb = (w.detach().clone().requires_grad_(True) for _ in range(2))
+        assert torch.equal(got, sum(torch.autograd.grad(gated_linear(x, wa, wb), (wa, wb), dy)))
+
+
+def test_offsets_beyond_32_bits():
+    """Activations and outputs of more than 2^32 elements: everything is zero but the last rows, whose results are those of these rows
+    alone (cut along the contraction in another way: to rounding, not to the bit)."""
+    from volterra_vae_amd.dense_ops import linear_backward, linear_forward
+    gen = torch.Generator().manual_seed(1)
+    for dtype, m, k in ((torch.bfloat16, (1 << 21) + 77, 2056), (torch.float32, (1 << 20) + 99, 4104), (torch.float16, (1 << 21) + 5, 2051)):
+        w = normal(gen, 24, k, scale=k ** -0.5, dtype=dtype)
+        x = torch.zeros((m, k), dtype=dtype, device=dev())
+        tail = normal(gen, 300, k, dtype=dtype)
+        x[-300:] = tail
+        y = linear_forward(x, w)[0]
+        ref = tail.double() @ w.double().t()
+        near(y[-300:], ref, u(dtype) * ref.abs() + 8 * EPS32 * steps(k, dtype) ** 0.5 * s2(tail.double(), w.double()) + 1e-30, "y")
+        assert float(y[:-300].abs().max()) == 0.0
+        dy = torch.zeros_like(y)
+        dy[-300:] = normal(gen, 300, 24, dtype=dtype)
+        dx, dw, db = linear_backward(dy, x, w)
+        ref = dy[-300:].double().t() @ tail.double()
+        near(dw, ref, u(dtype) * ref.abs() + 32 * EPS32 * steps(300, dtype) ** 0.5 * s2(dy[-300:].double().t(), tail.double().t()) + 1e-30, "dw")
+        ref = dy[-300:].double() @ w.double()
+        near(dx[-300:], ref, u(dtype) * ref.abs() + 32 * EPS32 * steps(24, dtype) ** 0.5 * s2(dy[-300:].double(), w.double().t()) + 1e-30, "dx")
+        assert float(dx[:-300].abs().max()) == 0.0
+        del x, y, dy, dx
+    # an output beyond 2^32 elements
+    x, w = normal(gen, (1 << 20) + 33, 8, dtype=torch.bfloat16), normal(gen, 4104, 8, dtype=torch.bfloat16)
+    y = linear_forward(x, w)[0]
+    ref = x[-2000:].double() @ w.double().t()
+    assert y.numel() > 1 << 32
+    near(y[-2000:], ref, u(y.dtype) * ref.abs() + 8 * EPS32 * steps(8, y.dtype) ** 0.5 * s2(x[-2000:].double(), w.double()), "y")
+
+
 def test_no_rows_give_empty_outputs_and_zero_parameter_gradients():
     from volterra_vae_amd.dense_ops import gated_linear, linear
     for dtype in DTYPES:

@@ -194,6 +194,24 @@ def test_no_rows_one_weight_for_all_and_a_side_stream():
     assert torch.equal(loss, topk_distillation(z, t, idx))
 
 
+def test_offsets_beyond_32_bits():
+    """Logits and gradient of more than 2^32 elements, rows held in registers and rows read twice: the last rows
+    against the formula (a row that starts elsewhere in a 16-byte piece adds up in another order)."""
+    from volterra_vae_amd.dense_ops import topk_distillation_step
+    for m, v in (((1 << 16) + 9, 65600), ((1 << 15) + 3, 131200), ((1 << 27) + 5, 33)):
+        z = torch.zeros((m, v), dtype=torch.bfloat16, device=dev())
+        zs, ts, idxs, ws = case(64, v, 4, torch.bfloat16, 2)
+        z[-64:] = zs
+        t, idx, w = ts[:1].repeat(m, 1), torch.zeros((m, 4), dtype=torch.int32, device=dev()), torch.ones(m, device=dev())
+        t[-64:], idx[-64:], w[-64:] = ts, idxs, ws
+        loss, grad = topk_distillation_step(z, t, idx, w)
+        ref, ref_grad, scale, grad_scale = reference(zs, ts, idxs, ws, 1.0)
+        assert bool(((loss[-64:].double().cpu() - ref).abs() <= 16 * EPS32 * scale + 1e-30).all())
+        assert bool(((grad[-64:].double().cpu() - ref_grad).abs() <= 2.0 ** -8 * ref_grad.abs() + 16 * EPS32 * grad_scale + 1e-37).all())
+        assert grad.numel() > 1 << 32 and bool(torch.isfinite(loss).all())
+        del z, grad
+
+
 def test_the_gradient_agrees_with_differences():
     """h = 2^-5 along a unit direction: truncation h^2 / 6 of a third derivative below 1 / T, rounding 2^-22 / h: 1e-3 of the scale."""
     from volterra_vae_amd.dense_ops import topk_distillation, topk_distillation_step

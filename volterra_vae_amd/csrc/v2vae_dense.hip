@@ -118,9 +118,9 @@ static int check_dense(const v2vae_dense* d, bool gated, bool backward, bool res
     if (d->ld_x > WIDTH_LIMIT || d->ld_w > WIDTH_LIMIT || (gated && d->ld_w2 > WIDTH_LIMIT) || (residual && d->ld_res > WIDTH_LIMIT) ||
         (backward && d->ld_dy > WIDTH_LIMIT))
         return V2VAE_ESIZE;
-    // tiles of 64 x 64 (gated forward: 64 x 64 features) are counted in 31 bits
-    const int64_t m = (d->rows + 63) / 64, n = (d->out + 63) / 64, k = (d->in + 63) / 64;
-    if (m * n >= INT32_MAX || m * k >= INT32_MAX || n * k >= INT32_MAX) return V2VAE_ESIZE;
+    // a launch holds fewer than 2^32 threads: 256 for every tile of 64 x 64 (gated forward: 64 x 32 features)
+    const int64_t m = (d->rows + 63) / 64, n = (d->out + 63) / 64 * (gated ? 2 : 1), k = (d->in + 63) / 64, most = (int64_t)1 << 24;
+    if (m * n >= most || m * k >= most || n * k >= most) return V2VAE_ESIZE;
     return V2VAE_OK;
 }
 

@@ -301,8 +301,9 @@ template <bool TRANSPOSED> __global__ __launch_bounds__(256) void k_split_planes
     const int tid = threadIdx.x;
     float v[8];
     int r, k;
+    const int across = TRANSPOSED ? a.ld / 32 : (a.ld + 127) / 128, bx = blockIdx.x % across, by = blockIdx.x / across;
     if constexpr (TRANSPOSED) {  // 32 k x 64 rows a block
-        const int k0 = blockIdx.x * 32, r0 = blockIdx.y * 64, pad = a.ld / (a.gated ? 2 : 1), which = k0 >= pad ? 1 : 0;
+        const int k0 = bx * 32, r0 = by * 64, pad = a.ld / (a.gated ? 2 : 1), which = k0 >= pad ? 1 : 0;
         for (int i = tid; i < 32 * 64; i += 256) {
             const int kk = k0 - which * pad + (i >> 6), c = r0 + (i & 63);
             s_t[i >> 6][i & 63] = kk < a.N && c < a.K ? a.w[which][kk * a.ld_w[which] + c] : 0.f;
@@ -313,8 +314,8 @@ template <bool TRANSPOSED> __global__ __launch_bounds__(256) void k_split_planes
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = s_t[(tid & 3) * 8 + e][tid >> 2];
     } else {                     // 16 rows x 128 k a block
-        r = blockIdx.y * 16 + (tid >> 4);
-        k = blockIdx.x * 128 + (tid & 15) * 8;
+        r = by * 16 + (tid >> 4);
+        k = bx * 128 + (tid & 15) * 8;
         const int which = a.gated ? (r >> 5) & 1 : 0, f = a.gated ? (r >> 6) * 32 + (r & 31) : r;
         const float* const p = a.w[which] + f * a.ld_w[which];
 #pragma unroll

@@ -16,8 +16,8 @@ int split_planes(const GemmArgs& g, bool transposed, bool gated, int N, int K, h
     a.N = N;
     a.K = K;
     a.gated = gated;
-    if (transposed) hipLaunchKernelGGL(k_split_planes<true>, dim3(a.ld / 32, (a.rows + 63) / 64), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(k_split_planes<false>, dim3((a.ld + 127) / 128, (a.rows + 15) / 16), dim3(256), 0, st, a);
+    if (transposed) hipLaunchKernelGGL(k_split_planes<true>, dim3((unsigned)(a.ld / 32) * ((a.rows + 63) / 64)), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(k_split_planes<false>, dim3((unsigned)((a.ld + 127) / 128) * ((a.rows + 15) / 16)), dim3(256), 0, st, a);
     return dense_launch_error("dense layer, weights");
 }
 

@@ -311,15 +311,18 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void k_distill(DistillArgs a) {
     }
 }
 
-template <typename T, int G, int NV, bool HELD, bool ONE> static void go_mode(const DistillArgs& a, int mode, hipStream_t st) {
+template <typename T, int G, int NV, bool HELD, bool ONE> static int go_mode(const DistillArgs& a, int mode, hipStream_t st) {
     constexpr int ROWS = G > 64 ? 1 : 256 / G, NT = G > 64 ? G : 256;
-    const dim3 grid((unsigned)((a.rows + ROWS - 1) / ROWS));
+    const int64_t blocks = (a.rows + ROWS - 1) / ROWS;
+    if (blocks * NT >= (int64_t)1 << 32) return V2VAE_ESIZE;  // a launch holds fewer threads
+    const dim3 grid((unsigned)blocks);
     if (mode == DO_LOSS) hipLaunchKernelGGL((k_distill<T, G, NV, HELD, DO_LOSS, ONE>), grid, dim3(NT), 0, st, a);
     else if (mode == DO_GRAD) hipLaunchKernelGGL((k_distill<T, G, NV, HELD, DO_GRAD, ONE>), grid, dim3(NT), 0, st, a);
     else hipLaunchKernelGGL((k_distill<T, G, NV, HELD, DO_LOSS | DO_GRAD, ONE>), grid, dim3(NT), 0, st, a);
+    return dense_launch_error("distillation");
 }
-template <typename T, int G, int NV, bool HELD> static void go(const DistillArgs& a, int mode, hipStream_t st) {
-    if (a.k <= (G > 64 ? 64 : G)) go_mode<T, G, NV, HELD, true>(a, mode, st); else go_mode<T, G, NV, HELD, false>(a, mode, st);
+template <typename T, int G, int NV, bool HELD> static int go(const DistillArgs& a, int mode, hipStream_t st) {
+    return a.k <= (G > 64 ? 64 : G) ? go_mode<T, G, NV, HELD, true>(a, mode, st) : go_mode<T, G, NV, HELD, false>(a, mode, st);
 }
 
 template <typename T> static int distill(const DistillArgs& a, int mode, hipStream_t st) {
@@ -327,23 +330,22 @@ template <typename T> static int distill(const DistillArgs& a, int mode, hipStre
     // pieces of a row: V / E if every row starts at one, else of a row that starts anywhere
     const bool aligned = ((uintptr_t)a.z & 15) == 0 && (a.ld_z % E == 0 || a.rows == 1);
     const int64_t pieces = aligned ? (a.V + E - 1) / E : (a.V + 2 * E - 2) / E;
-    if (pieces <= 8) go<T, 8, 1, true>(a, mode, st);
-    else if (pieces <= 16) go<T, 16, 1, true>(a, mode, st);
-    else if (pieces <= 32) go<T, 16, 2, true>(a, mode, st);
-    else if (pieces <= 64) go<T, 32, 2, true>(a, mode, st);
-    else if (pieces <= 256) go<T, 64, 4, true>(a, mode, st);
-    else if (pieces <= 1024) go<T, 256, 4, true>(a, mode, st);
-    else if (pieces <= 2048) go<T, 256, 8, true>(a, mode, st);
-    else if (pieces <= 4096) go<T, 512, 8, true>(a, mode, st);
-    else if (pieces <= 8192) go<T, 1024, 8, true>(a, mode, st);
-    else go<T, 1024, 1, false>(a, mode, st);
-    return dense_launch_error("distillation");
+    if (pieces <= 8) return go<T, 8, 1, true>(a, mode, st);
+    if (pieces <= 16) return go<T, 16, 1, true>(a, mode, st);
+    if (pieces <= 32) return go<T, 16, 2, true>(a, mode, st);
+    if (pieces <= 64) return go<T, 32, 2, true>(a, mode, st);
+    if (pieces <= 256) return go<T, 64, 4, true>(a, mode, st);
+    if (pieces <= 1024) return go<T, 256, 4, true>(a, mode, st);
+    if (pieces <= 2048) return go<T, 256, 8, true>(a, mode, st);
+    if (pieces <= 4096) return go<T, 512, 8, true>(a, mode, st);
+    if (pieces <= 8192) return go<T, 1024, 8, true>(a, mode, st);
+    return go<T, 1024, 1, false>(a, mode, st);
 }
 
 static int check_distill(const v2vae_distill* d) {
     if (!d || d->dtype < V2VAE_F32 || d->dtype > V2VAE_F16 || d->teacher_dtype < V2VAE_F32 || d->teacher_dtype > V2VAE_F16) return V2VAE_EINVAL;
     if ((d->index_bits != 32 && d->index_bits != 64) || d->reserved != 0 || d->k < 1 || d->rows < 0 || d->vocab < 1) return V2VAE_EINVAL;
-    if (!(d->temperature > 0.f) || !isfinite(d->temperature) || !isfinite(1.f / d->temperature)) return V2VAE_EINVAL;
+    if (!(d->temperature >= 1e-4f && d->temperature <= 1e4f)) return V2VAE_EINVAL;
     if (d->ld_logits < d->vocab || d->ld_teacher < d->k || d->ld_index < d->k) return V2VAE_EINVAL;
     if (d->k > V2VAE_DISTILL_MAX_K || d->rows > ((int64_t)1 << 30) || d->vocab > ((int64_t)1 << 30)) return V2VAE_ESIZE;
     return V2VAE_OK;

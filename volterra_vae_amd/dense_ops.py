@@ -12,7 +12,6 @@ that run without autograd (and for HIP graphs, into which they can be captured).
 from __future__ import annotations
 
 import functools
-import math
 from typing import Optional, Tuple
 
 import torch
@@ -317,8 +316,8 @@ def _distill(logits, teacher_logits, teacher_index, temperature):
     if teacher_logits.shape[0] != m or tuple(teacher_index.shape) != (m, k):
         raise ValueError(f"teacher_logits and teacher_index: expected {(m, k)}, got {tuple(teacher_logits.shape)} and "
                          f"{tuple(teacher_index.shape)}")
-    if not (temperature > 0 and math.isfinite(temperature)):
-        raise ValueError(f"temperature must be positive and finite (got {temperature})")
+    if not 1e-4 <= temperature <= 1e4:
+        raise ValueError(f"temperature: 1e-4 ... 1e4 (got {temperature})")
     return Distill(_DTYPES[logits.dtype], _DTYPES[teacher_logits.dtype], 32 if teacher_index.dtype == torch.int32 else 64, k, m, v,
                    _row_stride(logits) if m > 1 else v, _row_stride(teacher_logits), _row_stride(teacher_index), temperature, 0)
 
