@@ -141,7 +141,7 @@ struct GemmArgs {
     int64_t lda, ldb[2], ldc;  // elements between rows (k contiguous) or between k (rows contiguous)
     int M, N, K;            // rows of A, rows of B (output columns; gated forward: features), contraction length of a segment
     int segs, batch, splits, steps_per_split;
-    int vec_a, vec_b;       // 16-byte loads allowed
+    int pad_a, pad_b;       // rows of A, B are padded with zeros to a multiple of 16 bytes
     int vec_c;              // eight columns at a time in the epilogue: N, strides and pointers allow it
     const void* bias[2];
     const void* residual;

@@ -13,7 +13,8 @@ struct SlopeArgs {
     const void* dy;
     int64_t ld_dy;
     const float* z[2];  // pre-activations [M][N] (NULL: no activation), gated: gate and up
-    void* d[2];         // dz [M][N] (NULL: only the sums)
+    void* d[2];         // dz [M][ld_d], zeros in columns N ... ld_d - 1 (NULL: only the sums)
+    int64_t ld_d;
     float* part[2];     // [chunks][N] (NULL: no sums)
     int64_t M, rows_per_chunk;
     int N, cx;          // cx threads along the columns, 256 / cx along the rows
@@ -29,6 +30,14 @@ template <typename T, int V, int ACT, bool GATED> __global__ __launch_bounds__(2
     float s0[V], s1[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) s0[v] = s1[v] = 0.f;
+    if (n >= a.N && n < a.ld_d && a.d[0]) {  // V = 1: the padding (V = 4: N is a multiple of 4, and so is what is left)
+        for (int64_t m = lo + ty; m < hi; m += ry)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                ((T*)a.d[0])[m * a.ld_d + n + v] = (T)0.f;
+                if constexpr (GATED) ((T*)a.d[1])[m * a.ld_d + n + v] = (T)0.f;
+            }
+    }
     if (n < a.N) {
 #pragma unroll 2
         for (int64_t m = lo + ty; m < hi; m += ry) {
@@ -46,8 +55,8 @@ template <typename T, int V, int ACT, bool GATED> __global__ __launch_bounds__(2
                     o0.e[v] = (T)dg;
                     o1.e[v] = (T)du;
                 }
-                *reinterpret_cast<TV*>((T*)a.d[0] + m * a.N + n) = o0;
-                *reinterpret_cast<TV*>((T*)a.d[1] + m * a.N + n) = o1;
+                *reinterpret_cast<TV*>((T*)a.d[0] + m * a.ld_d + n) = o0;
+                *reinterpret_cast<TV*>((T*)a.d[1] + m * a.ld_d + n) = o1;
             } else {
                 FV z;
                 if (a.z[0]) z = *reinterpret_cast<const FV*>(a.z[0] + m * a.N + n);
@@ -58,7 +67,7 @@ template <typename T, int V, int ACT, bool GATED> __global__ __launch_bounds__(2
                     s0[v] += d;
                     o0.e[v] = (T)d;
                 }
-                if (a.d[0]) *reinterpret_cast<TV*>((T*)a.d[0] + m * a.N + n) = o0;
+                if (a.d[0]) *reinterpret_cast<TV*>((T*)a.d[0] + m * a.ld_d + n) = o0;
             }
         }
     }
@@ -101,6 +110,30 @@ template <typename T> __global__ __launch_bounds__(1024) void k_column_join(cons
     }
 }
 
+// ---- rows of whole 16-byte pieces --------------------------------------------------------------------------------------------
+// 16-bit matrices whose rows are not: copied once, padded with zeros, for the product kernel that loads tiles straight into LDS.
+// One pass over the operand, eight columns a thread (the loads may be unaligned, the stores are not).
+struct PackArgs { const void* src[2]; void* dst[2]; int64_t ld_src[2], R; int C, ld; };
+__global__ __launch_bounds__(256) void k_pack_rows(PackArgs a) {
+    struct __attribute__((packed, aligned(2))) Loose { u32x4 raw; };
+    const int per = a.ld / 8, which = blockIdx.y;
+    const uint16_t* const src = (const uint16_t*)a.src[which];
+    uint16_t* const dst = (uint16_t*)a.dst[which];
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.R * per; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / per;
+        const int c = (int)(i - r * per) * 8;
+        const uint16_t* const p = src + r * a.ld_src[which] + c;
+        union { u32x4 raw; uint16_t e[8]; } v;
+        if (c + 8 <= a.C) {
+            v.raw = reinterpret_cast<const Loose*>(p)->raw;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v.e[e] = c + e < a.C ? p[e] : (uint16_t)0;
+        }
+        *reinterpret_cast<u32x4*>(dst + r * a.ld + c) = v.raw;
+    }
+}
+
 // ---- host side ---------------------------------------------------------------------------------------------------------------
 static int elem_bytes(int dtype) { return dtype == V2VAE_F32 ? 4 : 2; }
 static bool aligned_to(const void* p, int n) { return ((uintptr_t)p % n) == 0; }
@@ -123,6 +156,8 @@ static int check_dense(const v2vae_dense* d, bool gated, bool backward, bool res
     if (m * n >= most || m * k >= most || n * k >= most) return V2VAE_ESIZE;
     return V2VAE_OK;
 }
+
+constexpr double PACK_FORWARD = 4e9, PACK_BACKWARD = 3e8;  // rows x in x out from which copies pay
 
 // How a product M x N x K is cut: tile size and the number of parts of the contraction.  `direct`: 16-bit operands, aligned.
 // The workspace does not know the alignment, so it is laid out for the larger of the two cuts.
@@ -203,24 +238,62 @@ static void slope_shape(int64_t M, int64_t N, int V, int* cx, int* gx, int* chun
 }
 
 // workspace of the backward pass: dz (two for the gated block), the column partials, the partials of the two products
-struct BwdLayout { size_t dz[2], part[2], planes, prod, total; };
+// 16-bit operands whose rows are not whole 16-byte pieces: copied when the products are large enough to win the copies back.  Measured
+// in bf16, forward and gradients, us without / with copies: 4001 x 2047 x 2043 86 / 63 and 518 / 138, 2000 x 101 x 3999 80 / 65 backward,
+// 65537 x 131 x 257 55 / 67 forward (therefore without) and 186 / 129 backward, 1001 x 515 x 1027 60 / 57 backward.
+struct Packs { bool x, w, dz; size_t x_bytes, w_bytes; int ld_in, ld_out; };
+static Packs packs_of(const v2vae_dense* d, bool gated, bool backward) {
+    Packs p = {};
+    p.ld_in = (int)((d->in + 7) / 8 * 8);
+    p.ld_out = (int)d->out;
+    if (d->dtype == V2VAE_F32 || d->rows <= ROWS_MAX || d->in < 32 || d->out < 32) return p;
+    if ((double)d->rows * d->in * d->out * (gated ? 2 : 1) < (backward ? PACK_BACKWARD : PACK_FORWARD)) return p;
+    const bool odd = d->in % 8 != 0;
+    p.x = odd || d->ld_x % 8 != 0;
+    p.w = odd || d->ld_w % 8 != 0 || (gated && d->ld_w2 % 8 != 0);
+    p.x_bytes = p.x ? round_up((size_t)d->rows * p.ld_in * 2) : 0;
+    p.w_bytes = p.w ? round_up((size_t)d->out * p.ld_in * 2) * (gated ? 2 : 1) : 0;
+    if (backward) {
+        p.ld_out = (int)((d->out + 7) / 8 * 8);
+        p.dz = d->out % 8 != 0 || d->ld_dy % 8 != 0;  // without an activation dy itself is copied
+    }
+    return p;
+}
+static void pack_rows(const void* s0, const void* s1, int64_t ld0, int64_t ld1, void* d0, void* d1, int64_t R, int C, int ld, hipStream_t st) {
+    PackArgs a = {{s0, s1}, {d0, d1}, {ld0, ld1}, R, C, ld};
+    int64_t blocks = (R * (ld / 8) + 255) / 256;
+    if (blocks > 8192) blocks = 8192;
+    if (blocks > 0) hipLaunchKernelGGL(k_pack_rows, dim3((unsigned)blocks, s1 ? 2 : 1), dim3(256), 0, st, a);
+}
+
+struct BwdLayout { size_t dz[2], part[2], planes, x, w, prod, total; };
 static BwdLayout bwd_layout(const v2vae_dense* d, bool gated) {
     BwdLayout l;
+    const Packs p = packs_of(d, gated, true);
     const int n = gated ? 2 : 1;
     size_t o = 0;
     for (int i = 0; i < 2; ++i) {
         l.dz[i] = o;
-        if (i < n && (gated || d->activation != V2VAE_ACT_NONE)) o += round_up((size_t)d->rows * d->out * elem_bytes(d->dtype));
+        if (i < n && (gated || d->activation != V2VAE_ACT_NONE || p.dz)) o += round_up((size_t)d->rows * p.ld_out * elem_bytes(d->dtype));
     }
     int cx, gx, c1, c4;
-    slope_shape(d->rows, d->out, 1, &cx, &gx, &c1);
-    slope_shape(d->rows, d->out, 4, &cx, &gx, &c4);
+    size_t most = 1;
+    for (int64_t width : {d->out, (int64_t)p.ld_out}) {
+        slope_shape(d->rows, width, 1, &cx, &gx, &c1);
+        slope_shape(d->rows, width, 4, &cx, &gx, &c4);
+        if ((size_t)c1 > most) most = c1;
+        if ((size_t)c4 > most) most = c4;
+    }
     for (int i = 0; i < 2; ++i) {
         l.part[i] = o;
-        if (i < n) o += round_up((size_t)(c1 > c4 ? c1 : c4) * d->out * 4);
+        if (i < n) o += round_up(most * d->out * 4);
     }
     l.planes = o;
     o += planes_of(d, gated, true).bytes;
+    l.x = o;
+    o += p.x_bytes;
+    l.w = o;
+    o += p.w_bytes;
     l.prod = o;
     const size_t a = partial_bytes(d->rows, d->in, d->out, n, 1, d->dtype, false);
     const size_t b = partial_bytes(d->out, d->in, d->rows, 1, n, d->dtype, false);
@@ -234,17 +307,16 @@ static int run_product(GemmArgs& g, int dtype, int layout, bool gated, float* pa
     auto aligned_rows = [&](const void* const p[2], int64_t ld0, int64_t ld1) {
         return aligned_to(p[0], 16) && (p[1] == nullptr || aligned_to(p[1], 16)) && ld0 % e == 0 && ld1 % e == 0;
     };
-    const bool rows_a = aligned_rows(g.a, g.lda, g.lda), rows_b = aligned_rows(g.b, g.ldb[0], g.ldb[1]);
     const bool a_kc = layout != LAYOUT_MM, b_kc = layout == LAYOUT_KK;
-    g.vec_a = a_kc && rows_a && g.K % e == 0;
-    g.vec_b = b_kc && rows_b && g.K % e == 0;
+    // every row whole 16-byte pieces, in memory and in the part of it that counts (or zeros behind that)
+    const bool whole_a = aligned_rows(g.a, g.lda, g.lda) && (g.pad_a || (a_kc ? g.K : g.M) % e == 0);
+    const bool whole_b = aligned_rows(g.b, g.ldb[0], g.ldb[1]) && (g.pad_b || (b_kc ? g.K : g.N) % e == 0);
     auto fit = [&](const void* p, int64_t ld) { return aligned_to(p, 16) && (p == nullptr || ld % e == 0); };
     g.vec_c = g.N % 8 == 0 && fit(g.c[0], g.ldc) && fit(g.c[1], g.ldc) && fit(g.bias[0], 0) && fit(g.bias[1], 0) && fit(g.residual, g.ldr) &&
               fit(g.z[0], 0) && fit(g.z[1], 0);
-    // straight to LDS: 16-bit, every row of both operands whole 16-byte pieces, offsets inside a tile below 2^31, one stride
+    // straight to LDS: 16-bit, whole pieces, offsets inside a tile below 2^31, one stride
     const int64_t ld_max = g.lda > g.ldb[0] ? (g.lda > g.ldb[1] ? g.lda : g.ldb[1]) : (g.ldb[0] > g.ldb[1] ? g.ldb[0] : g.ldb[1]);
-    const bool direct = dtype != V2VAE_F32 && (a_kc ? g.vec_a : rows_a && g.M % 8 == 0) && (b_kc ? g.vec_b : rows_b && g.N % 8 == 0) &&
-                        ld_max <= (1 << 21) && (gated || g.ldb[0] == g.ldb[1]);
+    const bool direct = dtype != V2VAE_F32 && whole_a && whole_b && ld_max <= (1 << 21) && (gated || g.ldb[0] == g.ldb[1]);
     const Cut c = cut_product(g.M, g.N, g.K, g.segs, g.batch, dtype, gated, direct);
     g.splits = c.splits;
     g.steps_per_split = c.per;
@@ -291,25 +363,39 @@ static int forward(const v2vae_dense* d, const void* x, const void* w0, const vo
         const int rc = use_planes(g, p, false, gated, (char*)ws, st);
         if (rc != V2VAE_OK) return rc;
     }
-    if (d->rows <= ROWS_MAX) {
-        const int e = 16 / elem_bytes(d->dtype);
-        g.vec_a = aligned_to(x, 16) && d->ld_x % e == 0 && d->in % e == 0;
-        g.vec_b = aligned_to(w0, 16) && d->ld_w % e == 0 && (!gated || (aligned_to(w1, 16) && d->ld_w2 % e == 0)) && d->in % e == 0;
-        return dense_rows(g, d->dtype, gated, st);
+    if (d->rows <= ROWS_MAX) return dense_rows(g, d->dtype, gated, st);
+    const Packs k = packs_of(d, gated, false);
+    char* at = (char*)ws + p.bytes;
+    if (k.x) {
+        pack_rows(x, nullptr, d->ld_x, 0, at, nullptr, d->rows, g.K, k.ld_in, st);
+        g.a[0] = at;
+        g.lda = k.ld_in;
+        g.pad_a = 1;
+        at += k.x_bytes;
     }
-    return run_product(g, d->dtype, LAYOUT_KK, gated, (float*)((char*)ws + p.bytes), st);
+    if (k.w) {
+        char* const up = gated ? at + k.w_bytes / 2 : nullptr;
+        pack_rows(w0, w1, d->ld_w, d->ld_w2, at, up, d->out, g.K, k.ld_in, st);
+        g.b[0] = at;
+        g.b[1] = up;
+        g.ldb[0] = g.ldb[1] = k.ld_in;
+        g.pad_b = 1;
+        at += k.w_bytes;
+    }
+    return run_product(g, d->dtype, LAYOUT_KK, gated, (float*)at, st);
 }
 
 static int backward(const v2vae_dense* d, const void* x, const void* w0, const void* w1, const float* z, const void* dy, void* dx,
                     void* dw0, void* dw1, void* db0, void* db1, void* ws, hipStream_t st) {
-    const bool gated = w1 != nullptr, act = gated || d->activation != V2VAE_ACT_NONE;
+    const Packs k = packs_of(d, w1 != nullptr, true);
+    const bool gated = w1 != nullptr, act = gated || d->activation != V2VAE_ACT_NONE, copy = act || k.dz;
     const BwdLayout l = bwd_layout(d, gated);
     char* const base = (char*)ws;
     const int64_t M = d->rows;
     const void* dz[2] = {dy, nullptr};
     int64_t ld_dz = d->ld_dy;
     const bool want_b = db0 || db1, want_dz = dx || dw0 || dw1;
-    if ((act && want_dz) || want_b) {
+    if ((copy && want_dz) || want_b) {
         SlopeArgs s = {};
         s.dy = dy;
         s.ld_dy = d->ld_dy;
@@ -317,12 +403,14 @@ static int backward(const v2vae_dense* d, const void* x, const void* w0, const v
         s.N = (int)d->out;
         s.z[0] = act ? z : nullptr;
         s.z[1] = gated ? z + M * d->out : nullptr;
-        if (act) {
+        s.ld_d = d->out;
+        if (copy && want_dz) {
+            s.ld_d = k.ld_out;
             s.d[0] = base + l.dz[0];
             s.d[1] = gated ? base + l.dz[1] : nullptr;
             dz[0] = s.d[0];
             dz[1] = s.d[1];
-            ld_dz = d->out;
+            ld_dz = k.ld_out;
         }
         if (want_b) {
             s.part[0] = (float*)(base + l.part[0]);
@@ -331,7 +419,7 @@ static int backward(const v2vae_dense* d, const void* x, const void* w0, const v
         const int bytes = elem_bytes(d->dtype);
         const bool v4 = d->out % 4 == 0 && d->ld_dy % 4 == 0 && aligned_to(dy, 4 * bytes) && (!act || aligned_to(z, 16));
         int gx, chunks;
-        slope_shape(M, d->out, v4 ? 4 : 1, &s.cx, &gx, &chunks);
+        slope_shape(M, s.ld_d, v4 ? 4 : 1, &s.cx, &gx, &chunks);
         s.rows_per_chunk = (M + chunks - 1) / chunks;
         const dim3 grid(gx, chunks);
         auto slopes = [&](auto t, auto kind) {
@@ -365,6 +453,12 @@ static int backward(const v2vae_dense* d, const void* x, const void* w0, const v
         if (rc != V2VAE_OK) return rc;
     }
     float* const prod = (float*)(base + l.prod);
+    const bool padded = k.dz;
+    if (dx && k.w && M > 0) {
+        char* const up = gated ? base + l.w + k.w_bytes / 2 : nullptr;
+        pack_rows(w0, w1, d->ld_w, d->ld_w2, base + l.w, up, d->out, (int)d->in, k.ld_in, st);
+    }
+    if ((dw0 || dw1) && k.x) pack_rows(x, nullptr, d->ld_x, 0, base + l.x, nullptr, M, (int)d->in, k.ld_in, st);
     if (dx) {
         GemmArgs g = {};
         g.a[0] = dz[0];
@@ -375,6 +469,13 @@ static int backward(const v2vae_dense* d, const void* x, const void* w0, const v
         g.lda = ld_dz;
         g.ldb[0] = d->ld_w;
         g.ldb[1] = gated ? d->ld_w2 : d->ld_w;
+        g.pad_a = padded;
+        if (k.w) {
+            g.b[0] = base + l.w;
+            g.b[1] = gated ? base + l.w + k.w_bytes / 2 : nullptr;
+            g.ldb[0] = g.ldb[1] = k.ld_in;
+            g.pad_b = 1;
+        }
         g.ldc = d->in;
         g.M = (int)M;
         g.N = (int)d->in;
@@ -398,6 +499,12 @@ static int backward(const v2vae_dense* d, const void* x, const void* w0, const v
         g.c[1] = dw1;
         g.lda = ld_dz;
         g.ldb[0] = g.ldb[1] = d->ld_x;
+        g.pad_a = padded;
+        if (k.x) {
+            g.b[0] = g.b[1] = base + l.x;
+            g.ldb[0] = g.ldb[1] = k.ld_in;
+            g.pad_b = 1;
+        }
         g.ldc = d->in;
         g.M = (int)d->out;
         g.N = (int)d->in;
@@ -419,14 +526,16 @@ size_t v2vae_linear_workspace_bytes(const v2vae_dense* d, int backward) {
     if (check_dense(d, false, backward != 0, false) != V2VAE_OK) return 0;
     if (backward) return bwd_layout(d, false).total;
     if (d->rows <= ROWS_MAX) return 0;
-    return planes_of(d, false, false).bytes + partial_bytes(d->rows, d->out, d->in, 1, 1, d->dtype, false);
+    const Packs k = packs_of(d, false, false);
+    return planes_of(d, false, false).bytes + k.x_bytes + k.w_bytes + partial_bytes(d->rows, d->out, d->in, 1, 1, d->dtype, false);
 }
 
 size_t v2vae_gated_workspace_bytes(const v2vae_dense* d, int backward) {
     if (check_dense(d, true, backward != 0, false) != V2VAE_OK) return 0;
     if (backward) return bwd_layout(d, true).total;
     if (d->rows <= ROWS_MAX) return 0;
-    return planes_of(d, true, false).bytes + partial_bytes(d->rows, d->out, d->in, 1, 1, d->dtype, true);
+    const Packs k = packs_of(d, true, false);
+    return planes_of(d, true, false).bytes + k.x_bytes + k.w_bytes + partial_bytes(d->rows, d->out, d->in, 1, 1, d->dtype, true);
 }
 
 int v2vae_linear_fwd(const v2vae_dense* d, const void* x, const void* w, const void* bias, const void* residual, void* y, float* z,

@@ -10,7 +10,8 @@
 //    ds_read_b64_tr_b16 (16 lanes read 4 k x 16 rows and receive 4 k of one row each).  Line k holds its 64-byte blocks at
 //    position b ^ (k % 4 + 4 (k / 8 % 2)): the eight lines that one instruction reads then fall on different banks.
 // Rows beyond the matrix repeat its last row (or last 16 bytes): their products are not stored.  The last step of a contraction
-// that is not a multiple of 64 takes what lies beyond from a page of zeros.
+// that is not a multiple of 64 takes the 16-byte pieces (or lines) beyond it from a page of zeros.  Operands whose rows are not whole
+// pieces come as copies that are padded with zeros (pad_a, pad_b; v2vae_dense.hip).
 #ifndef V2VAE_DENSE_DIRECT_H
 #define V2VAE_DENSE_DIRECT_H
 #include "v2vae_dense_gemm.h"
@@ -61,7 +62,7 @@ template <typename T, int ROWS, int NW, bool KC, bool GATED> struct Tile {
             } else {
                 const int k = (i * 64 + lane) / (ROWS / 8), p = (i * 64 + lane) % (ROWS / 8);
                 const int piece = p ^ (4 * ((k & 3) | (((k >> 3) & 1) << 2)) % (ROWS / 8));
-                const int row = first + piece * 8 < R ? piece * 8 : R - 8 - first;
+                const int row = first + piece * 8 < R ? piece * 8 : (R - 1) / 8 * 8 - first;
                 off[j] = (unsigned)(k * ld + row) * 2u;
             }
         }

@@ -77,14 +77,14 @@ def _enqueue(fn, name, t, *args):
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_bytes(gated, backward, dtype, act, rows, columns, out):
+def _workspace_bytes(gated, backward, *description):
     f = lib.v2vae_gated_workspace_bytes if gated else lib.v2vae_linear_workspace_bytes
-    return f(Dense(dtype, act, rows, columns, out, columns, columns, columns, out, out), backward)
+    return f(Dense(*description), backward)
 
 
-def _workspace(gated, backward, act, x, n):
+def _workspace(gated, backward, d, x):
     """Scratch memory of one call, from torch's allocator: of the current stream, or of the graph that is being captured."""
-    size = _workspace_bytes(gated, backward, _DTYPES[x.dtype], act, x.shape[0], x.shape[1], n)
+    size = _workspace_bytes(gated, backward, d.dtype, d.activation, d.rows, d.in_, d.out, d.ld_x, d.ld_w, d.ld_w2, d.ld_res, d.ld_dy)
     return torch.empty(max(size, 256), dtype=torch.uint8, device=x.device) if size or backward else None
 
 
@@ -144,7 +144,7 @@ def linear_forward(x, weight, bias=None, *, residual=None, activation="none",
     d = _dense(x, weight, act, residual=residual)
     y = x.new_empty((m, n))
     z = torch.empty((m, n), dtype=torch.float32, device=x.device) if keep and act else None
-    ws = _workspace(False, 0, act, x, n)
+    ws = None if m <= 16 else _workspace(False, 0, d, x)  # few rows need none
     _enqueue(lib.v2vae_linear_fwd, "v2vae_linear_fwd", x, d, x.data_ptr(), weight.data_ptr(), _p(bias), _p(residual), y.data_ptr(), _p(z),
              _p(ws))
     return y, z
@@ -170,7 +170,7 @@ def _linear_backward(dy, x, weight, z, act, need):
     d = _dense(x, weight, act, dy=dy)
     new = lambda wanted, *shape: x.new_empty(shape) if wanted else None  # noqa: E731
     dx, dw, db = new(need[0], m, k), new(need[1], n, k), new(need[2], n)
-    ws = _workspace(False, 1, act, x, n)
+    ws = _workspace(False, 1, d, x)
     _enqueue(lib.v2vae_linear_bwd, "v2vae_linear_bwd", x, d, _p(x), _p(weight), _p(z) if act else None, _p(dy), _p(dx), _p(dw), _p(db), _p(ws))
     return dx, dw, db
 
@@ -237,7 +237,7 @@ def gated_forward(x, weight_gate, weight_up, bias_gate=None, bias_up=None, *, ac
     d = _dense(x, weight_gate, act, w2=weight_up)
     h = x.new_empty((m, n))
     gu = torch.empty((2, m, n), dtype=torch.float32, device=x.device) if keep else None
-    ws = _workspace(True, 0, act, x, n)
+    ws = None if m <= 16 else _workspace(True, 0, d, x)
     _enqueue(lib.v2vae_gated_fwd, "v2vae_gated_fwd", x, d, x.data_ptr(), weight_gate.data_ptr(), weight_up.data_ptr(), _p(bias_gate),
              _p(bias_up), h.data_ptr(), _p(gu), _p(ws))
     return h, gu
@@ -263,7 +263,7 @@ def _gated_backward(dh, x, weight_gate, weight_up, gu, act, need):
     d = _dense(x, weight_gate, act, w2=weight_up, dy=dh)
     new = lambda wanted, *shape: x.new_empty(shape) if wanted else None  # noqa: E731
     out = [new(need[0], m, k), new(need[1], n, k), new(need[2], n, k), new(need[3], n), new(need[4], n)]
-    ws = _workspace(True, 1, act, x, n)
+    ws = _workspace(True, 1, d, x)
     _enqueue(lib.v2vae_gated_bwd, "v2vae_gated_bwd", x, d, _p(x), _p(weight_gate), _p(weight_up), _p(gu), _p(dh), *[_p(t) for t in out], _p(ws))
     return tuple(out)
 
