@@ -1,8 +1,8 @@
 // One to sixteen rows through a dense layer or a gated block: the form that answers single symbols.
 //
 // The weights are read once and nothing else counts, so the kernel is a stream over them.  A workgroup owns 16 weight rows (gated
-// block: 8 gate and 8 up rows of the same features); its 16 waves (8 up to 1024 columns) take turns along the contraction, 128
-// elements each, and multiply on v_mfma_f32_16x16x32 with the input rows as the other operand (rows beyond the last repeat it): the matrix
+// block: 8 gate and 8 up rows of the same features); its waves (8, or 16) take turns along the contraction, 128 elements
+// each, and multiply on v_mfma_f32_16x16x32 with the input rows as the other operand (rows beyond the last repeat it): the matrix
 // instruction sums over lanes, which costs a vector kernel six shuffles per output and wave.  The fragments come straight from
 // memory (16 bytes a lane, any alignment); float operands are split into three bf16 pieces in registers (six products).  The
 // waves' sums are joined through LDS in a fixed order.
@@ -55,29 +55,47 @@ template <typename T, int W, bool GATED> __global__ __launch_bounds__(64 * W) vo
     const T* const w = (const T*)g.b[which] + (int64_t)nc * g.ldb[which];
     const T* const x = (const T*)g.a[0] + (int64_t)mc * g.lda;
     acc4 acc = acc4{0.f, 0.f, 0.f, 0.f};
-    auto chunk = [&](int k0, auto tail) {
-        Eight<T> wv[4], xv[4];
+    constexpr int CH = 4, CE = CH * 32;  // loads and elements of a wave's turn
+    struct Turn { Eight<T> v[CH]; };
+    auto load = [&](const T* from, int k0, auto tail) {
+        Turn t;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int k = k0 + i * 32 + kl;
-            wv[i] = load_eight<T, decltype(tail)::value>(w, k, g.K);
-            xv[i] = load_eight<T, decltype(tail)::value>(x, k, g.K);
-        }
+        for (int i = 0; i < CH; ++i) t.v[i] = load_eight<T, decltype(tail)::value>(from, k0 + i * 32 + kl, g.K);
+        return t;
+    };
+    auto multiply = [&](const Turn& wt, const Turn& xt) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < CH; ++i) {
             frag xf[NP], wf[NP];
-            pieces_of<T>(xv[i], xf);
-            pieces_of<T>(wv[i], wf);
+            pieces_of<T>(xt.v[i], xf);
+            pieces_of<T>(wt.v[i], wf);
 #pragma unroll
             for (int sum = NP - 1; sum >= 0; --sum)
 #pragma unroll
                 for (int p = 0; p <= sum; ++p) acc = mma16(wf[p], xf[sum - p], acc);
         }
     };
-    const int whole = g.K / 128 * 128;
-#pragma unroll 2
-    for (int k0 = wave * 128; k0 < whole; k0 += W * 128) chunk(k0, std::false_type());
-    if (whole < g.K && (whole / 128) % W == wave) chunk(whole, std::true_type());
+    const int whole = g.K / CE * CE;
+    // The weights of the next turn are asked for before this one's are multiplied.  The last turn asks for its own again (out of the
+    // caches): without a branch the compiler knows what is in flight and waits for no more than it needs.
+    int k = wave * CE;
+    if (k < whole) {
+        auto after = [&](int at) { return at + W * CE < whole ? at + W * CE : at; };
+        Turn w0 = load(w, k, std::false_type()), w1;
+        for (;;) {
+            const Turn x0 = load(x, k, std::false_type());
+            w1 = load(w, after(k), std::false_type());
+            multiply(w0, x0);
+            k += W * CE;
+            if (k >= whole) break;
+            const Turn x1 = load(x, k, std::false_type());
+            w0 = load(w, after(k), std::false_type());
+            multiply(w1, x1);
+            k += W * CE;
+            if (k >= whole) break;
+        }
+    }
+    if (whole < g.K && (whole / CE) % W == wave) multiply(load(w, whole, std::true_type()), load(x, whole, std::true_type()));
     // lane: input row lane % 16, weight rows 4 (lane / 16) ... + 3
 #pragma unroll
     for (int e = 0; e < 4; ++e) s_sum[wave][r][4 * (lane >> 4) + e] = acc[e];
@@ -105,7 +123,8 @@ template <typename T, int W> static void launch_waves(const GemmArgs& g, bool ga
     else hipLaunchKernelGGL((k_dense_rows<T, W, false>), dim3((g.N + 15) / 16), dim3(64 * W), 0, st, g);
 }
 template <typename T> static void launch_rows(const GemmArgs& g, bool gated, hipStream_t st) {
-    if (g.K > 1024) launch_waves<T, 16>(g, gated, st); else launch_waves<T, 8>(g, gated, st);
+    // float needs twice the registers a turn: eight waves; 16 bit from 1025 columns on sixteen
+    if (sizeof(T) == 2 && g.K > 1024) launch_waves<T, sizeof(T) == 2 ? 16 : 8>(g, gated, st); else launch_waves<T, 8>(g, gated, st);
 }
 
 int dense_rows(const GemmArgs& g, int dtype, bool gated, hipStream_t st) {
