@@ -69,7 +69,7 @@ def laid_out(t, how):
 
 
 SHAPES = [(1, 1, 1), (1, 4096, 72), (2, 129, 5), (5, 64, 130), (11, 50, 64), (16, 1000, 33), (17, 50, 64), (64, 64, 64), (65, 8, 1),
-          (129, 130, 67), (200, 257, 300), (1000, 96, 33), (40, 3000, 24), (257, 512, 384), (2500, 48, 40), (3, 8200, 9)]
+          (129, 130, 67), (200, 257, 300), (1000, 96, 33), (40, 3000, 24), (257, 512, 384), (2500, 48, 40), (3, 8200, 9), (30, 1000, 40), (4, 1301, 35), (7, 2049, 2050)]
 
 
 def linear_case(m, k, n, dtype, act, bias, residual, how, seed):

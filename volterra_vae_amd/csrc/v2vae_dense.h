@@ -250,8 +250,8 @@ int gemm_split(const GemmArgs&, int layout, bool gated, int tile, hipStream_t); 
 int gemm_staged_bf16(const GemmArgs&, int layout, bool gated, int tile, hipStream_t);
 int gemm_staged_f16(const GemmArgs&, int layout, bool gated, int tile, hipStream_t);
 
-// one to sixteen rows (v2vae_dense_rows.hip)
-constexpr int ROWS_MAX = 16;
+// few rows (v2vae_dense_rows.hip); beyond, the tiled products read the weights as fast
+inline int64_t few_rows(int dtype) { return dtype == V2VAE_F32 ? 32 : 16; }
 int dense_rows(const GemmArgs& g, int dtype, bool gated, hipStream_t st);
 
 int dense_launch_error(const char* where);  // V2VAE_OK, or V2VAE_ELAUNCH with the text kept for v2vae_last_error

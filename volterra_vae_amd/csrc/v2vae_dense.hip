@@ -246,7 +246,7 @@ static Packs packs_of(const v2vae_dense* d, bool gated, bool backward) {
     Packs p = {};
     p.ld_in = (int)((d->in + 7) / 8 * 8);
     p.ld_out = (int)d->out;
-    if (d->dtype == V2VAE_F32 || d->rows <= ROWS_MAX || d->in < 32 || d->out < 32) return p;
+    if (d->dtype == V2VAE_F32 || d->rows <= few_rows(d->dtype) || d->in < 32 || d->out < 32) return p;
     if ((double)d->rows * d->in * d->out * (gated ? 2 : 1) < (backward ? PACK_BACKWARD : PACK_FORWARD)) return p;
     const bool odd = d->in % 8 != 0;
     p.x = odd || d->ld_x % 8 != 0;
@@ -363,7 +363,7 @@ static int forward(const v2vae_dense* d, const void* x, const void* w0, const vo
         const int rc = use_planes(g, p, false, gated, (char*)ws, st);
         if (rc != V2VAE_OK) return rc;
     }
-    if (d->rows <= ROWS_MAX) return dense_rows(g, d->dtype, gated, st);
+    if (d->rows <= few_rows(d->dtype)) return dense_rows(g, d->dtype, gated, st);
     const Packs k = packs_of(d, gated, false);
     char* at = (char*)ws + p.bytes;
     if (k.x) {
@@ -525,7 +525,7 @@ extern "C" {
 size_t v2vae_linear_workspace_bytes(const v2vae_dense* d, int backward) {
     if (check_dense(d, false, backward != 0, false) != V2VAE_OK) return 0;
     if (backward) return bwd_layout(d, false).total;
-    if (d->rows <= ROWS_MAX) return 0;
+    if (d->rows <= few_rows(d->dtype)) return 0;
     const Packs k = packs_of(d, false, false);
     return planes_of(d, false, false).bytes + k.x_bytes + k.w_bytes + partial_bytes(d->rows, d->out, d->in, 1, 1, d->dtype, false);
 }
@@ -533,7 +533,7 @@ size_t v2vae_linear_workspace_bytes(const v2vae_dense* d, int backward) {
 size_t v2vae_gated_workspace_bytes(const v2vae_dense* d, int backward) {
     if (check_dense(d, true, backward != 0, false) != V2VAE_OK) return 0;
     if (backward) return bwd_layout(d, true).total;
-    if (d->rows <= ROWS_MAX) return 0;
+    if (d->rows <= few_rows(d->dtype)) return 0;
     const Packs k = packs_of(d, true, false);
     return planes_of(d, true, false).bytes + k.x_bytes + k.w_bytes + partial_bytes(d->rows, d->out, d->in, 1, 1, d->dtype, true);
 }
