@@ -173,9 +173,10 @@ static Cut cut_product(int64_t M, int64_t N, int64_t K, int segs, int batch, int
     if (dtype == V2VAE_F32) {
         const int64_t rows = (M + 127) / 128, wide = rows * ((N * (gated ? 2 : 1) + 127) / 128) * batch;
         const int64_t narrow = rows * ((N * (gated ? 2 : 1) + 63) / 64) * batch;
-        // 128 columns a tile unless that leaves too few workgroups or a half-empty last column of tiles (130 columns, 65536 rows: the
-        // two gradient products take 60 and 55 us with 64 columns a tile, 66 and 76 us with 128)
-        c.tile = (wide >= 256 || wide * (steps / 8) >= 256) && wide * 2 == narrow ? TILE_128 : TILE_64;
+        // 128 columns a tile where that leaves two workgroups a compute unit, of at least 16 steps if the contraction is cut (300 x 2000 x 2000 forward: 39 us with 128 columns, 31 with
+        // 64) and no half-empty last column of tiles (130 columns, 65536 rows: the two gradient products take 60 and 55 us with 64
+        // columns a tile, 66 and 76 with 128); 32768 x 256 x 512 the other way round: gated forward 135 us with 128, 150 with 64
+        c.tile = (wide >= 512 || wide * (steps / 16) >= 512) && wide * 2 == narrow ? TILE_128 : TILE_64;
         tiles = c.tile == TILE_128 ? wide : narrow;
     } else if (direct && tiles_of(256) >= 128 && full(tiles_of(256), 256) >= 0.88 * full(tiles_of(128), 512)) {
         c.tile = TILE_256;
@@ -188,8 +189,11 @@ static Cut cut_product(int64_t M, int64_t N, int64_t K, int segs, int batch, int
         tiles = ((M + 63) / 64) * ((N + 63) / 64) * batch;
     }
     if (tiles < 256) {
+        // The contraction in parts, to two workgroups a compute unit; a part is eight steps at least (1000 x 1000 x 1000 float32 forward:
+        // 29 us, 38 with four), four where there are few tiles (100 x 500 x 700: 19 us with eight, 15 with four).
+        const int64_t least = tiles < 32 ? 4 : 8;
         s = 512 / (tiles < 1 ? 1 : tiles);
-        if (s > steps / 8) s = steps / 8;
+        if (s > steps / least) s = steps / least;
         if (s < 1) s = 1;
     }
     c.per = (int)((steps + s - 1) / s);
