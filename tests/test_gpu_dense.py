@@ -433,3 +433,12 @@ def test_a_captured_block_replays_with_new_inputs():
             torch.cuda.synchronize()
             for p, q in zip(captured, eager):
                 assert torch.equal(p, q)
+
+
+def test_every_tile_width_of_the_float32_product():
+    """Column counts for which tiles of 64, 96, 128 and 160 columns are chosen, in both directions of a layer."""
+    from volterra_vae_amd.dense_ops import linear_backward, linear_forward
+    for k, n in ((40, 20), (96, 70), (130, 128), (150, 300), (161, 95), (300, 33)):
+        x, w, b, r, dy = linear_case(66000, k, n, torch.float32, "silu", True, True, "odd" if k % 2 else "plain", k)
+        y, z = linear_forward(x, w, b, residual=r, activation="silu", keep=True)
+        check_linear(x, w, b, r, dy, "silu", y, linear_backward(dy, x, w, z, activation="silu"), torch.float32)

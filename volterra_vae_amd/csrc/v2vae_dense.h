@@ -242,7 +242,7 @@ __device__ __forceinline__ void finish_gated(const GemmArgs& g, int64_t m, int n
 }
 // launchers, one object file per element type; 0 or a V2VAE_E* code
 enum { LAYOUT_KK = 0, LAYOUT_KM = 1, LAYOUT_MM = 2 };  // A / B with the contraction (K) or the row index (M) contiguous
-enum { TILE_128 = 0, TILE_64 = 1, TILE_256 = 2 };
+enum { TILE_128, TILE_64, TILE_256, TILE_96, TILE_160 };
 int gemm_direct_bf16(const GemmArgs&, int layout, bool gated, int tile, hipStream_t);
 int gemm_direct_f16(const GemmArgs&, int layout, bool gated, int tile, hipStream_t);
 int split_planes(const GemmArgs&, bool transposed, bool gated, int N, int K, hipStream_t);  // b[], ldb[]: N x K weights

@@ -162,7 +162,7 @@ constexpr double PACK_FORWARD = 4e9, PACK_BACKWARD = 3e8;  // rows x in x out fr
 // How a product M x N x K is cut: tile size and the number of parts of the contraction.  `direct`: 16-bit operands, aligned.
 // The workspace does not know the alignment, so it is laid out for the larger of the two cuts.
 struct Cut { int tile, splits, per; };
-static Cut cut_product(int64_t M, int64_t N, int64_t K, int segs, int batch, int dtype, bool gated, bool direct) {
+static Cut cut_product(int64_t M, int64_t N, int64_t K, int segs, int batch, int dtype, bool gated, bool direct, bool planes) {
     const int64_t bk = dtype == V2VAE_F32 ? 32 : 64, steps = ((K + bk - 1) / bk) * segs;
     auto tiles_of = [&](int64_t t) { return ((M + t - 1) / t) * ((N * (gated ? 2 : 1) + t - 1) / t) * batch; };
     // A compute unit holds one 256 x 256 tile or two of 128 x 128.  The larger tile runs 1.12 times as fast (8192 x 4096 x 4096
@@ -178,6 +178,20 @@ static Cut cut_product(int64_t M, int64_t N, int64_t K, int segs, int batch, int
         // columns a tile, 66 and 76 with 128); 32768 x 256 x 512 the other way round: gated forward 135 us with 128, 150 with 64
         c.tile = (wide >= 512 || wide * (steps / 16) >= 512) && wide * 2 == narrow ? TILE_128 : TILE_64;
         tiles = c.tile == TILE_128 ? wide : narrow;
+        if (planes && !gated) {
+            // One matrix of split weights: of the widths that leave two workgroups a compute unit, the one of least work.  A step
+            // of a tile costs 12 cycles a column in matrix instructions and about 500 for A's splitting and the loads, whatever
+            // the width (65536 x 256 -> 130: 60 us with 64 columns, 51 with 160).
+            const struct { int tile, width; } widths[] = {{TILE_64, 64}, {TILE_96, 96}, {TILE_128, 128}, {TILE_160, 160}};
+            int64_t best = 0;
+            for (const auto& w : widths) {
+                const int64_t across = (N + w.width - 1) / w.width, cost = across * (12 * w.width + 500);
+                if (w.tile != TILE_64 && (rows * across < 512 || cost >= best)) continue;
+                best = cost;
+                c.tile = w.tile;
+                tiles = rows * across;
+            }
+        }
     } else if (direct && tiles_of(256) >= 128 && full(tiles_of(256), 256) >= 0.88 * full(tiles_of(128), 512)) {
         c.tile = TILE_256;
         tiles = tiles_of(256);
@@ -202,10 +216,10 @@ static Cut cut_product(int64_t M, int64_t N, int64_t K, int segs, int batch, int
     if (c.splits < 1) c.splits = 1;
     return c;
 }
-static size_t partial_bytes(int64_t M, int64_t N, int64_t K, int segs, int batch, int dtype, bool gated) {
+static size_t partial_bytes(int64_t M, int64_t N, int64_t K, int segs, int batch, int dtype, bool gated, bool planes) {
     int most = 1;
     for (int direct = 0; direct < (dtype == V2VAE_F32 ? 1 : 2); ++direct) {
-        const Cut c = cut_product(M, N, K, segs, batch, dtype, gated, direct);
+        const Cut c = cut_product(M, N, K, segs, batch, dtype, gated, direct, planes);
         if (c.splits > most) most = c.splits;
     }
     return most > 1 ? round_up((size_t)most * batch * M * N * (gated ? 2 : 1) * 4) : 0;
@@ -299,8 +313,8 @@ static BwdLayout bwd_layout(const v2vae_dense* d, bool gated) {
     l.w = o;
     o += p.w_bytes;
     l.prod = o;
-    const size_t a = partial_bytes(d->rows, d->in, d->out, n, 1, d->dtype, false);
-    const size_t b = partial_bytes(d->out, d->in, d->rows, 1, n, d->dtype, false);
+    const size_t a = partial_bytes(d->rows, d->in, d->out, n, 1, d->dtype, false, planes_of(d, gated, true).bytes > 0);
+    const size_t b = partial_bytes(d->out, d->in, d->rows, 1, n, d->dtype, false, false);
     l.total = o + (a > b ? a : b);
     return l;
 }
@@ -321,7 +335,7 @@ static int run_product(GemmArgs& g, int dtype, int layout, bool gated, float* pa
     // straight to LDS: 16-bit, whole pieces, offsets inside a tile below 2^31, one stride
     const int64_t ld_max = g.lda > g.ldb[0] ? (g.lda > g.ldb[1] ? g.lda : g.ldb[1]) : (g.ldb[0] > g.ldb[1] ? g.ldb[0] : g.ldb[1]);
     const bool direct = dtype != V2VAE_F32 && whole_a && whole_b && ld_max <= (1 << 21) && (gated || g.ldb[0] == g.ldb[1]);
-    const Cut c = cut_product(g.M, g.N, g.K, g.segs, g.batch, dtype, gated, direct);
+    const Cut c = cut_product(g.M, g.N, g.K, g.segs, g.batch, dtype, gated, direct, g.planes != nullptr);
     g.splits = c.splits;
     g.steps_per_split = c.per;
     g.partial = c.splits > 1 ? partial : nullptr;
@@ -531,7 +545,8 @@ size_t v2vae_linear_workspace_bytes(const v2vae_dense* d, int backward) {
     if (backward) return bwd_layout(d, false).total;
     if (d->rows <= few_rows(d->dtype)) return 0;
     const Packs k = packs_of(d, false, false);
-    return planes_of(d, false, false).bytes + k.x_bytes + k.w_bytes + partial_bytes(d->rows, d->out, d->in, 1, 1, d->dtype, false);
+    const size_t planes = planes_of(d, false, false).bytes;
+    return planes + k.x_bytes + k.w_bytes + partial_bytes(d->rows, d->out, d->in, 1, 1, d->dtype, false, planes > 0);
 }
 
 size_t v2vae_gated_workspace_bytes(const v2vae_dense* d, int backward) {
@@ -539,7 +554,8 @@ size_t v2vae_gated_workspace_bytes(const v2vae_dense* d, int backward) {
     if (backward) return bwd_layout(d, true).total;
     if (d->rows <= few_rows(d->dtype)) return 0;
     const Packs k = packs_of(d, true, false);
-    return planes_of(d, true, false).bytes + k.x_bytes + k.w_bytes + partial_bytes(d->rows, d->out, d->in, 1, 1, d->dtype, true);
+    const size_t planes = planes_of(d, true, false).bytes;
+    return planes + k.x_bytes + k.w_bytes + partial_bytes(d->rows, d->out, d->in, 1, 1, d->dtype, true, planes > 0);
 }
 
 int v2vae_linear_fwd(const v2vae_dense* d, const void* x, const void* w, const void* bias, const void* residual, void* y, float* z,

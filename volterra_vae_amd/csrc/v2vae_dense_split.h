@@ -34,11 +34,11 @@ __device__ __forceinline__ float tail_at(const char* base, unsigned off, int k, 
 }
 
 template <int TN, bool AKC, int FROM, bool GATED>
-__global__ __launch_bounds__(256, FROM == B_PLANES ? (TN == 4 ? 3 : 4) : 2) void k_gemm_split(GemmArgs g) {
+__global__ __launch_bounds__(256, FROM == B_PLANES ? (TN <= 2 ? 4 : TN <= 4 ? 3 : 2) : 2) void k_gemm_split(GemmArgs g) {
     constexpr int BK = 32, BM = 128, BN = 32 * TN, EPI = 4 * EPI_BYTES<2>;
     constexpr bool PLANES = FROM == B_PLANES, BKC = FROM == B_ROWS;
     constexpr int ROWB = PLANES ? 64 : 80, PLANE = BN * ROWB, TILE = 3 * PLANE;
-    static_assert(TN % 2 == 0, "the epilogue takes blocks in pairs");
+    static_assert(TN % 2 == 0 || (PLANES && !GATED), "tiles of an odd number of blocks: weights from planes, one matrix");
     __shared__ __align__(1024) char lds[2 * TILE > EPI ? 2 * TILE : EPI];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
     const int out_bn = GATED ? BN / 2 : BN;
@@ -61,14 +61,15 @@ __global__ __launch_bounds__(256, FROM == B_PLANES ? (TN == 4 ? 3 : 4) : 2) void
     const bool over = AKC && (int64_t)(g.M - mt - BM) * lda >= BK;
     typedef struct __attribute__((packed, aligned(4))) { float e[4]; } Loose4;
     constexpr int PASS = BN / 32, KT = BK * BN / 256;  // B_ROWS: 16-byte loads, B_COLUMNS: elements, per thread
-    constexpr int NB = PLANES ? 3 * BN / 64 : BKC ? PASS : 1;
+    constexpr int LOADS = 3 * BN / 16, NB = PLANES ? (LOADS + 3) / 4 : BKC ? PASS : 1;
     struct SetA { float v[2][8]; };
     struct SetB { float v[PLANES ? 1 : KT]; };
     unsigned off_b[NB];
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
         if constexpr (PLANES) {  // 16 rows of one plane an instruction
-            const int i = j * 4 + wave, plane = i / (BN / 16), r = i % (BN / 16) * 16 + (lane >> 2), piece = (lane & 3) ^ ((r >> 2) & 3);
+            const int i = j * 4 + wave < LOADS ? j * 4 + wave : LOADS - 1, plane = i / (BN / 16);
+            const int r = i % (BN / 16) * 16 + (lane >> 2), piece = (lane & 3) ^ ((r >> 2) & 3);
             const int last = g.plane_rows - 1, row = tn * BN + r < last ? tn * BN + r : last;
             off_b[j] = (unsigned)((int64_t)plane * g.plane_bytes + (int64_t)(row - tn * BN) * g.plane_ld * 2 + piece * 16);
         } else if constexpr (BKC) {
@@ -114,7 +115,8 @@ __global__ __launch_bounds__(256, FROM == B_PLANES ? (TN == 4 ? 3 : 4) : 2) void
     auto planes_to_lds = [&](int s, int buf) {
         const char* const b = uniform64((const char*)g.planes + ((int64_t)tn * BN * g.plane_ld + (int64_t)s * BK) * 2);
 #pragma unroll
-        for (int j = 0; j < NB; ++j) load_to_lds(b, off_b[j], lds0 + buf + (j * 4 + wave) * 1024);
+        for (int j = 0; j < NB; ++j)
+            if (LOADS % 4 == 0 || j * 4 + wave < LOADS) load_to_lds(b, off_b[j], lds0 + buf + (j * 4 + wave) * 1024);
     };
     auto fetch_a = [&](int s, SetA& ra) {
         const int seg = s >= steps_seg ? 1 : 0, k0 = (s - seg * steps_seg) * BK, left = g.K - k0;
@@ -279,9 +281,13 @@ __global__ __launch_bounds__(256, FROM == B_PLANES ? (TN == 4 ? 3 : 4) : 2) void
 
     float* const part = g.partial ? g.partial + ((int64_t)bat * g.splits + split) * ((int64_t)g.M * (GATED ? 2 : 1) * g.N) : nullptr;
 #pragma unroll
-    for (int j = 0; j < TN; j += 2) {
+    for (int j = 0; j + 1 < TN; j += 2) {
         const f32x16 pair[2] = {acc[j], acc[j + 1]};
         finish_block<float, 2, GATED>(g, pair, lds + wave * EPI_BYTES<2>, lane, m0, n0 + (GATED ? 16 : 32) * j, part, bat);
+    }
+    if constexpr (TN % 2 != 0) {
+        const f32x16 last[1] = {acc[TN - 1]};
+        finish_block<float, 1, false>(g, last, lds + wave * EPI_BYTES<2>, lane, m0, n0 + 32 * (TN - 1), part, bat);
     }
 }
 
@@ -337,6 +343,10 @@ template <int TN, bool AKC, int FROM, bool GATED> void launch_split(const GemmAr
     if (g.partial) launch_join<float, GATED>(g, st);
 }
 template <bool AKC, int FROM, bool GATED> void pick_split(const GemmArgs& g, int tile, hipStream_t st) {
+    if constexpr (FROM == B_PLANES && !GATED) {
+        if (tile == TILE_96) return launch_split<3, AKC, FROM, GATED>(g, st);
+        if (tile == TILE_160) return launch_split<5, AKC, FROM, GATED>(g, st);
+    }
     if (tile == TILE_128) launch_split<4, AKC, FROM, GATED>(g, st); else launch_split<2, AKC, FROM, GATED>(g, st);
 }
 
