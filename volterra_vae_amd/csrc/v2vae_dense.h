@@ -26,9 +26,10 @@ template <typename T> struct Vec16 {
 };
 
 template <typename T> struct Elem;
-template <> struct Elem<float> { static constexpr int NP = 3, BK = 32; typedef bf16x8 frag; };
-template <> struct Elem<bf16_t> { static constexpr int NP = 1, BK = 64; typedef bf16x8 frag; };
-template <> struct Elem<f16_t> { static constexpr int NP = 1, BK = 64; typedef f16x8 frag; };
+// bf16 pieces of an element, operand of a matrix instruction
+template <> struct Elem<float> { static constexpr int NP = 3; typedef bf16x8 frag; };
+template <> struct Elem<bf16_t> { static constexpr int NP = 1; typedef bf16x8 frag; };
+template <> struct Elem<f16_t> { static constexpr int NP = 1; typedef f16x8 frag; };
 
 __device__ __forceinline__ f32x16 mma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mma32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
@@ -240,9 +241,9 @@ __device__ __forceinline__ void finish_gated(const GemmArgs& g, int64_t m, int n
     for (int e = 0; e < C; ++e) gate[e] *= up[e];
     store_columns<T, C>(g.c[0], m * g.ldc + n, count, whole, gate);
 }
-// launchers, one object file per element type; 0 or a V2VAE_E* code
+// launchers; 0 or a V2VAE_E* code
 enum { LAYOUT_KK = 0, LAYOUT_KM = 1, LAYOUT_MM = 2 };  // A / B with the contraction (K) or the row index (M) contiguous
-enum { TILE_128, TILE_64, TILE_256, TILE_96, TILE_160 };
+enum { TILE_128, TILE_64, TILE_256, TILE_96, TILE_160 };  // float32: columns of a tile of 128 rows; else both sides
 int gemm_direct_bf16(const GemmArgs&, int layout, bool gated, int tile, hipStream_t);
 int gemm_direct_f16(const GemmArgs&, int layout, bool gated, int tile, hipStream_t);
 int split_planes(const GemmArgs&, bool transposed, bool gated, int N, int K, hipStream_t);  // b[], ldb[]: N x K weights

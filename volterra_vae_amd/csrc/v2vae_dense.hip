@@ -173,9 +173,10 @@ static Cut cut_product(int64_t M, int64_t N, int64_t K, int segs, int batch, int
     if (dtype == V2VAE_F32) {
         const int64_t rows = (M + 127) / 128, wide = rows * ((N * (gated ? 2 : 1) + 127) / 128) * batch;
         const int64_t narrow = rows * ((N * (gated ? 2 : 1) + 63) / 64) * batch;
-        // 128 columns a tile where that leaves two workgroups a compute unit, of at least 16 steps if the contraction is cut (300 x 2000 x 2000 forward: 39 us with 128 columns, 31 with
-        // 64) and no half-empty last column of tiles (130 columns, 65536 rows: the two gradient products take 60 and 55 us with 64
-        // columns a tile, 66 and 76 with 128); 32768 x 256 x 512 the other way round: gated forward 135 us with 128, 150 with 64
+        // 128 columns a tile where that leaves two workgroups a compute unit, of at least 16 steps if the contraction is cut (300 x
+        // 2000 x 2000 forward: 39 us with 128 columns, 31 with 64) and no half-empty last column of tiles (130 columns, 65536 rows:
+        // the weight gradient takes 55 us with 64 columns a tile, 76 with 128); 32768 x 256 x 512 the other way round: gated forward
+        // 135 us with 128, 150 with 64
         c.tile = (wide >= 512 || wide * (steps / 16) >= 512) && wide * 2 == narrow ? TILE_128 : TILE_64;
         tiles = c.tile == TILE_128 ? wide : narrow;
         if (planes && !gated) {
@@ -203,8 +204,8 @@ static Cut cut_product(int64_t M, int64_t N, int64_t K, int segs, int batch, int
         tiles = ((M + 63) / 64) * ((N + 63) / 64) * batch;
     }
     if (tiles < 256) {
-        // The contraction in parts, to two workgroups a compute unit; a part is eight steps at least (1000 x 1000 x 1000 float32 forward:
-        // 29 us, 38 with four), four where there are few tiles (100 x 500 x 700: 19 us with eight, 15 with four).
+        // The contraction in parts, to two workgroups a compute unit; a part is eight steps at least (1000 x 1000 x 1000 float32
+        // forward: 29 us, 38 with four), four where there are few tiles (100 x 500 x 700: 19 us with eight, 15 with four).
         const int64_t least = tiles < 32 ? 4 : 8;
         s = 512 / (tiles < 1 ? 1 : tiles);
         if (s > steps / least) s = steps / least;
@@ -237,7 +238,7 @@ static Planes planes_of(const v2vae_dense* d, bool gated, bool transposed) {
     p.ld = (int)(transposed ? pad(d->out) * (gated ? 2 : 1) : pad(d->in));
     p.plane = (size_t)p.rows * p.ld * 2;
     // a tile's lane offsets span all three planes in 32 bits, and its columns are counted in 31
-    if (2 * p.plane + (size_t)128 * p.ld * 2 >= (size_t)0xFFFF0000u) return Planes{};
+    if (2 * p.plane + (size_t)160 * p.ld * 2 >= (size_t)0xFFFF0000u) return Planes{};
     p.bytes = round_up(3 * p.plane);
     return p;
 }
@@ -255,9 +256,8 @@ static void slope_shape(int64_t M, int64_t N, int V, int* cx, int* gx, int* chun
     *chunks = (int)(n < 1 ? 1 : n);
 }
 
-// workspace of the backward pass: dz (two for the gated block), the column partials, the partials of the two products
-// 16-bit operands whose rows are not whole 16-byte pieces: copied when the products are large enough to win the copies back.  Measured
-// in bf16, forward and gradients, us without / with copies: 4001 x 2047 x 2043 86 / 63 and 518 / 138, 2000 x 101 x 3999 80 / 65 backward,
+// 16-bit operands whose rows are not whole 16-byte pieces: copied when the products are large enough to win the copies back.
+// Measured in bf16, forward and gradients, us without / with copies: 4001 x 2047 x 2043 86 / 63 and 518 / 138, 2000 x 101 x 3999 80 / 65 backward,
 // 65537 x 131 x 257 55 / 67 forward (therefore without) and 186 / 129 backward, 1001 x 515 x 1027 60 / 57 backward.
 struct Packs { bool x, w, dz; size_t x_bytes, w_bytes; int ld_in, ld_out; };
 static Packs packs_of(const v2vae_dense* d, bool gated, bool backward) {
@@ -284,6 +284,7 @@ static void pack_rows(const void* s0, const void* s1, int64_t ld0, int64_t ld1, 
     if (blocks > 0) hipLaunchKernelGGL(k_pack_rows, dim3((unsigned)blocks, s1 ? 2 : 1), dim3(256), 0, st, a);
 }
 
+// workspace of the backward pass: dz (two for the gated block), the column partials, planes or copies, the partials of a product
 struct BwdLayout { size_t dz[2], part[2], planes, x, w, prod, total; };
 static BwdLayout bwd_layout(const v2vae_dense* d, bool gated) {
     BwdLayout l;

@@ -1,16 +1,17 @@
-// The staged matrix product of the dense layers: D[m][n] = sum_k A(m, k) B(n, k), any strides, any alignment, any size.
+// The staged matrix product of the dense layers for 16-bit operands, and what all their products share: the order of tiles, the
+// epilogue, the join of a split contraction.  D[m][n] = sum_k A(m, k) B(n, k), any strides, any alignment, any size.
 //
 // A workgroup of four waves owns a (64 TM) x (64 TN) tile of D, each wave 32 TM x 32 TN of it in accumulators of
-// v_mfma_f32_32x32x16.  A contraction step of 128 bytes of every row goes global -> registers -> LDS: the next step's loads are
+// v_mfma_f32_32x32x16.  A contraction step of 64 elements of every row goes global -> registers -> LDS: the next step's loads are
 // in flight while the current one is multiplied, and the step through registers is what makes the rest general:
-//  * float32: every element is split into three bf16 pieces (exact sum, see v2vae_bf16_split.h; here the gfx950 conversion
-//    instruction rounds two at a time) and six piece products per element pair are accumulated in float: float32 results at six
-//    bf16 instructions (bf16 pipe / 6 = 417 TF) where the f32 matrix instructions give 157 TF.
 //  * an operand whose rows, not whose contraction, are contiguous (both operands of a weight gradient) is read with lanes along
 //    the rows and transposed by the store into LDS;
-//  * rows and contraction ends that do not fill a tile, and rows that are not 16-byte aligned, are loaded element by element.
-// LDS rows are 128 (float: 64) bytes of 16-bit pieces plus 16 bytes: the row stride is an odd multiple of 16 bytes, so the
-// 16-byte reads of 16 consecutive rows touch every bank once.
+//  * rows and contraction ends that do not fill a tile are loaded element by element, and rows may start at any element.
+// LDS rows are 128 bytes plus 16: the row stride is an odd multiple of 16 bytes, so the 16-byte reads of 16 consecutive rows touch
+// every bank once.
+//
+// Bound by the loads, which are many and small for rows that are not 16-byte aligned: 65537 x 131 -> 257 bf16 forward 55 us (80 TF);
+// from PACK_FORWARD and PACK_BACKWARD on such operands are copied for the direct kernel instead (both sides there).
 #ifndef V2VAE_DENSE_GEMM_H
 #define V2VAE_DENSE_GEMM_H
 #include "v2vae_dense.h"
@@ -22,7 +23,7 @@ template <typename T, int ROWS, bool KC> struct Stage;
 
 // contraction contiguous: eight lanes along a row (16 bytes each), 32 rows a pass
 template <typename T, int ROWS> struct Stage<T, ROWS, true> {
-    static constexpr int E = 16 / sizeof(T), PASS = ROWS / 32, BK = Elem<T>::BK, ROWB = BK * 2 + 16;
+    static constexpr int E = 8, PASS = ROWS / 32, BK = 64, ROWB = BK * 2 + 16;
     Vec16<T> v[PASS];
     // row_of(r): pointer of tile row r at k = 0, or NULL beyond the matrix
     template <typename F> __device__ __forceinline__ void load(int tid, int k0, int K, F row_of) {
@@ -44,24 +45,13 @@ template <typename T, int ROWS> struct Stage<T, ROWS, true> {
     }
     __device__ __forceinline__ void store(int tid, char* lds) const {
 #pragma unroll
-        for (int j = 0; j < PASS; ++j) {
-            char* d = lds + ((tid >> 3) + 32 * j) * ROWB;
-            if constexpr (sizeof(T) == 4) {
-                unsigned lo[3], hi[3];
-                split_pair(v[j].e[0], v[j].e[1], lo);
-                split_pair(v[j].e[2], v[j].e[3], hi);
-#pragma unroll
-                for (int p = 0; p < 3; ++p) *reinterpret_cast<u32x2*>(d + p * ROWS * ROWB + (tid & 7) * 8) = u32x2{lo[p], hi[p]};
-            } else {
-                *reinterpret_cast<u32x4*>(d + (tid & 7) * 16) = v[j].raw;
-            }
-        }
+        for (int j = 0; j < PASS; ++j) *reinterpret_cast<u32x4*>(lds + ((tid >> 3) + 32 * j) * ROWB + (tid & 7) * 16) = v[j].raw;
     }
 };
 
 // rows contiguous: lanes along the rows (element loads, coalesced at any alignment), every thread KT consecutive k of its row
 template <typename T, int ROWS> struct Stage<T, ROWS, false> {
-    static constexpr int BK = Elem<T>::BK, ROWB = BK * 2 + 16, KT = BK * ROWS / 256;
+    static constexpr int BK = 64, ROWB = BK * 2 + 16, KT = BK * ROWS / 256;
     T v[KT];
     template <typename F> __device__ __forceinline__ void load(int tid, int k0, int K, int64_t ld, F row_of) {
         const int k = k0 + (tid / ROWS) * KT;
@@ -72,24 +62,12 @@ template <typename T, int ROWS> struct Stage<T, ROWS, false> {
     }
     __device__ __forceinline__ void store(int tid, char* lds) const {
         char* d = lds + (tid % ROWS) * ROWB + (tid / ROWS) * KT * 2;
-        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int e = 0; e < KT; e += 8) {
-                unsigned q[4][3];
+        for (int e = 0; e < KT; e += 8) {
+            Vec16<T> w;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) split_pair(v[e + 2 * i], v[e + 2 * i + 1], q[i]);
-#pragma unroll
-                for (int p = 0; p < 3; ++p)
-                    *reinterpret_cast<u32x4*>(d + p * ROWS * ROWB + e * 2) = u32x4{q[0][p], q[1][p], q[2][p], q[3][p]};
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < KT; e += 8) {
-                Vec16<T> w;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) w.e[i] = v[e + i];
-                *reinterpret_cast<u32x4*>(d + e * 2) = w.raw;
-            }
+            for (int i = 0; i < 8; ++i) w.e[i] = v[e + i];
+            *reinterpret_cast<u32x4*>(d + e * 2) = w.raw;
         }
     }
 };
@@ -166,13 +144,13 @@ __device__ __forceinline__ void finish_block(const GemmArgs& g, const f32x16 (&a
 
 template <typename T, int TM, int TN, bool AKC, bool BKC, bool GATED>
 __global__ __launch_bounds__(256, 2) void k_gemm_staged(GemmArgs g) {
-    constexpr int NP = Elem<T>::NP, BK = Elem<T>::BK, ROWB = BK * 2 + 16, BM = 64 * TM, BN = 64 * TN;
+    constexpr int BK = 64, ROWB = BK * 2 + 16, BM = 64 * TM, BN = 64 * TN;
     static_assert(!GATED || TN == 2, "a gated wave holds one gate and one up block");
     typedef typename Elem<T>::frag frag;
-    constexpr int TILES = NP * (BM + BN) * ROWB, EPI = 4 * EPI_BYTES<TN>;
+    constexpr int TILES = (BM + BN) * ROWB, EPI = 4 * EPI_BYTES<TN>;
     __shared__ __align__(16) char lds[TILES > EPI ? TILES : EPI];
     char* const lds_a = lds;
-    char* const lds_b = lds + NP * BM * ROWB;
+    char* const lds_b = lds + BM * ROWB;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
     const int out_bn = GATED ? BN / 2 : BN;
     const int tiles_m = (g.M + BM - 1) / BM, tiles_n = (g.N + out_bn - 1) / out_bn;
@@ -227,23 +205,15 @@ __global__ __launch_bounds__(256, 2) void k_gemm_staged(GemmArgs g) {
         if (s + 1 < s_hi) fetch(s + 1);
 #pragma unroll
         for (int kk = 0; kk < BK / 16; ++kk) {
-            frag a[TM][NP], b[TN][NP];
+            frag a[TM], b[TN];
 #pragma unroll
-            for (int p = 0; p < NP; ++p) {
+            for (int i = 0; i < TM; ++i) a[i] = *reinterpret_cast<const frag*>(fa + i * 32 * ROWB + kk * 32);
 #pragma unroll
-                for (int i = 0; i < TM; ++i) a[i][p] = *reinterpret_cast<const frag*>(fa + (p * BM + i * 32) * ROWB + kk * 32);
+            for (int j = 0; j < TN; ++j) b[j] = *reinterpret_cast<const frag*>(fb + j * 32 * ROWB + kk * 32);
 #pragma unroll
-                for (int j = 0; j < TN; ++j) b[j][p] = *reinterpret_cast<const frag*>(fb + (p * BN + j * 32) * ROWB + kk * 32);
-            }
-            // piece products, the smallest first
+            for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int sum = NP - 1; sum >= 0; --sum)
-#pragma unroll
-                for (int p = 0; p <= sum; ++p)
-#pragma unroll
-                    for (int i = 0; i < TM; ++i)
-#pragma unroll
-                        for (int j = 0; j < TN; ++j) acc[i][j] = mma32(b[j][sum - p], a[i][p], acc[i][j]);
+                for (int j = 0; j < TN; ++j) acc[i][j] = mma32(b[j], a[i], acc[i][j]);
         }
         __syncthreads();
         if (s + 1 < s_hi) {

@@ -1,8 +1,8 @@
 // Few rows through a dense layer or a gated block: the form that answers single symbols (16 bit up to 16 rows, float up to 32).
 //
 // The weights are read once and nothing else counts, so the kernel is a stream over them.  A workgroup owns 16 weight rows (gated
-// block: 8 gate and 8 up rows of the same features); its waves (8, or 16) take turns along the contraction, 128 elements
-// each, and multiply on v_mfma_f32_16x16x32 with the input rows as the other operand (rows beyond the last repeat it): the matrix
+// block: 8 gate and 8 up rows of the same features); its waves (8, or 16) take turns along the contraction, 128 elements each, and
+// multiply on v_mfma_f32_16x16x32 with the input rows as the other operand (rows beyond the last repeat it): the matrix
 // instruction sums over lanes, which costs a vector kernel six shuffles per output and wave.  The fragments come straight from
 // memory (16 bytes a lane, any alignment); float operands are split into three bf16 pieces in registers (six products).  The
 // waves' sums are joined through LDS in a fixed order.
