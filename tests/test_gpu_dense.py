@@ -442,3 +442,49 @@ def test_every_tile_width_of_the_float32_product():
         x, w, b, r, dy = linear_case(66000, k, n, torch.float32, "silu", True, True, "odd" if k % 2 else "plain", k)
         y, z = linear_forward(x, w, b, residual=r, activation="silu", keep=True)
         check_linear(x, w, b, r, dy, "silu", y, linear_backward(dy, x, w, z, activation="silu"), torch.float32)
+
+
+def test_refusals():
+    from volterra_vae_amd._lib import V2VAEError
+    from volterra_vae_amd.dense_ops import gated_backward, gated_forward, gated_linear, linear, linear_backward, linear_forward
+    x, w, b = (torch.zeros(*s, device=dev()) for s in ((6, 5), (4, 5), (4,)))
+    neg = torch.zeros(6, 1, dtype=torch.complex64, device=dev()).conj().imag
+    assert neg.is_neg()
+    for match, args, kw in (
+            ("weight is torch.bfloat16", (x, w.bfloat16()), {}),
+            ("weight: 4 columns", (x, w[:, :4]), {}),
+            ("weight must have 2 dim", (x, w[0]), {}),
+            ("weight must have unit stride", (x, torch.zeros(4, 10, device=dev())[:, ::2]), {}),
+            ("x must have unit stride", (torch.zeros(5, 6, device=dev()).t(), w), {}),
+            ("weight: empty", (x, w[:0]), {}),
+            ("bias: 3 values", (x, w, b[:3]), {}),
+            ("bias is torch.float16", (x, w, b.half()), {}),
+            ("bias must have unit stride", (x, w, torch.zeros(1, device=dev()).expand(4)), {}),
+            ("residual: expected", (x, w, b), dict(residual=torch.zeros(6, 5, device=dev()))),
+            ("negation that is not carried out", (neg, w[:, :1]), {}),
+            ("negation that is not carried out", (x[:, :1], neg[:4]), {}),
+            ("weight must be|weight is on|weight must live", (x, w.cpu()), {})):
+        with pytest.raises((ValueError, RuntimeError), match=match):
+            linear(*args, **kw)
+    with pytest.raises(NotImplementedError, match="float32, bfloat16 or float16"):
+        linear(x.double(), w.double())
+    with pytest.raises(ValueError, match="weight_up: expected"):
+        gated_linear(x, w, w[:3])
+    with pytest.raises(ValueError, match="bias_up: 3 values"):
+        gated_linear(x, w, w, b, b[:3])
+    wide = torch.empty_strided((2, 5), ((1 << 22) + 1, 1), device=dev())
+    with pytest.raises(V2VAEError):
+        linear(wide, w)
+    with pytest.raises(V2VAEError):
+        linear_backward(torch.zeros(2, 4, device=dev()), wide, w)
+    y, z = linear_forward(x, w, b, activation="silu", keep=True)
+    for match, args in (("z: the pre-activations", (y, x, w)), ("kept pre-activations is", (y, x, w, z.half())),
+                        ("expected a contiguous", (y, x, w, z[:5])), ("expected a contiguous", (y, x, w, torch.zeros(6, 8, device=dev())[:, ::2][:, :4])),
+                        ("dy: expected", (y[:5], x, w, z)), ("dy is", (y.half(), x, w, z))):
+        with pytest.raises(ValueError, match=match + "|unit stride"):
+            linear_backward(*args, activation="silu")
+    h, gu = gated_forward(x, w, w, keep=True)
+    with pytest.raises(ValueError, match="expected a contiguous"):
+        gated_backward(h, x, w, w, gu[:, :5])
+    with pytest.raises(ValueError, match="dh: expected"):
+        gated_backward(h[:, :3], x, w, w, gu)

@@ -244,3 +244,29 @@ def test_a_captured_step_replays():
             graph.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(p, q) for p, q in zip(captured, eager))
+
+
+def test_refusals():
+    from volterra_vae_amd._lib import V2VAEError
+    from volterra_vae_amd.dense_ops import topk_distillation, topk_distillation_step
+    z, t = torch.zeros(6, 9, device=dev()), torch.zeros(6, 3, device=dev())
+    i, w = torch.zeros(6, 3, dtype=torch.int64, device=dev()), torch.ones(6, device=dev())
+    for error, match, args, kw in (
+            (NotImplementedError, "float32, bfloat16 or float16", (z.double(), t, i), {}),
+            (NotImplementedError, "teacher_logits", (z, t.double(), i), {}),
+            (ValueError, "int32 or int64", (z, t, i.short()), {}),
+            (ValueError, "expected", (z, t[:5], i), {}),
+            (ValueError, "expected", (z, t, i[:, :2]), {}),
+            (ValueError, "entries a row", (z, t[:, :0], i[:, :0]), {}),
+            (ValueError, "entries a row", (z, torch.zeros(6, 1025, device=dev()), torch.zeros(6, 1025, dtype=torch.int32, device=dev())), {}),
+            (ValueError, "no classes", (z[:, :0], t, i), {}),
+            (ValueError, "unit stride", (torch.zeros(9, 6, device=dev()).t(), t, i), {}),
+            (ValueError, "not differentiable in the teacher", (z, t.clone().requires_grad_(), i), {}),
+            (RuntimeError, "no CPU implementation", (z, t.cpu(), i), {}),
+            (V2VAEError, "v2vae_distill_fwd", (z[:1].expand(6, 9), t, i), {}),
+            *((ValueError, "temperature", (z, t, i), dict(temperature=x)) for x in (0.0, -1.0, 9e-5, 2e4, float("nan"), float("inf")))):
+        with pytest.raises(error, match=match):
+            topk_distillation(*args, **kw)
+    for bad in (w[:5], w.double(), torch.ones(1, device=dev()).expand(6)):
+        with pytest.raises(ValueError, match="row_weight"):
+            topk_distillation_step(z, t, i, bad)

@@ -6,8 +6,9 @@ may overlap (windows that slide over one received sequence are a matrix with the
 
 Two ways to train: the functions named above are differentiable; `linear_forward` / `linear_backward`, `gated_forward` /
 `gated_backward` and `topk_distillation_step` are the same passes with every gradient an explicit result, for training loops
-that run without autograd (and for HIP graphs, into which they can be captured).  `torch.ops.v2vae.linear`,
-`torch.ops.v2vae.gated_linear` and `torch.ops.v2vae.topk_distillation` are the differentiable forms as registered ops.
+that run without autograd, and for HIP graphs: these are what to capture (a backward pass of autograd that is captured while an
+eager graph of the same leaves lives ends the process).  `torch.ops.v2vae.linear`, `torch.ops.v2vae.gated_linear` and
+`torch.ops.v2vae.topk_distillation` are the differentiable forms as registered ops.
 """
 from __future__ import annotations
 
@@ -29,7 +30,7 @@ def _check_tensor(t, name, dim, like=None, dtype=None):
         want = dtype if dtype is not None else (like.dtype if like is not None else t.dtype)
         index = t.get_device()
         if (t.dtype is want and (like is not None or want in _DTYPES) and index >= 0 and (like is None or index == like.get_device())
-                and t.dim() == dim and (t.stride(-1) == 1 or t.shape[-1] <= 1)):
+                and t.dim() == dim and (t.stride(-1) == 1 or t.shape[-1] <= 1) and not t.is_neg()):
             return
     except (AttributeError, IndexError):
         pass
@@ -46,6 +47,8 @@ def _check_tensor(t, name, dim, like=None, dtype=None):
         raise ValueError(f"{name} is {t.dtype}, expected {want}")
     if t.dim() != dim:
         raise ValueError(f"{name} must have {dim} dimension{'s' if dim > 1 else ''} (got {t.dim()})")
+    if t.is_neg():
+        raise ValueError(f"{name} is a negation that is not carried out yet (pass {name}.resolve_neg())")
     raise ValueError(f"{name} must have unit stride in its last dimension")
 
 
@@ -93,9 +96,9 @@ def _check_layer(x, weight, name, bias, bias_name):
         dtype, index = x.dtype, x.get_device()
         n, k = weight.shape
         if (weight.dtype is dtype and weight.get_device() == index and k == x.shape[1] and n > 0 and k > 0
-                and (weight.stride(1) == 1 or k == 1)
+                and (weight.stride(1) == 1 or k == 1) and not weight.is_neg()
                 and (bias is None or (bias.dtype is dtype and bias.get_device() == index and bias.shape == (n,)
-                                      and (bias.stride(0) == 1 or n == 1)))):
+                                      and (bias.stride(0) == 1 or n == 1) and not bias.is_neg()))):
             return
     except (AttributeError, ValueError, IndexError):
         pass
@@ -191,7 +194,7 @@ class _Linear(torch.autograd.Function):
         need = ctx.needs_input_grad
         dx = dw = db = None
         if any(need[:3]):
-            g = dy if dy.shape[1] <= 1 or dy.stride(1) == 1 else dy.contiguous()
+            g = (dy if dy.shape[1] <= 1 or dy.stride(1) == 1 else dy.contiguous()).resolve_neg()
             dx, dw, db = _linear_backward(g, x, weight, z, ACTIVATIONS[ctx.activation], need)
         return dx, dw, db, dy if need[3] else None, None
 
@@ -280,7 +283,7 @@ class _Gated(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
         x, weight_gate, weight_up, gu = ctx.saved_tensors
-        g = dh if dh.shape[1] <= 1 or dh.stride(1) == 1 else dh.contiguous()
+        g = (dh if dh.shape[1] <= 1 or dh.stride(1) == 1 else dh.contiguous()).resolve_neg()
         return (*_gated_backward(g, x, weight_gate, weight_up, gu, ACTIVATIONS[ctx.activation], ctx.needs_input_grad), None)
 
 
@@ -350,7 +353,7 @@ class _Distillation(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, weight):
         logits, teacher_logits, teacher_index, stats = ctx.saved_tensors
-        weight, grad = weight.contiguous(), logits.new_empty(logits.shape)
+        weight, grad = weight.contiguous().resolve_neg(), logits.new_empty(logits.shape)
         _enqueue(lib.v2vae_distill_bwd, "v2vae_distill_bwd", logits, ctx.d, _p(logits), _p(teacher_logits), _p(teacher_index), _p(stats),
                  _p(weight), _p(grad))
         return grad, None, None, None
@@ -372,7 +375,8 @@ def topk_distillation(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
         p = softmax(teacher / T),  q = softmax(logits / T),  loss = T^2 sum_j p_j (log p_j - log q[index_j])
 
     An entry with index < 0 or a teacher logit of -inf is absent; a row without present entries has loss and gradient 0; a class
-    that a row names twice counts twice.  An index >= V makes the row NaN.  Differentiable in `logits`; the teacher is not."""
+    that a row names twice counts twice.  An index >= V makes the row NaN.  Differentiable in `logits`; the teacher is not.  Rows
+    of the three matrices may lie any distance apart, but may not overlap."""
     if isinstance(teacher_logits, torch.Tensor) and teacher_logits.requires_grad and torch.is_grad_enabled():
         raise ValueError("teacher_logits: the loss is not differentiable in the teacher (pass teacher_logits.detach())")
     if isinstance(logits, torch.Tensor) and _grads_wanted(logits):
