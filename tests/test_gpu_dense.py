@@ -488,3 +488,24 @@ def test_refusals():
         gated_backward(h, x, w, w, gu[:, :5])
     with pytest.raises(ValueError, match="dh: expected"):
         gated_backward(h[:, :3], x, w, w, gu)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16", "f16"])
+def test_every_choice_of_gradients_gives_the_same_ones(dtype):
+    from volterra_vae_amd.dense_ops import gated_backward, gated_forward, linear_backward, linear_forward
+    x, w, b, r, dy = linear_case(70, 33, 45, dtype, "silu", True, True, "odd", 3)
+    _, z = linear_forward(x, w, b, activation="silu", keep=True)
+    full = linear_backward(dy, x, w, z, activation="silu")
+    plain = linear_backward(dy, x, w)
+    for i in range(8):
+        need = [bool(i >> q & 1) for q in range(3)]
+        for every, some in ((full, linear_backward(dy, x, w, z, activation="silu", need=need)), (plain, linear_backward(dy, x, w, need=need))):
+            for n, p, q in zip(need, every, some):
+                assert torch.equal(p, q) if n else q is None
+    x, wg, wu, bg, bu, dh = gated_case(70, 33, 45, dtype, True, "odd", 3)
+    _, gu = gated_forward(x, wg, wu, bg, bu, keep=True)
+    full = gated_backward(dh, x, wg, wu, gu)
+    for i in range(32):
+        need = [bool(i >> q & 1) for q in range(5)]
+        for n, p, q in zip(need, full, gated_backward(dh, x, wg, wu, gu, need=need)):
+            assert torch.equal(p, q) if n else q is None

@@ -270,3 +270,14 @@ def test_refusals():
     for bad in (w[:5], w.double(), torch.ones(1, device=dev()).expand(6)):
         with pytest.raises(ValueError, match="row_weight"):
             topk_distillation_step(z, t, i, bad)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16", "f16"])
+def test_every_number_of_entries_beside_every_length_of_rows(dtype):
+    """More entries than a short row's lanes, as many, fewer; classes named twice."""
+    for v in (9, 33, 70, 130, 260, 600, 1500, 5000):
+        for k in (1, 8, 9, 16, 17, 32, 33, 64, 65, 200):
+            z, t, idx, w = case(7, v, min(k, v), dtype, v + k)
+            if k > 3:
+                idx[::2, 2] = idx[::2, 0]
+            check(z, t, idx, w, 1.3)

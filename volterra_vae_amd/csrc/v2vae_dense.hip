@@ -17,12 +17,11 @@ struct SlopeArgs {
     int64_t ld_d;
     float* part[2];     // [chunks][N] (NULL: no sums)
     int64_t M, rows_per_chunk;
-    int N, cx;          // cx threads along the columns, 256 / cx along the rows
+    int N, cx;          // cx threads along the columns, four each, 256 / cx along the rows
 };
 
-template <typename T, int V, int ACT, bool GATED> __global__ __launch_bounds__(256) void k_dense_slopes(SlopeArgs a) {
-    struct alignas(V * sizeof(T)) TV { T e[V]; };
-    struct alignas(V * 4) FV { float e[V]; };
+template <typename T, int ACT, bool GATED> __global__ __launch_bounds__(256) void k_dense_slopes(SlopeArgs a) {
+    constexpr int V = 4;  // columns a thread
     __shared__ float s_sum[GATED ? 2 : 1][256 * V];
     const int tid = threadIdx.x, cx = a.cx, ry = 256 / cx, tx = tid % cx, ty = tid / cx;
     const int64_t n = ((int64_t)blockIdx.x * cx + tx) * V;
@@ -30,47 +29,36 @@ template <typename T, int V, int ACT, bool GATED> __global__ __launch_bounds__(2
     float s0[V], s1[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) s0[v] = s1[v] = 0.f;
-    if (n >= a.N && n < a.ld_d && a.d[0]) {  // V = 1: the padding (V = 4: N is a multiple of 4, and so is what is left)
-        for (int64_t m = lo + ty; m < hi; m += ry)
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                ((T*)a.d[0])[m * a.ld_d + n + v] = (T)0.f;
-                if constexpr (GATED) ((T*)a.d[1])[m * a.ld_d + n + v] = (T)0.f;
-            }
-    }
-    if (n < a.N) {
+    // WHOLE: all V columns exist; else those beyond N are zeros, and stored where dz has columns for them
+    auto rows = [&](auto all) {
+        constexpr bool WHOLE = decltype(all)::value;
+        const int count = (int)(a.N - n), out = (int)(a.ld_d - n);
 #pragma unroll 2
         for (int64_t m = lo + ty; m < hi; m += ry) {
-            const TV dy = *reinterpret_cast<const TV*>((const T*)a.dy + m * a.ld_dy + n);
-            TV o0, o1;
-            if constexpr (GATED) {
-                const FV gate = *reinterpret_cast<const FV*>(a.z[0] + m * a.N + n), up = *reinterpret_cast<const FV*>(a.z[1] + m * a.N + n);
+            float dy[V], z0[V], z1[V];
+            load_columns<T, V>(a.dy, m * a.ld_dy + n, count, WHOLE, dy);
+            if (a.z[0]) load_columns<float, V>(a.z[0], m * a.N + n, count, WHOLE, z0);
+            if constexpr (GATED) load_columns<float, V>(a.z[1], m * a.N + n, count, WHOLE, z1);
 #pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    float val;
-                    const float slope = act_slope(ACT, gate.e[v], &val), d = (float)dy.e[v];
-                    const float dg = d * up.e[v] * slope, du = d * val;
-                    s0[v] += dg;
-                    s1[v] += du;
-                    o0.e[v] = (T)dg;
-                    o1.e[v] = (T)du;
+            for (int v = 0; v < V; ++v) {
+                float val;
+                if constexpr (GATED) {
+                    const float slope = act_slope(ACT, z0[v], &val), d = dy[v];
+                    dy[v] = d * z1[v] * slope;
+                    z1[v] = d * val;
+                    s1[v] += z1[v];
+                } else {
+                    if (a.z[0]) dy[v] *= act_slope(ACT, z0[v], &val);
                 }
-                *reinterpret_cast<TV*>((T*)a.d[0] + m * a.ld_d + n) = o0;
-                *reinterpret_cast<TV*>((T*)a.d[1] + m * a.ld_d + n) = o1;
-            } else {
-                FV z;
-                if (a.z[0]) z = *reinterpret_cast<const FV*>(a.z[0] + m * a.N + n);
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    float val, d = (float)dy.e[v];
-                    if (a.z[0]) d *= act_slope(ACT, z.e[v], &val);
-                    s0[v] += d;
-                    o0.e[v] = (T)d;
-                }
-                if (a.d[0]) *reinterpret_cast<TV*>((T*)a.d[0] + m * a.ld_d + n) = o0;
+                s0[v] += dy[v];
             }
+            if (a.d[0]) store_columns<T, V>(a.d[0], m * a.ld_d + n, out, WHOLE, dy);
+            if constexpr (GATED)
+                if (a.d[1]) store_columns<T, V>(a.d[1], m * a.ld_d + n, out, WHOLE, z1);
         }
-    }
+    };
+    if (n + V <= a.N) rows(std::true_type());
+    else if (n < a.ld_d) rows(std::false_type());
     if (a.part[0] == nullptr) return;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -159,6 +147,7 @@ static int check_dense(const v2vae_dense* d, bool gated, bool backward, bool res
 
 constexpr double PACK_FORWARD = 4e9, PACK_BACKWARD = 3e8;  // rows x in x out from which copies pay
 
+constexpr int64_t STEPS_256 = 8;
 // How a product M x N x K is cut: tile size and the number of parts of the contraction.  `direct`: 16-bit operands, aligned.
 // The workspace does not know the alignment, so it is laid out for the larger of the two cuts.
 struct Cut { int tile, splits, per; };
@@ -193,7 +182,10 @@ static Cut cut_product(int64_t M, int64_t N, int64_t K, int segs, int batch, int
                 tiles = rows * across;
             }
         }
-    } else if (direct && tiles_of(256) >= 128 && full(tiles_of(256), 256) >= 0.88 * full(tiles_of(128), 512)) {
+    } else if (direct && N * (gated ? 2 : 1) <= 64) {  // 128 x 64: one column of tiles, more of them on a compute unit
+        c.tile = TILE_64;
+        tiles = ((M + 127) / 128) * batch;
+    } else if (direct && steps >= STEPS_256 && tiles_of(256) >= 128 && full(tiles_of(256), 256) >= 0.88 * full(tiles_of(128), 512)) {
         c.tile = TILE_256;
         tiles = tiles_of(256);
     } else if (tiles_of(128) >= 256 || tiles_of(128) * (steps / 8) >= 256 || direct) {
@@ -243,8 +235,8 @@ static Planes planes_of(const v2vae_dense* d, bool gated, bool transposed) {
     return p;
 }
 
-static void slope_shape(int64_t M, int64_t N, int V, int* cx, int* gx, int* chunks) {
-    const int64_t cols = (N + V - 1) / V;
+static void slope_shape(int64_t M, int64_t N, int* cx, int* gx, int* chunks) {
+    const int64_t cols = (N + 3) / 4;
     int c = 1;
     while (c < cols && c < 64) c *= 2;
     *cx = c;
@@ -295,13 +287,11 @@ static BwdLayout bwd_layout(const v2vae_dense* d, bool gated) {
         l.dz[i] = o;
         if (i < n && (gated || d->activation != V2VAE_ACT_NONE || p.dz)) o += round_up((size_t)d->rows * p.ld_out * elem_bytes(d->dtype));
     }
-    int cx, gx, c1, c4;
+    int cx, gx, chunks;
     size_t most = 1;
     for (int64_t width : {d->out, (int64_t)p.ld_out}) {
-        slope_shape(d->rows, width, 1, &cx, &gx, &c1);
-        slope_shape(d->rows, width, 4, &cx, &gx, &c4);
-        if ((size_t)c1 > most) most = c1;
-        if ((size_t)c4 > most) most = c4;
+        slope_shape(d->rows, width, &cx, &gx, &chunks);
+        if ((size_t)chunks > most) most = chunks;
     }
     for (int i = 0; i < 2; ++i) {
         l.part[i] = o;
@@ -322,7 +312,7 @@ static BwdLayout bwd_layout(const v2vae_dense* d, bool gated) {
 
 static int run_product(GemmArgs& g, int dtype, int layout, bool gated, float* partial, hipStream_t st) {
     if (g.M == 0 || g.N == 0) return V2VAE_OK;
-    const int e = 16 / elem_bytes(dtype), bytes = elem_bytes(dtype);
+    const int e = 16 / elem_bytes(dtype);
     auto aligned_rows = [&](const void* const p[2], int64_t ld0, int64_t ld1) {
         return aligned_to(p[0], 16) && (p[1] == nullptr || aligned_to(p[1], 16)) && ld0 % e == 0 && ld1 % e == 0;
     };
@@ -330,9 +320,6 @@ static int run_product(GemmArgs& g, int dtype, int layout, bool gated, float* pa
     // every row whole 16-byte pieces, in memory and in the part of it that counts (or zeros behind that)
     const bool whole_a = aligned_rows(g.a, g.lda, g.lda) && (g.pad_a || (a_kc ? g.K : g.M) % e == 0);
     const bool whole_b = aligned_rows(g.b, g.ldb[0], g.ldb[1]) && (g.pad_b || (b_kc ? g.K : g.N) % e == 0);
-    auto fit = [&](const void* p, int64_t ld) { return aligned_to(p, 16) && (p == nullptr || ld % e == 0); };
-    g.vec_c = g.N % 8 == 0 && fit(g.c[0], g.ldc) && fit(g.c[1], g.ldc) && fit(g.bias[0], 0) && fit(g.bias[1], 0) && fit(g.residual, g.ldr) &&
-              fit(g.z[0], 0) && fit(g.z[1], 0);
     // straight to LDS: 16-bit, whole pieces, offsets inside a tile below 2^31, one stride
     const int64_t ld_max = g.lda > g.ldb[0] ? (g.lda > g.ldb[1] ? g.lda : g.ldb[1]) : (g.ldb[0] > g.ldb[1] ? g.ldb[0] : g.ldb[1]);
     const bool direct = dtype != V2VAE_F32 && whole_a && whole_b && ld_max <= (1 << 21) && (gated || g.ldb[0] == g.ldb[1]);
@@ -435,22 +422,15 @@ static int backward(const v2vae_dense* d, const void* x, const void* w0, const v
             s.part[0] = (float*)(base + l.part[0]);
             s.part[1] = gated ? (float*)(base + l.part[1]) : nullptr;
         }
-        const int bytes = elem_bytes(d->dtype);
-        const bool v4 = d->out % 4 == 0 && d->ld_dy % 4 == 0 && aligned_to(dy, 4 * bytes) && (!act || aligned_to(z, 16));
         int gx, chunks;
-        slope_shape(M, s.ld_d, v4 ? 4 : 1, &s.cx, &gx, &chunks);
+        slope_shape(M, s.ld_d, &s.cx, &gx, &chunks);
         s.rows_per_chunk = (M + chunks - 1) / chunks;
         const dim3 grid(gx, chunks);
         auto slopes = [&](auto t, auto kind) {
             typedef decltype(t) T;
             constexpr int ACT = decltype(kind)::value;
-            if (gated) {
-                if (v4) hipLaunchKernelGGL((k_dense_slopes<T, 4, ACT, true>), grid, dim3(256), 0, st, s);
-                else hipLaunchKernelGGL((k_dense_slopes<T, 1, ACT, true>), grid, dim3(256), 0, st, s);
-            } else {
-                if (v4) hipLaunchKernelGGL((k_dense_slopes<T, 4, ACT, false>), grid, dim3(256), 0, st, s);
-                else hipLaunchKernelGGL((k_dense_slopes<T, 1, ACT, false>), grid, dim3(256), 0, st, s);
-            }
+            if (gated) hipLaunchKernelGGL((k_dense_slopes<T, ACT, true>), grid, dim3(256), 0, st, s);
+            else hipLaunchKernelGGL((k_dense_slopes<T, ACT, false>), grid, dim3(256), 0, st, s);
         };
         auto go = [&](auto t) {
             typedef decltype(t) T;

@@ -268,6 +268,7 @@ template <typename T, int WM, int WN, int TM, int TN, bool AKC, bool BKC, bool G
 }
 template <typename T, bool AKC, bool BKC, bool GATED> void pick_direct(const GemmArgs& g, int tile, hipStream_t st) {
     if (tile == TILE_256) launch_direct<T, 2, 4, 4, 2, AKC, BKC, GATED>(g, st);
+    else if (tile == TILE_64) launch_direct<T, 4, 1, 1, 2, AKC, BKC, GATED>(g, st);
     else launch_direct<T, 2, 2, 2, 2, AKC, BKC, GATED>(g, st);
 }
 template <typename T> int gemm_direct(const GemmArgs& g, int layout, bool gated, int tile, hipStream_t st) {

@@ -102,13 +102,13 @@ __device__ __forceinline__ void finish_block(const GemmArgs& g, const f32x16 (&a
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     const int c = (lane % PER) * 8, n = n0 + c;
-    const bool whole = g.vec_c;  // N is a multiple of 8 then
+    const bool whole = n + 8 <= g.N;
     // the residual of a row is asked for while the row before it is finished
-    struct alignas(8 * sizeof(T) > 16 ? 16 : 8 * sizeof(T)) T8 { T e[8]; };
+    typedef Columns<T, 8> T8;
     const bool fetched = !GATED && !part && g.residual && whole;
     auto residual_at = [&](int r) {
         const int64_t m = m0 + r < g.M ? m0 + r : g.M - 1;
-        return *reinterpret_cast<const T8*>((const T*)g.residual + m * g.ldr + (n < g.N ? n : 0));
+        return *reinterpret_cast<const T8*>((const T*)g.residual + m * g.ldr + n);
     };
     T8 next;
     if (fetched) next = residual_at(lane / PER);
@@ -229,38 +229,64 @@ __global__ __launch_bounds__(256, 2) void k_gemm_staged(GemmArgs g) {
         finish_block<T, TN, GATED>(g, acc[i], lds + wave * EPI_BYTES<TN>, lane, m0 + (wm * TM + i) * 32, n0 + wn * (GATED ? 32 : 32 * TN), part, bat);
 }
 
-// Sums of a split contraction, added in the order of the splits, and the rest of the epilogue; C columns a thread.
-template <typename T, int C, bool GATED> __global__ __launch_bounds__(256) void k_gemm_join(GemmArgs g) {
-    const int64_t per = (int64_t)g.M * g.N * (GATED ? 2 : 1), count = (int64_t)g.M * (g.N / C);
-    const int bat = blockIdx.y;
+// Sums of a split contraction and the rest of the epilogue; C columns a thread.  Y threads share an output's parts, thread y those
+// from y on in steps of Y, and their sums are added in order.
+template <typename T, int C, int Y, bool GATED> __global__ __launch_bounds__(256) void k_gemm_join(GemmArgs g) {
+    constexpr int X = 256 / Y, W = GATED ? 2 : 1;
+    __shared__ float s_part[Y > 1 ? Y : 1][Y > 1 ? X : 1][Y > 1 ? W * C : 1];
+    const int64_t per = (int64_t)g.M * g.N * W, count = (int64_t)g.M * (g.N / C);
+    const int bat = blockIdx.y, x = threadIdx.x % X, y = threadIdx.x / X;
     const float* base = g.partial + bat * (int64_t)g.splits * per;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
-        const int64_t m = i / (g.N / C);
+    for (int64_t i0 = (int64_t)blockIdx.x * X; i0 < count; i0 += (int64_t)gridDim.x * X) {
+        const int64_t i = i0 + x < count ? i0 + x : count - 1, m = i / (g.N / C);
         const int n = (int)(i - m * (g.N / C)) * C;
         float s[C], u[C], v[C];
 #pragma unroll
         for (int e = 0; e < C; ++e) s[e] = u[e] = 0.f;
 #pragma unroll 4
-        for (int p = 0; p < g.splits; ++p) {
-            load_columns<float, C>(base, p * per + m * (GATED ? 2 : 1) * g.N + n, C, true, v);
+        for (int p = y; p < g.splits; p += Y) {
+            load_columns<float, C>(base, p * per + m * W * g.N + n, C, true, v);
 #pragma unroll
             for (int e = 0; e < C; ++e) s[e] += v[e];
             if constexpr (GATED) {
-                load_columns<float, C>(base, p * per + m * 2 * g.N + g.N + n, C, true, v);
+                load_columns<float, C>(base, p * per + m * W * g.N + g.N + n, C, true, v);
 #pragma unroll
                 for (int e = 0; e < C; ++e) u[e] += v[e];
             }
         }
+        if constexpr (Y > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < C; ++e) {
+                s_part[y][x][e] = s[e];
+                if constexpr (GATED) s_part[y][x][C + e] = u[e];
+            }
+            __syncthreads();
+            if (y > 0) continue;
+            for (int q = 1; q < Y; ++q)
+#pragma unroll
+                for (int e = 0; e < C; ++e) {
+                    s[e] += s_part[q][x][e];
+                    if constexpr (GATED) u[e] += s_part[q][x][C + e];
+                }
+        }
+        if (i0 + x >= count) continue;
         if constexpr (GATED) finish_gated<T, C>(g, m, n, s, u, true); else finish_value<T, C>(g, m, n, s, bat, true);
     }
 }
 
 template <typename T, bool GATED> void launch_join(const GemmArgs& g, hipStream_t st) {
-    const int c = g.vec_c ? 4 : 1;
-    int64_t blocks = ((int64_t)g.M * (g.N / c) + 255) / 256;
+    const int c = g.N % 4 == 0 ? 4 : 1;
+    const int64_t count = (int64_t)g.M * (g.N / c);
+    // many parts of few outputs (96 x 28 of 431 parts: JOIN_1 us with one thread an output, JOIN_16 with sixteen)
+    const bool shared = g.splits >= 32 && count < 65536;
+    int64_t blocks = shared ? (count + 15) / 16 : (count + 255) / 256;
     if (blocks > 4096) blocks = 4096;
-    if (c == 4) hipLaunchKernelGGL((k_gemm_join<T, 4, GATED>), dim3((unsigned)blocks, g.batch), dim3(256), 0, st, g);
-    else hipLaunchKernelGGL((k_gemm_join<T, 1, GATED>), dim3((unsigned)blocks, g.batch), dim3(256), 0, st, g);
+    const dim3 grid((unsigned)blocks, g.batch);
+    if (shared && c == 4) hipLaunchKernelGGL((k_gemm_join<T, 4, 16, GATED>), grid, dim3(256), 0, st, g);
+    else if (shared) hipLaunchKernelGGL((k_gemm_join<T, 1, 16, GATED>), grid, dim3(256), 0, st, g);
+    else if (c == 4) hipLaunchKernelGGL((k_gemm_join<T, 4, 1, GATED>), grid, dim3(256), 0, st, g);
+    else hipLaunchKernelGGL((k_gemm_join<T, 1, 1, GATED>), grid, dim3(256), 0, st, g);
 }
 
 template <typename T, int TM, int TN, bool AKC, bool BKC, bool GATED> void launch_staged(const GemmArgs& g, hipStream_t st) {

@@ -76,15 +76,17 @@ __device__ __forceinline__ float exp_diff(float z, float m, float c) { return __
 
 // G lanes a row, NV 16-byte pieces of the row held by each lane (HELD), or the row read once per pass.  MODE: DO_LOSS | DO_GRAD.
 // A DO_GRAD pass alone takes maximum and sum from `stats`.  ONE: the teacher's entries fit the lanes of one wave (k <= G and
-// k <= 64): each of them keeps one, and everything about them happens there while the row is on its way.
+// k <= 64): each of them keeps one, and everything about them happens there while the row is on its way.  Else they are dealt out
+// to the threads of the workgroup, their classes and probabilities in LDS for the merging of what names one class twice.
 template <typename T, int G, int NV, bool HELD, int MODE, bool ONE>
 __global__ __launch_bounds__(G > 64 ? G : 256) void k_distill(DistillArgs a) {
     constexpr int E = Vec16<T>::N, ROWS = G > 64 ? 1 : 256 / G, GE = G > 64 ? 64 : G;
-    constexpr bool STATS_GIVEN = MODE == DO_GRAD, LISTS = G > 64 && !ONE;
+    constexpr bool STATS_GIVEN = MODE == DO_GRAD;
+    static_assert(ONE || G > 64, "lists need a workgroup");
     __shared__ float s_red[G > 64 ? 5 * (G / 64) : 1];
     __shared__ int s_state;
-    __shared__ float s_p[LISTS ? V2VAE_DISTILL_MAX_K : 1];
-    __shared__ int s_c[LISTS ? V2VAE_DISTILL_MAX_K : 1];
+    __shared__ float s_p[ONE ? 1 : V2VAE_DISTILL_MAX_K];
+    __shared__ int s_c[ONE ? 1 : V2VAE_DISTILL_MAX_K];
     const Lanes<G> lanes{s_red};
     const Lanes<GE> wave{nullptr};
     const int tid = G > 64 ? threadIdx.x : threadIdx.x % G;
@@ -284,7 +286,7 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void k_distill(DistillArgs a) {
                 put(i, ev);
             }
         }
-        if constexpr (LISTS) {
+        if constexpr (!ONE) {
             for (int j = tid; j < a.k; j += G) {
                 s_c[j] = class_at(a, row, j);
                 s_p[j] = entry_p(j, s_c[j]);
@@ -295,13 +297,13 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void k_distill(DistillArgs a) {
             if (my_cls >= 0 && state == SOME && first) out[my_cls] = (T)(wt * (exp_diff(my_z, zm, c) * inv_l - p_all));
         } else {
             for (int j = tid; j < a.k; j += G) {
-                const int cls = LISTS ? s_c[j] : class_at(a, row, j);
+                const int cls = s_c[j];
                 if (cls < 0 || state != SOME) continue;
                 float p = 0.f;
                 bool one = true;
                 for (int i = 0; i < a.k; ++i) {
-                    if ((LISTS ? s_c[i] : class_at(a, row, i)) == cls) {
-                        p += LISTS ? s_p[i] : entry_p(i, cls);
+                    if (s_c[i] == cls) {
+                        p += s_p[i];
                         one &= i >= j;
                     }
                 }
@@ -322,19 +324,27 @@ template <typename T, int G, int NV, bool HELD, bool ONE> static int go_mode(con
     return dense_launch_error("distillation");
 }
 template <typename T, int G, int NV, bool HELD> static int go(const DistillArgs& a, int mode, hipStream_t st) {
-    return a.k <= (G > 64 ? 64 : G) ? go_mode<T, G, NV, HELD, true>(a, mode, st) : go_mode<T, G, NV, HELD, false>(a, mode, st);
+    if constexpr (G > 64) {
+        if (a.k > 64) return go_mode<T, G, NV, HELD, false>(a, mode, st);
+    }
+    return go_mode<T, G, NV, HELD, true>(a, mode, st);
 }
 
+// The group that holds a row has a lane for every teacher entry, up to 64 of them; more are the workgroup's, which keeps them in
+// LDS.  (Entries without a lane or LDS of their own, read again for every other one, took 98 us for 2 rows of 96 logits with 90
+// entries and 54 for 6984 rows of 65 with 50; DIST_A and DIST_B this way.)
 template <typename T> static int distill(const DistillArgs& a, int mode, hipStream_t st) {
     constexpr int E = Vec16<T>::N;
     // pieces of a row: V / E if every row starts at one, else of a row that starts anywhere
     const bool aligned = ((uintptr_t)a.z & 15) == 0 && (a.ld_z % E == 0 || a.rows == 1);
     const int64_t pieces = aligned ? (a.V + E - 1) / E : (a.V + 2 * E - 2) / E;
-    if (pieces <= 8) return go<T, 8, 1, true>(a, mode, st);
-    if (pieces <= 16) return go<T, 16, 1, true>(a, mode, st);
-    if (pieces <= 32) return go<T, 16, 2, true>(a, mode, st);
-    if (pieces <= 64) return go<T, 32, 2, true>(a, mode, st);
-    if (pieces <= 256) return go<T, 64, 4, true>(a, mode, st);
+    if (pieces <= 8 && a.k <= 8) return go<T, 8, 1, true>(a, mode, st);
+    if (pieces <= 16 && a.k <= 16) return go<T, 16, 1, true>(a, mode, st);
+    if (pieces <= 32 && a.k <= 16) return go<T, 16, 2, true>(a, mode, st);
+    if (pieces <= 64 && a.k <= 32) return go<T, 32, 2, true>(a, mode, st);
+    if (pieces <= 64 && a.k <= 64) return go<T, 64, 1, true>(a, mode, st);
+    if (pieces <= 256 && a.k <= 64) return go<T, 64, 4, true>(a, mode, st);
+    if (pieces <= 256) return go<T, 256, 1, true>(a, mode, st);
     if (pieces <= 1024) return go<T, 256, 4, true>(a, mode, st);
     if (pieces <= 2048) return go<T, 256, 8, true>(a, mode, st);
     if (pieces <= 4096) return go<T, 512, 8, true>(a, mode, st);
