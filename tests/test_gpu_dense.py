@@ -509,3 +509,30 @@ def test_every_choice_of_gradients_gives_the_same_ones(dtype):
         need = [bool(i >> q & 1) for q in range(5)]
         for n, p, q in zip(need, full, gated_backward(dh, x, wg, wu, gu, need=need)):
             assert torch.equal(p, q) if n else q is None
+
+
+def test_few_float32_rows_of_long_and_few_weights():
+    """The contraction in parts: every number of parts that the rule gives, with and without a rest."""
+    from volterra_vae_amd.dense_ops import gated_forward, linear_forward
+    for m, k, n in ((1, 3200, 16), (9, 8165, 504), (13, 6696, 876), (32, 4096, 33), (17, 20500, 5), (3, 40000, 100), (5, 22401, 9), (2, 3199, 700)):
+        x, w, b, r, dy = linear_case(m, k, n, torch.float32, "silu", True, True, "odd", m + k)
+        y, z = linear_forward(x, w, b, residual=r, activation="silu", keep=True)
+        check_linear(x, w, b, r, dy, "silu", y, None, torch.float32)
+        near(z, x.double() @ w.double().t() + b.double(), 8 * EPS32 * steps(k, torch.float32) ** 0.5 * s2(x.double(), w.double())
+             + 16 * EPS32 * b.double().abs() + 1e-30, "z")
+        x, wg, wu, bg, bu, dh = gated_case(m, k, n, torch.float32, True, "odd", m + k)
+        h, gu = gated_forward(x, wg, wu, bg, bu, keep=True)
+        check_gated(x, wg, wu, bg, bu, dh, "silu", h, None, torch.float32)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16", "f16"])
+def test_narrow_layers_of_many_rows(dtype):
+    """Few inputs, few outputs or both, at aligned and at odd widths, each with its gradients."""
+    from volterra_vae_amd.dense_ops import gated_backward, gated_forward, linear_backward, linear_forward
+    for m, k, n in ((5000, 40, 24), (3001, 64, 64), (20001, 25, 603), (20001, 603, 25), (9001, 9, 33), (4097, 200, 8), (2500, 8, 1000)):
+        x, w, b, r, dy = linear_case(m, k, n, dtype, "silu", True, True, "odd" if k % 2 else "plain", k + n)
+        y, z = linear_forward(x, w, b, residual=r, activation="silu", keep=True)
+        check_linear(x, w, b, r, dy, "silu", y, linear_backward(dy, x, w, z, activation="silu"), dtype)
+        x, wg, wu, bg, bu, dh = gated_case(m, k, n, dtype, True, "odd" if k % 2 else "plain", k + n)
+        h, gu = gated_forward(x, wg, wu, bg, bu, keep=True)
+        check_gated(x, wg, wu, bg, bu, dh, "silu", h, gated_backward(dh, x, wg, wu, gu), dtype)

@@ -156,7 +156,7 @@ struct GemmArgs {
 
 // What happens to the finished sums of row m, columns n ... n + C - 1 (batch entry 1 has an output of its own, nothing else).
 // `whole`: all C columns exist; they are moved together at any address (11816 x 464 -> 2 x 572 bf16, whose rows start at odd
-// multiples of 8 bytes: 44 us with element by element moves there, EPI_NEW this way).
+// multiples of 8 bytes: 44 us with element by element moves there, 32 this way).
 template <typename T, int C> struct __attribute__((packed, aligned(sizeof(T)))) Columns { T e[C]; };
 template <typename T, int C> __device__ __forceinline__ void load_columns(const void* p, int64_t at, int count, bool whole, float v[C]) {
     if (whole) {
@@ -252,6 +252,7 @@ int gemm_staged_f16(const GemmArgs&, int layout, bool gated, int tile, hipStream
 
 // few rows (v2vae_dense_rows.hip); beyond, the tiled products read the weights as fast
 inline int64_t few_rows(int dtype) { return dtype == V2VAE_F32 ? 32 : 16; }
+int rows_splits(int dtype, int64_t in, int64_t out, bool gated);  // parts of the contraction
 int dense_rows(const GemmArgs& g, int dtype, bool gated, hipStream_t st);
 
 int dense_launch_error(const char* where);  // V2VAE_OK, or V2VAE_ELAUNCH with the text kept for v2vae_last_error

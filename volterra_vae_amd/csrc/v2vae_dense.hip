@@ -147,7 +147,6 @@ static int check_dense(const v2vae_dense* d, bool gated, bool backward, bool res
 
 constexpr double PACK_FORWARD = 4e9, PACK_BACKWARD = 3e8;  // rows x in x out from which copies pay
 
-constexpr int64_t STEPS_256 = 8;
 // How a product M x N x K is cut: tile size and the number of parts of the contraction.  `direct`: 16-bit operands, aligned.
 // The workspace does not know the alignment, so it is laid out for the larger of the two cuts.
 struct Cut { int tile, splits, per; };
@@ -185,7 +184,7 @@ static Cut cut_product(int64_t M, int64_t N, int64_t K, int segs, int batch, int
     } else if (direct && N * (gated ? 2 : 1) <= 64) {  // 128 x 64: one column of tiles, more of them on a compute unit
         c.tile = TILE_64;
         tiles = ((M + 127) / 128) * batch;
-    } else if (direct && steps >= STEPS_256 && tiles_of(256) >= 128 && full(tiles_of(256), 256) >= 0.88 * full(tiles_of(128), 512)) {
+    } else if (direct && tiles_of(256) >= 128 && full(tiles_of(256), 256) >= 0.88 * full(tiles_of(128), 512)) {
         c.tile = TILE_256;
         tiles = tiles_of(256);
     } else if (tiles_of(128) >= 256 || tiles_of(128) * (steps / 8) >= 256 || direct) {
@@ -216,6 +215,11 @@ static size_t partial_bytes(int64_t M, int64_t N, int64_t K, int segs, int batch
         if (c.splits > most) most = c.splits;
     }
     return most > 1 ? round_up((size_t)most * batch * M * N * (gated ? 2 : 1) * 4) : 0;
+}
+
+static size_t rows_bytes(const v2vae_dense* d, bool gated) {
+    const int s = rows_splits(d->dtype, d->in, d->out, gated);
+    return s > 1 ? round_up((size_t)s * d->rows * d->out * (gated ? 2 : 1) * 4) : 0;
 }
 
 // float32: planes of split weights, for a forward (plane rows = weight rows) or a dx product (plane rows = weight columns).
@@ -250,13 +254,14 @@ static void slope_shape(int64_t M, int64_t N, int* cx, int* gx, int* chunks) {
 
 // 16-bit operands whose rows are not whole 16-byte pieces: copied when the products are large enough to win the copies back.
 // Measured in bf16, forward and gradients, us without / with copies: 4001 x 2047 x 2043 86 / 63 and 518 / 138, 2000 x 101 x 3999 80 / 65 backward,
-// 65537 x 131 x 257 55 / 67 forward (therefore without) and 186 / 129 backward, 1001 x 515 x 1027 60 / 57 backward.
+// 65537 x 131 x 257 55 / 67 forward (therefore without) and 186 / 129 backward, 1001 x 515 x 1027 60 / 57 backward.  Rows of a few
+// elements: 165488 x 28 x 96 36 / 70 forward (therefore without) and 97 / 66 backward, 141724 x 25 -> 2 x 161 287 / 178 backward.
 struct Packs { bool x, w, dz; size_t x_bytes, w_bytes; int ld_in, ld_out; };
 static Packs packs_of(const v2vae_dense* d, bool gated, bool backward) {
     Packs p = {};
     p.ld_in = (int)((d->in + 7) / 8 * 8);
     p.ld_out = (int)d->out;
-    if (d->dtype == V2VAE_F32 || d->rows <= few_rows(d->dtype) || d->in < 32 || d->out < 32) return p;
+    if (d->dtype == V2VAE_F32 || d->rows <= few_rows(d->dtype) || (!backward && (d->in < 32 || d->out < 32))) return p;
     if ((double)d->rows * d->in * d->out * (gated ? 2 : 1) < (backward ? PACK_BACKWARD : PACK_FORWARD)) return p;
     const bool odd = d->in % 8 != 0;
     p.x = odd || d->ld_x % 8 != 0;
@@ -369,7 +374,11 @@ static int forward(const v2vae_dense* d, const void* x, const void* w0, const vo
         const int rc = use_planes(g, p, false, gated, (char*)ws, st);
         if (rc != V2VAE_OK) return rc;
     }
-    if (d->rows <= few_rows(d->dtype)) return dense_rows(g, d->dtype, gated, st);
+    if (d->rows <= few_rows(d->dtype)) {
+        g.splits = rows_splits(d->dtype, d->in, d->out, gated);
+        g.partial = g.splits > 1 ? (float*)ws : nullptr;
+        return dense_rows(g, d->dtype, gated, st);
+    }
     const Packs k = packs_of(d, gated, false);
     char* at = (char*)ws + p.bytes;
     if (k.x) {
@@ -524,7 +533,7 @@ extern "C" {
 size_t v2vae_linear_workspace_bytes(const v2vae_dense* d, int backward) {
     if (check_dense(d, false, backward != 0, false) != V2VAE_OK) return 0;
     if (backward) return bwd_layout(d, false).total;
-    if (d->rows <= few_rows(d->dtype)) return 0;
+    if (d->rows <= few_rows(d->dtype)) return rows_bytes(d, false);
     const Packs k = packs_of(d, false, false);
     const size_t planes = planes_of(d, false, false).bytes;
     return planes + k.x_bytes + k.w_bytes + partial_bytes(d->rows, d->out, d->in, 1, 1, d->dtype, false, planes > 0);
@@ -533,7 +542,7 @@ size_t v2vae_linear_workspace_bytes(const v2vae_dense* d, int backward) {
 size_t v2vae_gated_workspace_bytes(const v2vae_dense* d, int backward) {
     if (check_dense(d, true, backward != 0, false) != V2VAE_OK) return 0;
     if (backward) return bwd_layout(d, true).total;
-    if (d->rows <= few_rows(d->dtype)) return 0;
+    if (d->rows <= few_rows(d->dtype)) return rows_bytes(d, true);
     const Packs k = packs_of(d, true, false);
     const size_t planes = planes_of(d, true, false).bytes;
     return planes + k.x_bytes + k.w_bytes + partial_bytes(d->rows, d->out, d->in, 1, 1, d->dtype, true, planes > 0);

@@ -92,6 +92,20 @@ template <int TN> constexpr int EPI_BYTES = 32 * EPI_ROWB<TN>;
 template <typename T, int TN, bool GATED>
 __device__ __forceinline__ void finish_block(const GemmArgs& g, const f32x16 (&acc)[TN], char* lds, int lane, int m0, int n0, float* part, int bat) {
     constexpr int ROWB = EPI_ROWB<TN>, COLS = GATED ? 32 : 32 * TN, PER = COLS / 8, ROWS = 64 / PER;
+    const int c = (lane % PER) * 8, n = n0 + c;
+    const bool whole = n + 8 <= g.N;
+    // the residual's rows are asked for before anything else
+    typedef Columns<T, 8> T8;
+    const bool fetched = !GATED && !part && g.residual && whole;
+    auto residual_at = [&](int r) {
+        const int64_t m = m0 + r < g.M ? m0 + r : g.M - 1;
+        return *reinterpret_cast<const T8*>((const T*)g.residual + m * g.ldr + n);
+    };
+    T8 next[32 / ROWS];
+    if (fetched) {
+#pragma unroll
+        for (int q = 0; q < 32 / ROWS; ++q) next[q] = residual_at(lane / PER + q * ROWS);
+    }
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int j = 0; j < TN; ++j)
@@ -101,22 +115,12 @@ __device__ __forceinline__ void finish_block(const GemmArgs& g, const f32x16 (&a
                 f32x4{acc[j][4 * q], acc[j][4 * q + 1], acc[j][4 * q + 2], acc[j][4 * q + 3]};
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    const int c = (lane % PER) * 8, n = n0 + c;
-    const bool whole = n + 8 <= g.N;
-    // the residual of a row is asked for while the row before it is finished
-    typedef Columns<T, 8> T8;
-    const bool fetched = !GATED && !part && g.residual && whole;
-    auto residual_at = [&](int r) {
-        const int64_t m = m0 + r < g.M ? m0 + r : g.M - 1;
-        return *reinterpret_cast<const T8*>((const T*)g.residual + m * g.ldr + n);
-    };
-    T8 next;
-    if (fetched) next = residual_at(lane / PER);
 #pragma unroll 1
     for (int r = lane / PER; r < 32; r += ROWS) {
         const int64_t m = m0 + r;
-        const T8 res = next;
-        if (fetched && r + ROWS < 32) next = residual_at(r + ROWS);
+        const T8 res = next[0];
+#pragma unroll
+        for (int q = 1; q < 32 / ROWS; ++q) next[q - 1] = next[q];
         if (m >= g.M || n >= g.N) continue;
         float s[8], u[8];
         const f32x4* p = reinterpret_cast<const f32x4*>(lds + r * ROWB + c * 4);
@@ -278,7 +282,7 @@ template <typename T, int C, int Y, bool GATED> __global__ __launch_bounds__(256
 template <typename T, bool GATED> void launch_join(const GemmArgs& g, hipStream_t st) {
     const int c = g.N % 4 == 0 ? 4 : 1;
     const int64_t count = (int64_t)g.M * (g.N / c);
-    // many parts of few outputs (96 x 28 of 431 parts: JOIN_1 us with one thread an output, JOIN_16 with sixteen)
+    // many parts of few outputs (96 x 28 of 431 parts: 40 us with one thread an output, 6 with sixteen)
     const bool shared = g.splits >= 32 && count < 65536;
     int64_t blocks = shared ? (count + 15) / 16 : (count + 255) / 256;
     if (blocks > 4096) blocks = 4096;

@@ -6,7 +6,7 @@
 // instruction sums over lanes, which costs a vector kernel six shuffles per output and wave.  The fragments come straight from
 // memory (16 bytes a lane, any alignment); float operands are split into three bf16 pieces in registers (six products).  The
 // waves' sums are joined through LDS in a fixed order.
-#include "v2vae_dense.h"
+#include "v2vae_dense_gemm.h"
 
 namespace v2vae {
 
@@ -104,33 +104,36 @@ template <typename T, int W, int MT, bool ODD, bool GATED> __global__ __launch_b
     };
     constexpr std::false_type inside{};
     constexpr std::true_type tail{};
-    const int whole = g.K / CE * CE;
+    const int whole = g.K / CE * CE, lo = blockIdx.y * g.steps_per_split * CE;
+    const bool last = blockIdx.y + 1 == gridDim.y;
+    const int hi = last || lo + g.steps_per_split * CE > whole ? whole : lo + g.steps_per_split * CE;
     // The weights of the next turn are asked for before this one's are multiplied.  The last turn asks for its own again (out of the
     // caches): without a branch the compiler knows what is in flight and waits for no more than it needs.
-    int k = wave * CE;
-    if (k < whole) {
-        auto after = [&](int at) { return at + W * CE < whole ? at + W * CE : at; };
+    int k = lo + wave * CE;
+    if (k < hi) {
+        auto after = [&](int at) { return at + W * CE < hi ? at + W * CE : at; };
         Turn w0 = load(w, k, inside), w1;
         for (;;) {
             const Turn x0 = load(x[0], k, inside);
             w1 = load(w, after(k), inside);
             multiply(w0, x0, k, inside);
             k += W * CE;
-            if (k >= whole) break;
+            if (k >= hi) break;
             const Turn x1 = load(x[0], k, inside);
             w0 = load(w, after(k), inside);
             multiply(w1, x1, k, inside);
             k += W * CE;
-            if (k >= whole) break;
+            if (k >= hi) break;
         }
     }
-    if (whole < g.K && (whole / CE) % W == wave) multiply(load(w, whole, tail), load(x[0], whole, tail), whole, tail);
+    if (last && whole < g.K && ((whole - lo) / CE) % W == wave) multiply(load(w, whole, tail), load(x[0], whole, tail), whole, tail);
     // lane: input row lane % 16, weight rows 4 (lane / 16) ... + 3
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s_sum[wave][16 * t + r][4 * (lane >> 4) + e] = acc[t][e];
     __syncthreads();
+    float* const part = g.partial ? g.partial + (int64_t)blockIdx.y * g.M * g.N * (GATED ? 2 : 1) : nullptr;
     for (int i = tid; i < 16 * MT * FT; i += 64 * W) {
         const int m = i / FT, f = i % FT;
         if (m >= g.M || n0 + f >= g.N) continue;
@@ -143,16 +146,36 @@ template <typename T, int W, int MT, bool ODD, bool GATED> __global__ __launch_b
         float s0 = total(f);
         if constexpr (GATED) {
             float s1 = total(f + 8);
+            if (part) {
+                part[(int64_t)m * 2 * g.N + n0 + f] = s0;
+                part[((int64_t)m * 2 + 1) * g.N + n0 + f] = s1;
+                continue;
+            }
             finish_gated<T, 1>(g, m, n0 + f, &s0, &s1, true);
         } else {
+            if (part) {
+                part[(int64_t)m * g.N + n0 + f] = s0;
+                continue;
+            }
             finish_value<T, 1>(g, m, n0 + f, &s0, 0, true);
         }
     }
 }
 
 template <typename T, int W, int MT, bool ODD> static void launch_waves(const GemmArgs& g, bool gated, hipStream_t st) {
-    if (gated) hipLaunchKernelGGL((k_dense_rows<T, W, MT, ODD, true>), dim3((g.N + 7) / 8), dim3(64 * W), 0, st, g);
-    else hipLaunchKernelGGL((k_dense_rows<T, W, MT, ODD, false>), dim3((g.N + 15) / 16), dim3(64 * W), 0, st, g);
+    if (gated) hipLaunchKernelGGL((k_dense_rows<T, W, MT, ODD, true>), dim3((g.N + 7) / 8, g.splits), dim3(64 * W), 0, st, g);
+    else hipLaunchKernelGGL((k_dense_rows<T, W, MT, ODD, false>), dim3((g.N + 15) / 16, g.splits), dim3(64 * W), 0, st, g);
+}
+// float on few, long weight rows: the contraction in parts, to a workgroup a compute unit (9 x 8165 -> 2 x 504: 25 us in one part,
+// 18 in four and their join).  16-bit rows, of half the bytes, end before a second launch would pay.
+int rows_splits(int dtype, int64_t in, int64_t out, bool gated) {
+    if (dtype != V2VAE_F32) return 1;
+    const int64_t groups = gated ? (out + 7) / 8 : (out + 15) / 16;
+    int64_t s = 256 / groups;
+    if (s > in / 1024) s = in / 1024;
+    if (s < 3) return 1;
+    const int64_t turns = in / 128, per = (turns + s - 1) / s;
+    return (int)((turns + per - 1) / per);  // none without a turn
 }
 template <typename T> static void launch_rows(const GemmArgs& g, bool gated, hipStream_t st) {
     // sixteen waves on a long contraction; float, which needs twice the registers a turn, eight
@@ -168,10 +191,15 @@ template <typename T> static void launch_rows(const GemmArgs& g, bool gated, hip
     }
 }
 
-int dense_rows(const GemmArgs& g, int dtype, bool gated, hipStream_t st) {
+int dense_rows(const GemmArgs& args, int dtype, bool gated, hipStream_t st) {
+    GemmArgs g = args;
+    g.steps_per_split = (g.K / 128 + g.splits - 1) / g.splits;
     if (dtype == V2VAE_F32) launch_rows<float>(g, gated, st);
     else if (dtype == V2VAE_BF16) launch_rows<bf16_t>(g, gated, st);
     else launch_rows<f16_t>(g, gated, st);
+    if (g.partial) {
+        if (gated) launch_join<float, true>(g, st); else launch_join<float, false>(g, st);
+    }
     return dense_launch_error("dense layer, few rows");
 }
 

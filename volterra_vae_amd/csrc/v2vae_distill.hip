@@ -332,7 +332,7 @@ template <typename T, int G, int NV, bool HELD> static int go(const DistillArgs&
 
 // The group that holds a row has a lane for every teacher entry, up to 64 of them; more are the workgroup's, which keeps them in
 // LDS.  (Entries without a lane or LDS of their own, read again for every other one, took 98 us for 2 rows of 96 logits with 90
-// entries and 54 for 6984 rows of 65 with 50; DIST_A and DIST_B this way.)
+// entries and 54 for 6984 rows of 65 with 50; 16 and 16 this way.)
 template <typename T> static int distill(const DistillArgs& a, int mode, hipStream_t st) {
     constexpr int E = Vec16<T>::N;
     // pieces of a row: V / E if every row starts at one, else of a row that starts anywhere

@@ -147,7 +147,7 @@ def linear_forward(x, weight, bias=None, *, residual=None, activation="none",
     d = _dense(x, weight, act, residual=residual)
     y = x.new_empty((m, n))
     z = torch.empty((m, n), dtype=torch.float32, device=x.device) if keep and act else None
-    ws = None if m <= 16 else _workspace(False, 0, d, x)  # few rows need none
+    ws = None if m <= 16 and x.dtype is not torch.float32 else _workspace(False, 0, d, x)  # few 16-bit rows need none
     _enqueue(lib.v2vae_linear_fwd, "v2vae_linear_fwd", x, d, x.data_ptr(), weight.data_ptr(), _p(bias), _p(residual), y.data_ptr(), _p(z),
              _p(ws))
     return y, z
@@ -240,7 +240,7 @@ def gated_forward(x, weight_gate, weight_up, bias_gate=None, bias_up=None, *, ac
     d = _dense(x, weight_gate, act, w2=weight_up)
     h = x.new_empty((m, n))
     gu = torch.empty((2, m, n), dtype=torch.float32, device=x.device) if keep else None
-    ws = None if m <= 16 else _workspace(True, 0, d, x)
+    ws = None if m <= 16 and x.dtype is not torch.float32 else _workspace(True, 0, d, x)
     _enqueue(lib.v2vae_gated_fwd, "v2vae_gated_fwd", x, d, x.data_ptr(), weight_gate.data_ptr(), weight_up.data_ptr(), _p(bias_gate),
              _p(bias_up), h.data_ptr(), _p(gu), _p(ws))
     return h, gu
