@@ -102,7 +102,10 @@ class DistilledEqualiser:
         """(per-symbol losses, {name: gradient of their mean}) for a window matrix and the teacher's top logits."""
         p = self._views(self._pack.to(self.dtype))
         logits, kept = self._forward(x, p, True)
-        weight = torch.full((x.shape[0],), 1.0 / x.shape[0], device=self.torch_device)
+        # float16: gradients of a large batch's mean would lie below its normal range, those of the sum above it; halfway, and
+        # the rest in float32
+        rest = x.shape[0] ** 0.5 if self.dtype == torch.float16 else 1.0
+        weight = torch.full((x.shape[0],), rest / x.shape[0], device=self.torch_device)
         loss, d = topk_distillation_step(logits, teacher_logits, teacher_index, weight, temperature=self.temperature)
         grads = {}
         d, grads["w_out"], grads["b_out"] = linear_backward(d, kept[-1][0], p["w_out"])
@@ -114,6 +117,8 @@ class DistilledEqualiser:
             d = d + dh
         x, z = kept[0]
         _, grads["w_in"], grads["b_in"] = linear_backward(d, x, p["w_in"], z, activation="tanh", need=(False, True, True))
+        if rest != 1.0:
+            grads = {name: g.float() / rest for name, g in grads.items()}
         return loss, grads
 
     def _class_map(self, teacher):
