@@ -233,7 +233,7 @@ __global__ __launch_bounds__(256, 2) void k_gemm_staged(GemmArgs g) {
         finish_block<T, TN, GATED>(g, acc[i], lds + wave * EPI_BYTES<TN>, lane, m0 + (wm * TM + i) * 32, n0 + wn * (GATED ? 32 : 32 * TN), part, bat);
 }
 
-// Sums of a split contraction and the rest of the epilogue; C columns a thread.  Y threads share an output's parts, thread y those
+// One pass over the parts, 4 ... 10 us, most of it the launch.  Sums of a split contraction and the rest of the epilogue; C columns a thread.  Y threads share an output's parts, thread y those
 // from y on in steps of Y, and their sums are added in order.
 template <typename T, int C, int Y, bool GATED> __global__ __launch_bounds__(256) void k_gemm_join(GemmArgs g) {
     constexpr int X = 256 / Y, W = GATED ? 2 : 1;
@@ -282,8 +282,8 @@ template <typename T, int C, int Y, bool GATED> __global__ __launch_bounds__(256
 template <typename T, bool GATED> void launch_join(const GemmArgs& g, hipStream_t st) {
     const int c = g.N % 4 == 0 ? 4 : 1;
     const int64_t count = (int64_t)g.M * (g.N / c);
-    // many parts of few outputs (96 x 28 of 431 parts: 40 us with one thread an output, 6 with sixteen)
-    const bool shared = g.splits >= 32 && count < 65536;
+    // many parts of few outputs (96 x 28 of 431 parts: 40 us with one thread an output, 6 with sixteen; 512 x 256 of 32 parts: 6 and 9)
+    const bool shared = g.splits >= 32 && (int64_t)g.M * g.N < 65536;
     int64_t blocks = shared ? (count + 15) / 16 : (count + 255) / 256;
     if (blocks > 4096) blocks = 4096;
     const dim3 grid((unsigned)blocks, g.batch);

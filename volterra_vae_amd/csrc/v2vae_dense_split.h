@@ -15,6 +15,11 @@
 //  * B_ROWS, B_COLUMNS: otherwise the workgroup splits its tile on the way into LDS (contraction or rows contiguous in memory).
 //    Both operands then come from far away and run two steps ahead, in two register sets each; the last two steps are written out
 //    so that the loop's loads are unconditional and the compiler can count what is in flight.
+// Bound by issue: splitting A (44 vector instructions a step and 32 x 32 block of it) and the matrix instructions share a SIMD's
+// cycles, which is why planes pay and why wider tiles do, up to the registers: 32768 x 256 -> 2 x 512 gated forward 120 us (143 TF, or
+// 860 TF of bf16 products; 39 us of it are its bytes), its dx 99, dw 113; 65536 x 256 -> 130 39 us; 262144 x 50 -> 64 38 us, of which
+// 23 are its bytes.  Measured and not kept: blocks of zeros at the edge skipped by a branch (training pass 420 us against 405), planes
+// through registers two steps ahead (fewer waves, slower).
 // One scalar base and 32-bit lane offsets per load: strides are at most 2^22 elements.
 // Rows beyond the matrix repeat its last one (their products are not stored); contraction ends take zeros, element by element.
 #ifndef V2VAE_DENSE_SPLIT_H
@@ -291,6 +296,7 @@ __global__ __launch_bounds__(256, FROM == B_PLANES ? (TN <= 2 ? 4 : TN <= 4 ? 3 
     }
 }
 
+// One pass over the weights, 2 x 512 rows of 256: 4 us, transposed 6.5; most of it is the launch.
 // Weights -> three planes [rows][ld] of bf16 pieces, contraction contiguous, zeros beyond its end (ld is a multiple of 32).
 //  forward: plane row r is weight row r; gated: blocks of 32 rows, gate and up of the same features in turn.
 //  backward (TRANSPOSED): plane row r is weight column r, the contraction runs over the weights' rows (gated: gate's, padded to a
