@@ -281,3 +281,16 @@ def test_every_number_of_entries_beside_every_length_of_rows(dtype):
             if k > 3:
                 idx[::2, 2] = idx[::2, 0]
             check(z, t, idx, w, 1.3)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16", "f16"])
+def test_many_long_rows(dtype):
+    """Rows that are streamed for the loss: aligned and not, with masked parts and rows of nothing, more entries than a wave has lanes."""
+    for v, k in ((17029, 16), (8200, 100)):
+        z, t, idx, w = case(520, v, k, dtype, v)
+        z[:, 100:5000] = -math.inf
+        z[7] = -math.inf
+        idx[7] = -1
+        idx[8, :2] = 3 * v // 4
+        idx[idx >= 100] = idx[idx >= 100].clamp_min(5000)
+        check(z, t, idx, w, 0.8)

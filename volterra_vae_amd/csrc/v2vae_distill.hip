@@ -147,8 +147,15 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void k_distill(DistillArgs a) {
             }
             if constexpr (MODE & DO_GRAD) {
                 for (int i = 0; i < a.k; ++i) {  // all lanes of the group, entry or not
-                    const int ci = __shfl(my_cls, i, GE);
-                    const float pi = __shfl(my_p, i, GE);
+                    int ci;
+                    float pi;
+                    if constexpr (GE == 64) {  // a whole wave: lane i's registers are read as scalars, without LDS
+                        ci = __builtin_amdgcn_readlane(my_cls, i);
+                        pi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_p), i));
+                    } else {
+                        ci = __shfl(my_cls, i, GE);
+                        pi = __shfl(my_p, i, GE);
+                    }
                     if (ci == my_cls) {
                         p_all += pi;
                         first &= i >= tid;
@@ -185,19 +192,26 @@ __global__ __launch_bounds__(G > 64 ? G : 256) void k_distill(DistillArgs a) {
                 }
             l = lanes.sum(l, 1);
         } else {
-            // one pass with a running maximum per thread, joined at the end
+            // one pass with a running maximum per thread, joined at the end; NV pieces in flight
             float mine = -INFINITY;
-            for (int i = tid; i < pieces; i += G) {
-                const Vec16<T> v = get(i);
-                float top = (float)v.e[0];
+            for (int i0 = tid; i0 < pieces; i0 += NV * G) {
+                Vec16<T> v[NV];
 #pragma unroll
-                for (int e = 1; e < E; ++e) top = fmaxf(top, (float)v.e[e]);
+                for (int i = 0; i < NV; ++i) v[i] = get(i0 + i * G);
+                float top = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) top = fmaxf(top, (float)v[i].e[e]);
                 if (top > mine) {
                     l *= exp_diff(mine, top, c);
                     mine = top;
                 }
+                const float at = finite(mine);
 #pragma unroll
-                for (int e = 0; e < E; ++e) l += exp_diff((float)v.e[e], finite(mine), c);
+                for (int i = 0; i < NV; ++i)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) l += exp_diff((float)v[i].e[e], at, c);
             }
             zmax = lanes.max(mine, 0);
             l = lanes.sum(mine == -INFINITY ? l : l * exp_diff(mine, zmax, c), 1);
@@ -342,6 +356,9 @@ template <typename T> static int distill(const DistillArgs& a, int mode, hipStre
     // pieces of a row: V / E if every row starts at one, else of a row that starts anywhere
     const bool aligned = ((uintptr_t)a.z & 15) == 0 && (a.ld_z % E == 0 || a.rows == 1);
     const int64_t pieces = aligned ? (a.V + E - 1) / E : (a.V + 2 * E - 2) / E;
+    // The loss alone needs no row held: many long rows stream through smaller workgroups (bf16 losses, held / streamed: 2688 x 17029 37 /
+    // 24 us, 4096 x 32000 53 / 44; f16 20000 x 6000 49 / 52, therefore held, and few rows have too few workgroups this way).
+    if (mode == DO_LOSS && pieces > 1024 && pieces <= 8192 && a.rows >= 512) return go<T, 256, 4, false>(a, mode, st);
     if (pieces <= 8 && a.k <= 8) return go<T, 8, 1, true>(a, mode, st);
     if (pieces <= 16 && a.k <= 16) return go<T, 16, 1, true>(a, mode, st);
     if (pieces <= 32 && a.k <= 16) return go<T, 16, 2, true>(a, mode, st);
@@ -353,7 +370,7 @@ template <typename T> static int distill(const DistillArgs& a, int mode, hipStre
     if (pieces <= 2048) return go<T, 256, 8, true>(a, mode, st);
     if (pieces <= 4096) return go<T, 512, 8, true>(a, mode, st);
     if (pieces <= 8192) return go<T, 1024, 8, true>(a, mode, st);
-    return go<T, 1024, 1, false>(a, mode, st);
+    return go<T, 1024, 4, false>(a, mode, st);
 }
 
 static int check_distill(const v2vae_distill* d) {
