@@ -6,10 +6,11 @@
 namespace v2vae {
 
 // ---- dz = dy act'(z) and its column sums -------------------------------------------------------------------------------------
-// One pass over dy and the float pre-activations; memory bound.  A block owns a strip of columns and a chunk of rows, sums its
-// columns in float in a fixed order (per thread along the rows, then over the block's row threads) and leaves one partial per
-// chunk; k_column_join adds the chunks (4 ... 5 us).  dz is rounded to T here, once, after its contribution to the column sum.
-// Float 65536 x 256: 43 us (4.6 TB/s); bf16 gated 4096 x 5632: 56 us (5.7 TB/s).
+// One pass over dy and the float pre-activations; memory bound.  A block owns a strip of columns and every so many rows (a chunk): all
+// blocks move through memory together (65536 x 256 float 38 us, 43 with rows that follow one another; gated 173475 x 1320 1180 and
+// 1300).  It sums its columns in float in a fixed order (per thread along the rows, then over the block's row threads) and leaves one
+// partial per chunk; k_column_join adds the chunks (4 ... 5 us).  dz is rounded to T here, once, after its contribution to the column
+// sum.  Float 65536 x 256: 5.3 TB/s; bf16 gated 4096 x 5632: 56 us (5.7 TB/s).
 struct SlopeArgs {
     const void* dy;
     int64_t ld_dy;
@@ -17,7 +18,7 @@ struct SlopeArgs {
     void* d[2];         // dz [M][ld_d], zeros in columns N ... ld_d - 1 (NULL: only the sums)
     int64_t ld_d;
     float* part[2];     // [chunks][N] (NULL: no sums)
-    int64_t M, rows_per_chunk;
+    int64_t M;
     int N, cx;          // cx threads along the columns, four each, 256 / cx along the rows
 };
 
@@ -26,20 +27,22 @@ template <typename T, int ACT, bool GATED> __global__ __launch_bounds__(256) voi
     __shared__ float s_sum[GATED ? 2 : 1][256 * V];
     const int tid = threadIdx.x, cx = a.cx, ry = 256 / cx, tx = tid % cx, ty = tid / cx;
     const int64_t n = ((int64_t)blockIdx.x * cx + tx) * V;
-    const int64_t lo = (int64_t)blockIdx.y * a.rows_per_chunk, hi = lo + a.rows_per_chunk < a.M ? lo + a.rows_per_chunk : a.M;
     float s0[V], s1[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) s0[v] = s1[v] = 0.f;
-    // WHOLE: all V columns exist; else those beyond N are zeros, and stored where dz has columns for them
+    // The last columns, fewer than V, are taken together with the ones before them, which their own thread has as well (and writes the
+    // same): a wave goes through its rows once, without a branch.  Not WHOLE: fewer than V columns in all.
+    const int beyond = n < a.N && n + V > a.N && a.N >= V ? (int)(n + V - a.N) : 0;
     auto rows = [&](auto all) {
         constexpr bool WHOLE = decltype(all)::value;
-        const int count = (int)(a.N - n), out = (int)(a.ld_d - n);
+        const int64_t n1 = n - beyond;
+        const int count = (int)(a.N - n1);
 #pragma unroll 2
-        for (int64_t m = lo + ty; m < hi; m += ry) {
+        for (int64_t m = (int64_t)blockIdx.y * ry + ty; m < a.M; m += (int64_t)gridDim.y * ry) {
             float dy[V], z0[V], z1[V];
-            load_columns<T, V>(a.dy, m * a.ld_dy + n, count, WHOLE, dy);
-            if (a.z[0]) load_columns<float, V>(a.z[0], m * a.N + n, count, WHOLE, z0);
-            if constexpr (GATED) load_columns<float, V>(a.z[1], m * a.N + n, count, WHOLE, z1);
+            load_columns<T, V>(a.dy, m * a.ld_dy + n1, count, WHOLE, dy);
+            if (a.z[0]) load_columns<float, V>(a.z[0], m * a.N + n1, count, WHOLE, z0);
+            if constexpr (GATED) load_columns<float, V>(a.z[1], m * a.N + n1, count, WHOLE, z1);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 float val;
@@ -53,13 +56,28 @@ template <typename T, int ACT, bool GATED> __global__ __launch_bounds__(256) voi
                 }
                 s0[v] += dy[v];
             }
-            if (a.d[0]) store_columns<T, V>(a.d[0], m * a.ld_d + n, out, WHOLE, dy);
+            if (a.d[0]) store_columns<T, V>(a.d[0], m * a.ld_d + n1, count, WHOLE, dy);
             if constexpr (GATED)
-                if (a.d[1]) store_columns<T, V>(a.d[1], m * a.ld_d + n, out, WHOLE, z1);
+                if (a.d[1]) store_columns<T, V>(a.d[1], m * a.ld_d + n1, count, WHOLE, z1);
         }
     };
-    if (n + V <= a.N) rows(std::true_type());
-    else if (n < a.ld_d) rows(std::false_type());
+    if (n < a.N) {
+        if (a.N >= V) rows(std::true_type()); else rows(std::false_type());
+    }
+    if (a.d[0] && n + V > a.N && n < a.ld_d) {  // zeros in the columns that dz is padded with
+        for (int64_t m = (int64_t)blockIdx.y * ry + ty; m < a.M; m += (int64_t)gridDim.y * ry)
+            for (int64_t i = n > a.N ? n : a.N; i < n + V && i < a.ld_d; ++i) {
+                ((T*)a.d[0])[m * a.ld_d + i] = (T)0.f;
+                if constexpr (GATED) ((T*)a.d[1])[m * a.ld_d + i] = (T)0.f;
+            }
+    }
+    for (int q = 0; q < beyond; ++q) {  // this thread's own columns to the front
+#pragma unroll
+        for (int v = 0; v + 1 < V; ++v) {
+            s0[v] = s0[v + 1];
+            s1[v] = s1[v + 1];
+        }
+    }
     if (a.part[0] == nullptr) return;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -156,8 +174,9 @@ static Cut cut_product(int64_t M, int64_t N, int64_t K, int segs, int batch, int
     const int64_t bk = dtype == V2VAE_F32 ? 32 : 64, steps = ((K + bk - 1) / bk) * segs;
     auto tiles_of = [&](int64_t t) { return ((M + t - 1) / t) * ((N * (gated ? 2 : 1) + t - 1) / t) * batch; };
     // A compute unit holds one 256 x 256 tile or two of 128 x 128.  The larger tile runs 1.12 times as fast (8192 x 4096 x 4096
-    // training pass 755 against 861 us) where the tiles fill the chip's last round as well: full() is the share they fill.
-    auto full = [](int64_t tiles, int64_t slots) { return (double)tiles / ((tiles + slots - 1) / slots * slots); };
+    // training pass 755 against 861 us) where the tiles fill the matrix and the chip's last round as well: rounds() is the work of
+    // all rounds (179673 x 331 -> 104 forward: 130 us with 256, 91 with 128).
+    auto rounds = [&](int64_t t, int64_t slots) { return (double)((tiles_of(t) + slots - 1) / slots * slots) * t * t; };
     Cut c;
     int64_t tiles, s = 1;
     if (dtype == V2VAE_F32) {
@@ -186,7 +205,7 @@ static Cut cut_product(int64_t M, int64_t N, int64_t K, int segs, int batch, int
     } else if (direct && N * (gated ? 2 : 1) <= 64) {  // 128 x 64: one column of tiles, more of them on a compute unit
         c.tile = TILE_64;
         tiles = ((M + 127) / 128) * batch;
-    } else if (direct && tiles_of(256) >= 128 && full(tiles_of(256), 256) >= 0.88 * full(tiles_of(128), 512)) {
+    } else if (direct && tiles_of(256) >= 128 && 0.88 * rounds(256, 256) <= rounds(128, 512)) {
         c.tile = TILE_256;
         tiles = tiles_of(256);
     } else if (tiles_of(128) >= 256 || tiles_of(128) * (steps / 8) >= 256 || direct) {
@@ -245,7 +264,13 @@ static void slope_shape(int64_t M, int64_t N, int* cx, int* gx, int* chunks) {
     const int64_t cols = (N + 3) / 4;
     int c = 1;
     while (c < cols && c < 64) c *= 2;
+    // Narrower strips, down to 256 bytes of float, where they leave fewer threads without a column (gated 166354 x 302, 76 threads'
+    // columns: 325 us in strips of 64, 286 in strips of 16).
+    auto padded = [&](int s) { return (cols + s - 1) / s * s; };
     *cx = c;
+    for (int s = c / 2; s >= 16; s /= 2)
+        if (padded(s) * 4 <= padded(c) * 3 && padded(s) < padded(*cx)) *cx = s;
+    c = *cx;
     *gx = (int)((cols + c - 1) / c);
     int64_t n = 2048 / *gx;
     const int64_t most = M / ((256 / c) * 4);
@@ -436,7 +461,6 @@ static int backward(const v2vae_dense* d, const void* x, const void* w0, const v
         }
         int gx, chunks;
         slope_shape(M, s.ld_d, &s.cx, &gx, &chunks);
-        s.rows_per_chunk = (M + chunks - 1) / chunks;
         const dim3 grid(gx, chunks);
         auto slopes = [&](auto t, auto kind) {
             typedef decltype(t) T;
