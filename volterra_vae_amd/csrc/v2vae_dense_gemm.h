@@ -233,8 +233,8 @@ __global__ __launch_bounds__(256, 2) void k_gemm_staged(GemmArgs g) {
         finish_block<T, TN, GATED>(g, acc[i], lds + wave * EPI_BYTES<TN>, lane, m0 + (wm * TM + i) * 32, n0 + wn * (GATED ? 32 : 32 * TN), part, bat);
 }
 
-// One pass over the parts, 4 ... 10 us, most of it the launch.  Sums of a split contraction and the rest of the epilogue; C columns a thread.  Y threads share an output's parts, thread y those
-// from y on in steps of Y, and their sums are added in order.
+// Sums of a split contraction and the rest of the epilogue; C columns a thread.  Y threads share an output's parts, thread y those
+// from y on in steps of Y, and their sums are added in order.  One pass over the parts, 4 ... 10 us, most of it the launch.
 template <typename T, int C, int Y, bool GATED> __global__ __launch_bounds__(256) void k_gemm_join(GemmArgs g) {
     constexpr int X = 256 / Y, W = GATED ? 2 : 1;
     __shared__ float s_part[Y > 1 ? Y : 1][Y > 1 ? X : 1][Y > 1 ? W * C : 1];

@@ -358,7 +358,9 @@ template <typename T> static int distill(const DistillArgs& a, int mode, hipStre
     const int64_t pieces = aligned ? (a.V + E - 1) / E : (a.V + 2 * E - 2) / E;
     // The loss alone needs no row held: many long rows stream through smaller workgroups (bf16 losses, held / streamed: 2688 x 17029 37 /
     // 24 us, 4096 x 32000 53 / 44; f16 20000 x 6000 49 / 52, therefore held, and few rows have too few workgroups this way).
-    if (mode == DO_LOSS && pieces > 1024 && pieces <= 8192 && a.rows >= 512) return go<T, 256, 4, false>(a, mode, st);
+    // (Rows beyond 2^22 are left to the held form, whose launch limits then refuse the same sizes for the loss as for the gradient.)
+    if (mode == DO_LOSS && pieces > 1024 && pieces <= 8192 && a.rows >= 512 && a.rows < (int64_t)1 << 22)
+        return go<T, 256, 4, false>(a, mode, st);
     if (pieces <= 8 && a.k <= 8) return go<T, 8, 1, true>(a, mode, st);
     if (pieces <= 16 && a.k <= 16) return go<T, 16, 1, true>(a, mode, st);
     if (pieces <= 32 && a.k <= 16) return go<T, 16, 2, true>(a, mode, st);
