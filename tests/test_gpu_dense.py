@@ -536,3 +536,29 @@ def test_narrow_layers_of_many_rows(dtype):
         x, wg, wu, bg, bu, dh = gated_case(m, k, n, dtype, True, "odd" if k % 2 else "plain", k + n)
         h, gu = gated_forward(x, wg, wu, bg, bu, keep=True)
         check_gated(x, wg, wu, bg, bu, dh, "silu", h, gated_backward(dh, x, wg, wu, gu), dtype)
+
+
+@pytest.mark.parametrize("m,k,n", [(300, 1024, 96), (500, 1024, 256), (1024, 2048, 512), (4096, 2048, 1000)], ids=lambda v: str(v))
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16", "f16"])
+def test_one_weight_of_a_gated_block(dtype, m, k, n):
+    """The other weight frozen, at sizes where one gradient alone has fewer tiles than the chip has room for: the same bits as of both
+    gradients, and nothing written behind the workspace that was asked for."""
+    from volterra_vae_amd import _lib
+    from volterra_vae_amd.dense_ops import _dense, gated_backward, gated_forward, gated_linear
+    x, wg, wu, bg, bu, dh = gated_case(m, k, n, dtype, True, "plain", m)
+    h, gu = gated_forward(x, wg, wu, bg, bu, keep=True)
+    full = gated_backward(dh, x, wg, wu, gu)
+    check_gated(x, wg, wu, bg, bu, dh, "silu", h, full, dtype)
+    for i in (1, 2):
+        leaves = [t.clone().requires_grad_(j in (0, i)) for j, t in enumerate((x, wg, wu, bg, bu))]
+        gx, gw = torch.autograd.grad(gated_linear(*leaves), (leaves[0], leaves[i]), dh)
+        assert torch.equal(gx, full[0]) and torch.equal(gw, full[i])
+        d = _dense(x, wg, 2, w2=wu, dy=dh)
+        size = _lib.lib.v2vae_gated_workspace_bytes(d, 1)
+        behind = 2 * n * k * 4 * 4   # more than four parts of two gradients would take
+        ws = torch.full((size + behind,), 0x5A, dtype=torch.uint8, device=dev())
+        out = torch.empty_like(wg)
+        _lib.check(_lib.lib.v2vae_gated_bwd(d, x.data_ptr(), wg.data_ptr(), wu.data_ptr(), gu.data_ptr(), dh.data_ptr(), None,
+                                            out.data_ptr() if i == 1 else None, out.data_ptr() if i == 2 else None, None, None, ws.data_ptr(),
+                                            torch.cuda.current_stream().cuda_stream))
+        assert torch.equal(out, full[i]) and bool((ws[size:] == 0x5A).all())

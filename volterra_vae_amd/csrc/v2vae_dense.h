@@ -6,7 +6,7 @@
 
 #include <type_traits>
 
-#include "../../include/v2vae_hip.h"
+#include "v2vae_dense_plan.h"
 
 namespace v2vae {
 
@@ -242,7 +242,6 @@ __device__ __forceinline__ void finish_gated(const GemmArgs& g, int64_t m, int n
 }
 // launchers; 0 or a V2VAE_E* code
 enum { LAYOUT_KK = 0, LAYOUT_KM = 1, LAYOUT_MM = 2 };  // A / B with the contraction (K) or the row index (M) contiguous
-enum { TILE_128, TILE_64, TILE_256, TILE_96, TILE_160 };  // float32: columns of a tile of 128 rows; else both sides
 int gemm_direct_bf16(const GemmArgs&, int layout, bool gated, int tile, hipStream_t);
 int gemm_direct_f16(const GemmArgs&, int layout, bool gated, int tile, hipStream_t);
 int split_planes(const GemmArgs&, bool transposed, bool gated, int N, int K, hipStream_t);  // b[], ldb[]: N x K weights
@@ -250,9 +249,6 @@ int gemm_split(const GemmArgs&, int layout, bool gated, int tile, hipStream_t); 
 int gemm_staged_bf16(const GemmArgs&, int layout, bool gated, int tile, hipStream_t);
 int gemm_staged_f16(const GemmArgs&, int layout, bool gated, int tile, hipStream_t);
 
-// few rows (v2vae_dense_rows.hip); beyond, the tiled products read the weights as fast
-inline int64_t few_rows(int dtype) { return dtype == V2VAE_F32 ? 32 : 16; }
-int rows_splits(int dtype, int64_t in, int64_t out, bool gated);  // parts of the contraction
 int dense_rows(const GemmArgs& g, int dtype, bool gated, hipStream_t st);
 
 int dense_launch_error(const char* where);  // V2VAE_OK, or V2VAE_ELAUNCH with the text kept for v2vae_last_error

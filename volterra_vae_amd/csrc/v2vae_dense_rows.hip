@@ -171,17 +171,6 @@ template <typename T, int W, int MT, bool ODD> static void launch_waves(const Ge
     if (gated) hipLaunchKernelGGL((k_dense_rows<T, W, MT, ODD, true>), dim3((g.N + 7) / 8, g.splits), dim3(64 * W), 0, st, g);
     else hipLaunchKernelGGL((k_dense_rows<T, W, MT, ODD, false>), dim3((g.N + 15) / 16, g.splits), dim3(64 * W), 0, st, g);
 }
-// float on few, long weight rows: the contraction in parts, to a workgroup a compute unit (9 x 8165 -> 2 x 504: 25 us in one part,
-// 18 in four and their join).  16-bit rows, of half the bytes, end before a second launch would pay.
-int rows_splits(int dtype, int64_t in, int64_t out, bool gated) {
-    if (dtype != V2VAE_F32) return 1;
-    const int64_t groups = gated ? (out + 7) / 8 : (out + 15) / 16;
-    int64_t s = 256 / groups;
-    if (s > in / 1024) s = in / 1024;
-    if (s < 3) return 1;
-    const int64_t turns = in / 128, per = (turns + s - 1) / s;
-    return (int)((turns + per - 1) / per);  // none without a turn
-}
 template <typename T> static void launch_rows(const GemmArgs& g, bool gated, hipStream_t st) {
     // sixteen waves on a long contraction; float, which needs twice the registers a turn, eight
     if constexpr (sizeof(T) == 4) {
