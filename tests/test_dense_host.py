@@ -122,3 +122,42 @@ def test_structures_match_the_header():
         declared = re.findall(r"(\w+)\s+(\w+);", body)
         kinds = {"int32_t": C.c_int32, "int64_t": C.c_int64, "float": C.c_float}
         assert [(n.rstrip("_"), t) for n, t in struct._fields_] == [(n, kinds[k]) for k, n in declared]
+
+
+def without_launches(monkeypatch):
+    """CPU tensors pass the checks and what would be launched is listed: (entry point, its arguments)."""
+    calls = []
+    monkeypatch.setattr(dense_ops, "_enqueue", lambda fn, name, t, *args: calls.append((name, args)))
+    monkeypatch.setattr(dense_ops, "_check_tensor", lambda *args, **kw: None)
+    monkeypatch.setattr(dense_ops, "_workspace", lambda gated, backward, d, x: torch.empty(256, dtype=torch.uint8))
+    return calls
+
+
+def test_the_backward_passes_describe_the_tensors_that_saved_tensor_hooks_give_back(monkeypatch):
+    """Hooks that move saved tensors elsewhere give strided ones back contiguous: the row strides of the backward call are theirs, not
+    those of the forward call."""
+    calls = without_launches(monkeypatch)
+    z = torch.zeros(6, 20)[:, 3:12].requires_grad_(True)
+    t, i = torch.zeros(6, 8)[:, 2:5], torch.zeros(6, 7, dtype=torch.int32)[:, 1:4]
+    x, w = torch.zeros(40, 20)[:, 3:12].requires_grad_(True), torch.zeros(5, 16)[:, :9].requires_grad_(True)
+    held = []   # what the hooks give back lives on: an address then names one tensor
+
+    def unpack(t):
+        held.append(t.contiguous())
+        return held[-1]
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        outs = [dense_ops.topk_distillation(z, t, i), dense_ops.linear(x, w, activation="silu"), dense_ops.gated_linear(x, w, w)]
+    for out, leaf in zip(outs, (z, x, x)):
+        torch.autograd.grad(out, leaf, torch.ones_like(out))
+    by_name = {name: args for name, args in calls}
+    d = by_name["v2vae_distill_fwd"][0]
+    assert (d.ld_logits, d.ld_teacher, d.ld_index) == (20, 8, 7)
+    d, *pointers = by_name["v2vae_distill_bwd"]
+    addresses = {a.data_ptr() for a in held}
+    assert pointers[0] in addresses and (d.ld_logits, d.ld_teacher, d.ld_index) == (9, 3, 3)
+    for name in ("v2vae_linear", "v2vae_gated"):
+        d = by_name[name + "_fwd"][0]
+        assert (d.ld_x, d.ld_w) == (20, 16)
+        d, *pointers = by_name[name + "_bwd"]
+        assert pointers[0] in addresses and (d.ld_x, d.ld_w) == (9, 9)

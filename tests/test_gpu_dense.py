@@ -562,3 +562,19 @@ def test_one_weight_of_a_gated_block(dtype, m, k, n):
                                             out.data_ptr() if i == 1 else None, out.data_ptr() if i == 2 else None, None, None, ws.data_ptr(),
                                             torch.cuda.current_stream().cuda_stream))
         assert torch.equal(out, full[i]) and bool((ws[size:] == 0x5A).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16", "f16"])
+def test_layers_whose_tensors_are_kept_on_the_host_between_the_passes(dtype):
+    """save_on_cpu gives strided rows back contiguous: gradients within the same bounds."""
+    from volterra_vae_amd.dense_ops import gated_linear, linear
+    x, w, b, r, dy = linear_case(70, 72, 56, dtype, "silu", True, True, "odd", 4)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    with torch.autograd.graph.save_on_cpu():
+        y = linear(*leaves, residual=r, activation="silu")
+    check_linear(x, w, b, r, dy, "silu", y.detach(), torch.autograd.grad(y, leaves, dy), dtype)
+    x, wg, wu, bg, bu, dh = gated_case(70, 72, 56, dtype, True, "odd", 4)
+    leaves = [t.requires_grad_(True) for t in (x, wg, wu, bg, bu)]
+    with torch.autograd.graph.save_on_cpu():
+        h = gated_linear(*leaves)
+    check_gated(x, wg, wu, bg, bu, dh, "silu", h.detach(), torch.autograd.grad(h, leaves, dh), dtype)

@@ -294,3 +294,22 @@ def test_many_long_rows(dtype):
         idx[8, :2] = 3 * v // 4
         idx[idx >= 100] = idx[idx >= 100].clamp_min(5000)
         check(z, t, idx, w, 0.8)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16", "f16"])
+def test_padded_rows_that_are_kept_on_the_host_between_the_passes(dtype):
+    """save_on_cpu gives strided rows back contiguous; the gradient is that of the same rows without the hooks, to the rounding of sums
+    whose rows start elsewhere in a 16-byte piece, and within the formula's bound."""
+    from volterra_vae_amd.dense_ops import topk_distillation
+    for v in (60, 3001, 40000):
+        z, t, idx, w = case(6, v, 9, dtype, v + 2)
+        zb, tb, ib = (torch.zeros((6, x.shape[1] + 7), dtype=x.dtype, device=dev()) for x in (z, t, idx))
+        zb[:, 3:3 + v], tb[:, 2:11], ib[:, 1:10] = z, t, idx
+        leaf = zb[:, 3:3 + v].requires_grad_(True)
+        with torch.autograd.graph.save_on_cpu():
+            loss = topk_distillation(leaf, tb[:, 2:11], ib[:, 1:10], temperature=1.5)
+        (grad,) = torch.autograd.grad(loss, leaf, w)
+        _, ref_grad, _, grad_scale = reference(z, t, idx, w, 1.5)
+        tiny = torch.finfo(dtype).tiny * torch.finfo(dtype).eps
+        bound = torch.finfo(dtype).eps / 2 * ref_grad.abs() + 16 * EPS32 * grad_scale + tiny
+        assert bool(((grad.double().cpu() - ref_grad).abs() <= bound).all())

@@ -321,8 +321,13 @@ def _distill(logits, teacher_logits, teacher_index, temperature):
                          f"{tuple(teacher_index.shape)}")
     if not 1e-4 <= temperature <= 1e4:
         raise ValueError(f"temperature: 1e-4 ... 1e4 (got {temperature})")
-    return Distill(_DTYPES[logits.dtype], _DTYPES[teacher_logits.dtype], 32 if teacher_index.dtype == torch.int32 else 64, k, m, v,
-                   _row_stride(logits) if m > 1 else v, _row_stride(teacher_logits), _row_stride(teacher_index), temperature, 0)
+    return _distill_block(logits, teacher_logits, teacher_index, temperature)
+
+
+def _distill_block(logits, teacher_logits, teacher_index, temperature):
+    return Distill(_DTYPES[logits.dtype], _DTYPES[teacher_logits.dtype], 32 if teacher_index.dtype == torch.int32 else 64,
+                   teacher_logits.shape[1], logits.shape[0], logits.shape[1], _row_stride(logits), _row_stride(teacher_logits),
+                   _row_stride(teacher_index), temperature, 0)
 
 
 def _check_weight(weight, logits):
@@ -344,17 +349,20 @@ def topk_distillation_step(logits, teacher_logits, teacher_index, row_weight, *,
 class _Distillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher_logits, teacher_index, temperature):
-        ctx.d = _distill(logits, teacher_logits, teacher_index, temperature)
-        loss, stats = _distill_forward(ctx.d, logits, teacher_logits, teacher_index, True)
+        d = _distill(logits, teacher_logits, teacher_index, temperature)
+        loss, stats = _distill_forward(d, logits, teacher_logits, teacher_index, True)
         ctx.save_for_backward(logits, teacher_logits, teacher_index, stats)
+        ctx.temperature = temperature
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, weight):
+        # hooks on saved tensors may give them back with other strides than the forward pass saw
         logits, teacher_logits, teacher_index, stats = ctx.saved_tensors
+        d = _distill_block(logits, teacher_logits, teacher_index, ctx.temperature)
         weight, grad = weight.contiguous().resolve_neg(), logits.new_empty(logits.shape)
-        _enqueue(lib.v2vae_distill_bwd, "v2vae_distill_bwd", logits, ctx.d, _p(logits), _p(teacher_logits), _p(teacher_index), _p(stats),
+        _enqueue(lib.v2vae_distill_bwd, "v2vae_distill_bwd", logits, d, _p(logits), _p(teacher_logits), _p(teacher_index), _p(stats),
                  _p(weight), _p(grad))
         return grad, None, None, None
 
