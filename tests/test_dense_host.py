@@ -161,3 +161,38 @@ def test_the_backward_passes_describe_the_tensors_that_saved_tensor_hooks_give_b
         assert (d.ld_x, d.ld_w) == (20, 16)
         d, *pointers = by_name[name + "_bwd"]
         assert pointers[0] in addresses and (d.ld_x, d.ld_w) == (9, 9)
+
+
+def test_forward_mode_derivatives_are_refused(monkeypatch):
+    """A dual tensor in any place raises, with and without a graph, in the differentiable and in the explicit passes; without tangents
+    the same calls pass inside a dual level."""
+    from torch.autograd import forward_ad as fw
+    calls = without_launches(monkeypatch)
+    x, w, b, r = torch.zeros(6, 5), torch.zeros(4, 5), torch.zeros(4), torch.zeros(6, 4)
+    z, t, i = torch.zeros(6, 9), torch.zeros(6, 3), torch.zeros(6, 3, dtype=torch.int32)
+    gu, v = torch.zeros(2, 6, 4), torch.zeros(6)
+    passes = [(lambda x, w, b, r: dense_ops.linear(x, w, b, residual=r), (x, w, b, r)),
+              (lambda x, w, u, b, c: dense_ops.gated_linear(x, w, u, b, c), (x, w, w, b, b)),
+              (lambda z, t: dense_ops.topk_distillation(z, t, i), (z, t)),
+              (lambda z, t, v: dense_ops.topk_distillation_step(z, t, i, v), (z, t, v)),
+              (lambda x, w, b, r: dense_ops.linear_forward(x, w, b, residual=r), (x, w, b, r)),
+              (lambda x, w, u: dense_ops.gated_forward(x, w, u), (x, w, w)),
+              (lambda d, x, w, z: dense_ops.linear_backward(d, x, w, z, activation="silu"), (r, x, w, r)),
+              (lambda d, x, w, u, g: dense_ops.gated_backward(d, x, w, u, g), (r, x, w, w, gu))]
+    with fw.dual_level():
+        for f, args in passes:
+            f(*args)
+            for place in range(len(args)):
+                dual = [fw.make_dual(a.clone(), torch.ones_like(a)) if n == place else a for n, a in enumerate(args)]
+                before = len(calls)
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    f(*dual)
+                assert len(calls) == before
+        with pytest.raises(NotImplementedError):
+            dense_ops.linear(fw.make_dual(x.clone().requires_grad_(), torch.ones_like(x)), w)
+        for out, leaf in ((lambda a: dense_ops.linear(a, w), x), (lambda a: dense_ops.gated_linear(a, w, w), x),
+                          (lambda a: dense_ops.topk_distillation(a, t, i), z)):
+            leaf = leaf.clone().requires_grad_()
+            y = out(leaf)
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                torch.autograd.grad(y, leaf, fw.make_dual(torch.ones_like(y), torch.ones_like(y)))

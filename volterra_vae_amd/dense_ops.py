@@ -7,7 +7,7 @@ may overlap (windows that slide over one received sequence are a matrix with the
 Two ways to train: the functions named above are differentiable; `linear_forward` / `linear_backward`, `gated_forward` /
 `gated_backward` and `topk_distillation_step` are the same passes with every gradient an explicit result, for training loops
 that run without autograd, and for HIP graphs: these are what to capture (a backward pass of autograd that is captured while an
-eager graph of the same leaves lives ends the process).  `torch.ops.v2vae.linear`, `torch.ops.v2vae.gated_linear` and
+eager graph of the same leaves lives ends the process).  Forward-mode derivatives are refused.  `torch.ops.v2vae.linear`, `torch.ops.v2vae.gated_linear` and
 `torch.ops.v2vae.topk_distillation` are the differentiable forms as registered ops.
 """
 from __future__ import annotations
@@ -16,6 +16,7 @@ import functools
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import Dense, Distill, check, lib
@@ -50,6 +51,14 @@ def _check_tensor(t, name, dim, like=None, dtype=None):
     if t.is_neg():
         raise ValueError(f"{name} is a negation that is not carried out yet (pass {name}.resolve_neg())")
     raise ValueError(f"{name} must have unit stride in its last dimension")
+
+
+def _refuse_tangents(*tensors):
+    """The kernels carry no tangents: a dual tensor's derivative would be lost without a word."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("forward-mode derivatives: these operators have a backward pass only")
 
 
 def _row_stride(t):
@@ -137,6 +146,7 @@ def linear_forward(x, weight, bias=None, *, residual=None, activation="none",
     """(y, z) for x [M, K], weight [N, K]: y = activation(x weight^T + bias) + residual, and, if `keep` and there is an
     activation, the float32 pre-activations z [M, N] that `linear_backward` wants (else None)."""
     act = _activation(activation)
+    _refuse_tangents(x, weight, bias, residual)
     _check_tensor(x, "x", 2)
     _check_layer(x, weight, "weight", bias, "bias")
     m, n = x.shape[0], weight.shape[0]
@@ -169,6 +179,7 @@ def linear_backward(dy, x, weight, z=None, *, activation="none", need=(True, Tru
 
 
 def _linear_backward(dy, x, weight, z, act, need):
+    _refuse_tangents(dy, x, weight, z)
     m, k, n = x.shape[0], x.shape[1], weight.shape[0]
     d = _dense(x, weight, act, dy=dy)
     new = lambda wanted, *shape: x.new_empty(shape) if wanted else None  # noqa: E731
@@ -231,6 +242,7 @@ def gated_forward(x, weight_gate, weight_up, bias_gate=None, bias_up=None, *, ac
     """(h, gu) for x [M, K], weights [N, K]: h = activation(x weight_gate^T + bias_gate) * (x weight_up^T + bias_up), and, if
     `keep`, the float32 pre-activations gu [2, M, N] (gate, up) that `gated_backward` wants (else None)."""
     act = _activation(activation)
+    _refuse_tangents(x, weight_gate, weight_up, bias_gate, bias_up)
     _check_tensor(x, "x", 2)
     _check_layer(x, weight_gate, "weight_gate", bias_gate, "bias_gate")
     _check_layer(x, weight_up, "weight_up", bias_up, "bias_up")
@@ -262,6 +274,7 @@ def gated_backward(dh, x, weight_gate, weight_up, gu, *, activation="silu", need
 
 
 def _gated_backward(dh, x, weight_gate, weight_up, gu, act, need):
+    _refuse_tangents(dh, x, weight_gate, weight_up, gu)
     m, k, n = x.shape[0], x.shape[1], weight_gate.shape[0]
     d = _dense(x, weight_gate, act, w2=weight_up, dy=dh)
     new = lambda wanted, *shape: x.new_empty(shape) if wanted else None  # noqa: E731
@@ -303,6 +316,7 @@ def gated_linear(x: torch.Tensor, weight_gate: torch.Tensor, weight_up: torch.Te
 
 # ------------------------------------------------------------------------------------------------ distillation
 def _distill(logits, teacher_logits, teacher_index, temperature):
+    _refuse_tangents(logits, teacher_logits)
     _check_tensor(logits, "logits", 2)
     if getattr(teacher_logits, "dtype", None) not in _DTYPES:
         raise NotImplementedError("teacher_logits: a float32, bfloat16 or float16 tensor")
@@ -331,6 +345,7 @@ def _distill_block(logits, teacher_logits, teacher_index, temperature):
 
 
 def _check_weight(weight, logits):
+    _refuse_tangents(weight)
     _check_tensor(weight, "row_weight", 1, like=logits, dtype=torch.float32)
     if weight.shape[0] != logits.shape[0]:
         raise ValueError(f"row_weight: expected {logits.shape[0]} values, got {weight.shape[0]}")
@@ -358,6 +373,7 @@ class _Distillation(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, weight):
+        _refuse_tangents(weight)
         # hooks on saved tensors may give them back with other strides than the forward pass saw
         logits, teacher_logits, teacher_index, stats = ctx.saved_tensors
         d = _distill_block(logits, teacher_logits, teacher_index, ctx.temperature)
