@@ -578,3 +578,36 @@ def test_layers_whose_tensors_are_kept_on_the_host_between_the_passes(dtype):
     with torch.autograd.graph.save_on_cpu():
         h = gated_linear(*leaves)
     check_gated(x, wg, wu, bg, bu, dh, "silu", h.detach(), torch.autograd.grad(h, leaves, dh), dtype)
+
+
+@pytest.mark.parametrize("act", ["tanh", "silu", "gelu"])
+def test_slopes_keep_their_relative_accuracy_in_the_tails(act):
+    """The bias gradient of a layer of one row is act'(z) itself, z = the kept pre-activation.  In units of 2^-24 of the value: tanh' is
+    1 - t^2 up to 0.55 (t^2 <= 0.25: below 2), then 4 e / (1 + e)^2 with e within 3, the reciprocal within 2 and there twice, three products:
+    10.  silu' = s + z e s^2 and gelu' = Phi + z phi are sums of two terms, each of an exponential within 3 and some five factors and
+    products (Phi: a polynomial whose terms add up to 2.5 times its value, ten steps of half a unit: 13): 16 of both terms'
+    magnitudes.  16 are allowed to all; tanh up to where e = exp(-2 |z|) is the smallest normal number."""
+    from volterra_vae_amd.dense_ops import linear_backward
+
+    def slopes(z):
+        z = z[None].to(dev())
+        x, w, dy = torch.zeros(1, 1, device=dev()), torch.zeros(z.shape[1], 1, device=dev()), torch.ones_like(z)
+        return linear_backward(dy, x, w, z, activation=act, need=(False, False, True))[2].double()
+
+    z = torch.cat((torch.linspace(0.0, 3.0, 3001), torch.linspace(3.0, 12.0, 9001), torch.linspace(12.0, 43.0, 3101)))
+    z = torch.cat((z, -z))
+    z = z[z.abs() <= {"tanh": 43.0, "silu": 40.0, "gelu": 12.0}[act]]
+    Z = z.double().to(dev())
+    if act == "tanh":
+        terms = [torch.cosh(Z) ** -2]
+    elif act == "silu":
+        s = torch.sigmoid(Z)
+        terms = [s, Z * s * torch.sigmoid(-Z)]
+    else:
+        terms = [0.5 * torch.erfc(-Z / 2 ** 0.5), Z * torch.exp(-0.5 * Z * Z) / (2 * torch.pi) ** 0.5]
+    err, size = (slopes(z) - sum(terms)).abs(), sum(t.abs() for t in terms)
+    assert bool((err <= 16 * EPS32 * size).all()), float((err / size).max() / EPS32)
+    # far out: 0 on the left, 0 (tanh) or 1 on the right, and a NaN stays one.  silu' is held at its value at -80, which is
+    # s (1 - 80 e s) = -79 exp(-80) = -79 * 1.8049e-35 = -1.426e-33.
+    far = slopes(torch.tensor([-90.0, -1e30, -3e38, -float("inf"), 90.0, 1e30, 3e38, float("inf"), float("nan")])).cpu()
+    assert far[:4].abs().max() < 1.43e-33 and bool((far[4:8] == (0.0 if act == "tanh" else 1.0)).all()) and bool(torch.isnan(far[8]))
