@@ -196,3 +196,33 @@ def test_forward_mode_derivatives_are_refused(monkeypatch):
             y = out(leaf)
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 torch.autograd.grad(y, leaf, fw.make_dual(torch.ones_like(y), torch.ones_like(y)))
+
+
+def test_every_pass_enters_a_traced_graph_as_an_op():
+    """Fake tensors through every pass: shapes and types of the results, and a graph whose nodes are the passes."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def passes(x, w, u, b, t, i, v):
+        h, gu = dense_ops.gated_forward(x, w, u, b, keep=True)
+        y, z = dense_ops.linear_forward(h, w.t().contiguous(), residual=x, activation="tanh", keep=True)
+        loss, dy = dense_ops.topk_distillation_step(y, t, i, v, temperature=2.0)
+        dh, dw, db = dense_ops.linear_backward(dy, h, w.t().contiguous(), z, activation="tanh", need=(True, False, True))
+        assert dw is None
+        grads = dense_ops.gated_backward(dh, x, w, u, gu, need=(True, True, False, True, False))
+        assert grads[2] is None and grads[4] is None
+        plain = torch.ops.v2vae.linear(x, w, b), torch.ops.v2vae.gated_linear(x, w, u), torch.ops.v2vae.topk_distillation(x, t, i)
+        return (y, z, gu, loss, dy, dh, db, grads[0], grads[1], grads[3], *plain)
+
+    for dtype in (torch.float32, torch.bfloat16):
+        with FakeTensorMode():
+            new = lambda *shape, dt=dtype: torch.empty(shape, dtype=dt, device="cuda")  # noqa: E731
+            args = (new(6, 8), new(4, 8), new(4, 8), new(4), new(6, 3), new(6, 3, dt=torch.int64), new(6, dt=torch.float32))
+            out = passes(*args)
+            f32 = torch.float32
+            assert [(tuple(o.shape), o.dtype) for o in out] == [
+                ((6, 8), dtype), ((6, 8), f32), ((2, 6, 4), f32), ((6,), f32), ((6, 8), dtype), ((6, 4), dtype), ((8,), dtype), ((6, 8), dtype),
+                ((4, 8), dtype), ((4,), dtype), ((6, 4), dtype), ((6, 4), dtype), ((6,), f32)]
+            code = make_fx(passes)(*args).code
+        for name in ("gated_forward", "linear_forward", "distillation_step", "linear_backward", "gated_backward", "distillation_forward"):
+            assert f"v2vae.{name}" in code, code

@@ -8,12 +8,14 @@ Two ways to train: the functions named above are differentiable; `linear_forward
 `gated_backward` and `topk_distillation_step` are the same passes with every gradient an explicit result, for training loops
 that run without autograd, and for HIP graphs: these are what to capture (a backward pass of autograd that is captured while an
 eager graph of the same leaves lives ends the process).  Forward-mode derivatives are refused.  `torch.ops.v2vae.linear`, `torch.ops.v2vae.gated_linear` and
-`torch.ops.v2vae.topk_distillation` are the differentiable forms as registered ops.
+`torch.ops.v2vae.topk_distillation` are the differentiable forms as registered ops.  Where a dispatch mode is at work (fake tensors,
+make_fx and what else traces a program), every pass enters the graph as an op with a shape function (`torch.ops.v2vae.linear_forward`,
+`linear_backward`, `gated_forward`, `gated_backward`, `distillation_forward`, `distillation_backward`, `distillation_step`).
 """
 from __future__ import annotations
 
 import functools
-from typing import Optional, Tuple
+from typing import List, Optional, Tuple
 
 import torch
 from torch.autograd import forward_ad
@@ -23,6 +25,7 @@ from ._lib import Dense, Distill, check, lib
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "tanh": 4}
 MAX_TEACHER_ENTRIES = 1024
+_NAMES = list(ACTIVATIONS)
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -59,6 +62,11 @@ def _refuse_tangents(*tensors):
         for t in tensors:
             if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
                 raise NotImplementedError("forward-mode derivatives: these operators have a backward pass only")
+
+
+def _traced():
+    """A dispatch mode is at work: it has to see an op, not the addresses of tensors that it may follow or that have no memory."""
+    return torch._C._len_torch_dispatch_stack() > 0
 
 
 def _row_stride(t):
@@ -154,6 +162,9 @@ def linear_forward(x, weight, bias=None, *, residual=None, activation="none",
         _check_tensor(residual, "residual", 2, like=x)
         if tuple(residual.shape) != (m, n):
             raise ValueError(f"residual: expected {(m, n)}, got {tuple(residual.shape)}")
+    if _traced():
+        y, z = torch.ops.v2vae.linear_forward(x, weight, bias, residual, activation, bool(keep))
+        return y, z if keep and act else None
     d = _dense(x, weight, act, residual=residual)
     y = x.new_empty((m, n))
     z = torch.empty((m, n), dtype=torch.float32, device=x.device) if keep and act else None
@@ -180,6 +191,9 @@ def linear_backward(dy, x, weight, z=None, *, activation="none", need=(True, Tru
 
 def _linear_backward(dy, x, weight, z, act, need):
     _refuse_tangents(dy, x, weight, z)
+    if _traced():
+        grads = torch.ops.v2vae.linear_backward(dy, x, weight, z if act else None, _NAMES[act], [bool(q) for q in need[:3]])
+        return tuple(g if q else None for g, q in zip(grads, need))
     m, k, n = x.shape[0], x.shape[1], weight.shape[0]
     d = _dense(x, weight, act, dy=dy)
     new = lambda wanted, *shape: x.new_empty(shape) if wanted else None  # noqa: E731
@@ -249,6 +263,9 @@ def gated_forward(x, weight_gate, weight_up, bias_gate=None, bias_up=None, *, ac
     if weight_up.shape != weight_gate.shape:
         raise ValueError(f"weight_up: expected {tuple(weight_gate.shape)}, got {tuple(weight_up.shape)}")
     m, n = x.shape[0], weight_gate.shape[0]
+    if _traced():
+        h, gu = torch.ops.v2vae.gated_forward(x, weight_gate, weight_up, bias_gate, bias_up, activation, bool(keep))
+        return h, gu if keep else None
     d = _dense(x, weight_gate, act, w2=weight_up)
     h = x.new_empty((m, n))
     gu = torch.empty((2, m, n), dtype=torch.float32, device=x.device) if keep else None
@@ -275,6 +292,9 @@ def gated_backward(dh, x, weight_gate, weight_up, gu, *, activation="silu", need
 
 def _gated_backward(dh, x, weight_gate, weight_up, gu, act, need):
     _refuse_tangents(dh, x, weight_gate, weight_up, gu)
+    if _traced():
+        grads = torch.ops.v2vae.gated_backward(dh, x, weight_gate, weight_up, gu, _NAMES[act], [bool(q) for q in need[:5]])
+        return tuple(g if q else None for g, q in zip(grads, need))
     m, k, n = x.shape[0], x.shape[1], weight_gate.shape[0]
     d = _dense(x, weight_gate, act, w2=weight_up, dy=dh)
     new = lambda wanted, *shape: x.new_empty(shape) if wanted else None  # noqa: E731
@@ -315,7 +335,7 @@ def gated_linear(x: torch.Tensor, weight_gate: torch.Tensor, weight_up: torch.Te
 
 
 # ------------------------------------------------------------------------------------------------ distillation
-def _distill(logits, teacher_logits, teacher_index, temperature):
+def _check_distill(logits, teacher_logits, teacher_index, temperature):
     _refuse_tangents(logits, teacher_logits)
     _check_tensor(logits, "logits", 2)
     if getattr(teacher_logits, "dtype", None) not in _DTYPES:
@@ -335,10 +355,9 @@ def _distill(logits, teacher_logits, teacher_index, temperature):
                          f"{tuple(teacher_index.shape)}")
     if not 1e-4 <= temperature <= 1e4:
         raise ValueError(f"temperature: 1e-4 ... 1e4 (got {temperature})")
-    return _distill_block(logits, teacher_logits, teacher_index, temperature)
 
 
-def _distill_block(logits, teacher_logits, teacher_index, temperature):
+def _distill(logits, teacher_logits, teacher_index, temperature):
     return Distill(_DTYPES[logits.dtype], _DTYPES[teacher_logits.dtype], 32 if teacher_index.dtype == torch.int32 else 64,
                    teacher_logits.shape[1], logits.shape[0], logits.shape[1], _row_stride(logits), _row_stride(teacher_logits),
                    _row_stride(teacher_index), temperature, 0)
@@ -353,8 +372,11 @@ def _check_weight(weight, logits):
 
 def topk_distillation_step(logits, teacher_logits, teacher_index, row_weight, *, temperature: float = 1.0):
     """(loss [M] float32, grad [M, V]): the losses of `topk_distillation` and d(sum of row_weight * loss) / d logits, one pass."""
-    d = _distill(logits, teacher_logits, teacher_index, temperature)
+    _check_distill(logits, teacher_logits, teacher_index, temperature)
     _check_weight(row_weight, logits)
+    if _traced():
+        return torch.ops.v2vae.distillation_step(logits, teacher_logits, teacher_index, row_weight, temperature)
+    d = _distill(logits, teacher_logits, teacher_index, temperature)
     loss, grad = row_weight.new_empty(row_weight.shape), logits.new_empty(logits.shape)
     _enqueue(lib.v2vae_distill_step, "v2vae_distill_step", logits, d, _p(logits), _p(teacher_logits), _p(teacher_index), _p(row_weight),
              _p(loss), _p(grad))
@@ -364,8 +386,8 @@ def topk_distillation_step(logits, teacher_logits, teacher_index, row_weight, *,
 class _Distillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher_logits, teacher_index, temperature):
-        d = _distill(logits, teacher_logits, teacher_index, temperature)
-        loss, stats = _distill_forward(d, logits, teacher_logits, teacher_index, True)
+        _check_distill(logits, teacher_logits, teacher_index, temperature)
+        loss, stats = _distill_forward(logits, teacher_logits, teacher_index, temperature, True)
         ctx.save_for_backward(logits, teacher_logits, teacher_index, stats)
         ctx.temperature = temperature
         return loss
@@ -375,20 +397,28 @@ class _Distillation(torch.autograd.Function):
     def backward(ctx, weight):
         _refuse_tangents(weight)
         # hooks on saved tensors may give them back with other strides than the forward pass saw
-        logits, teacher_logits, teacher_index, stats = ctx.saved_tensors
-        d = _distill_block(logits, teacher_logits, teacher_index, ctx.temperature)
-        weight, grad = weight.contiguous().resolve_neg(), logits.new_empty(logits.shape)
-        _enqueue(lib.v2vae_distill_bwd, "v2vae_distill_bwd", logits, d, _p(logits), _p(teacher_logits), _p(teacher_index), _p(stats),
-                 _p(weight), _p(grad))
-        return grad, None, None, None
+        return (_distill_backward(weight.contiguous().resolve_neg(), *ctx.saved_tensors, ctx.temperature), None, None, None)
 
 
-def _distill_forward(d, logits, teacher_logits, teacher_index, keep):
+def _distill_forward(logits, teacher_logits, teacher_index, temperature, keep):
+    if _traced():
+        loss, stats = torch.ops.v2vae.distillation_forward(logits, teacher_logits, teacher_index, temperature, keep)
+        return loss, stats if keep else None
     m = logits.shape[0]
+    d = _distill(logits, teacher_logits, teacher_index, temperature)
     loss = torch.empty(m, dtype=torch.float32, device=logits.device)
     stats = loss.new_empty((m, 2)) if keep else None
     _enqueue(lib.v2vae_distill_fwd, "v2vae_distill_fwd", logits, d, _p(logits), _p(teacher_logits), _p(teacher_index), _p(loss), _p(stats))
     return loss, stats
+
+
+def _distill_backward(weight, logits, teacher_logits, teacher_index, stats, temperature):
+    if _traced():
+        return torch.ops.v2vae.distillation_backward(weight, logits, teacher_logits, teacher_index, stats, temperature)
+    d, grad = _distill(logits, teacher_logits, teacher_index, temperature), logits.new_empty(logits.shape)
+    _enqueue(lib.v2vae_distill_bwd, "v2vae_distill_bwd", logits, d, _p(logits), _p(teacher_logits), _p(teacher_index), _p(stats), _p(weight),
+             _p(grad))
+    return grad
 
 
 def topk_distillation(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor, *,
@@ -405,11 +435,101 @@ def topk_distillation(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
         raise ValueError("teacher_logits: the loss is not differentiable in the teacher (pass teacher_logits.detach())")
     if isinstance(logits, torch.Tensor) and _grads_wanted(logits):
         return _Distillation.apply(logits, teacher_logits, teacher_index, temperature)
-    d = _distill(logits, teacher_logits, teacher_index, temperature)
-    return _distill_forward(d, logits, teacher_logits, teacher_index, False)[0]
+    _check_distill(logits, teacher_logits, teacher_index, temperature)
+    return _distill_forward(logits, teacher_logits, teacher_index, temperature, False)[0]
 
 
 # ------------------------------------------------------------------------------------------------ registered ops
+# The passes, for what traces a program.  An op returns tensors only: what a pass leaves out is empty there.
+def _filled(like, *tensors):
+    return tuple(like.new_empty(0) if t is None else t for t in tensors)
+
+
+@torch.library.custom_op("v2vae::linear_forward", mutates_args=(), device_types="cuda")
+def _op_linear_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], residual: Optional[torch.Tensor],
+                       activation: str, keep: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    y, z = linear_forward(x, weight, bias, residual=residual, activation=activation, keep=keep)
+    return _filled(x, y, z)
+
+
+@_op_linear_forward.register_fake
+def _(x, weight, bias, residual, activation, keep):
+    shape = (x.shape[0], weight.shape[0])
+    return _filled(x, x.new_empty(shape), x.new_empty(shape, dtype=torch.float32) if keep and activation != "none" else None)
+
+
+@torch.library.custom_op("v2vae::linear_backward", mutates_args=(), device_types="cuda")
+def _op_linear_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, z: Optional[torch.Tensor], activation: str,
+                        need: List[bool]) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _filled(x, *linear_backward(dy, x, weight, z, activation=activation, need=need))
+
+
+@_op_linear_backward.register_fake
+def _(dy, x, weight, z, activation, need):
+    shapes = (x.shape, weight.shape, weight.shape[:1])
+    return _filled(x, *(x.new_empty(s) if q else None for s, q in zip(shapes, need)))
+
+
+@torch.library.custom_op("v2vae::gated_forward", mutates_args=(), device_types="cuda")
+def _op_gated_forward(x: torch.Tensor, weight_gate: torch.Tensor, weight_up: torch.Tensor, bias_gate: Optional[torch.Tensor],
+                      bias_up: Optional[torch.Tensor], activation: str, keep: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    return _filled(x, *gated_forward(x, weight_gate, weight_up, bias_gate, bias_up, activation=activation, keep=keep))
+
+
+@_op_gated_forward.register_fake
+def _(x, weight_gate, weight_up, bias_gate, bias_up, activation, keep):
+    m, n = x.shape[0], weight_gate.shape[0]
+    return _filled(x, x.new_empty((m, n)), x.new_empty((2, m, n), dtype=torch.float32) if keep else None)
+
+
+@torch.library.custom_op("v2vae::gated_backward", mutates_args=(), device_types="cuda")
+def _op_gated_backward(dh: torch.Tensor, x: torch.Tensor, weight_gate: torch.Tensor, weight_up: torch.Tensor, gu: torch.Tensor, activation: str,
+                       need: List[bool]) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _filled(x, *gated_backward(dh, x, weight_gate, weight_up, gu, activation=activation, need=need))
+
+
+@_op_gated_backward.register_fake
+def _(dh, x, weight_gate, weight_up, gu, activation, need):
+    shapes = (x.shape, weight_gate.shape, weight_up.shape, weight_gate.shape[:1], weight_up.shape[:1])
+    return _filled(x, *(x.new_empty(s) if q else None for s, q in zip(shapes, need)))
+
+
+@torch.library.custom_op("v2vae::distillation_forward", mutates_args=(), device_types="cuda")
+def _op_distillation_forward(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor, temperature: float,
+                             keep: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    loss, stats = _distill_forward(logits, teacher_logits, teacher_index, temperature, keep)
+    return _filled(loss, loss, stats)
+
+
+@_op_distillation_forward.register_fake
+def _(logits, teacher_logits, teacher_index, temperature, keep):
+    m = logits.shape[0]
+    return logits.new_empty(m, dtype=torch.float32), logits.new_empty((m, 2) if keep else 0, dtype=torch.float32)
+
+
+@torch.library.custom_op("v2vae::distillation_backward", mutates_args=(), device_types="cuda")
+def _op_distillation_backward(weight: torch.Tensor, logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor,
+                              stats: torch.Tensor, temperature: float) -> torch.Tensor:
+    return _distill_backward(weight.contiguous(), logits, teacher_logits, teacher_index, stats.contiguous(), temperature)
+
+
+@_op_distillation_backward.register_fake
+def _(weight, logits, teacher_logits, teacher_index, stats, temperature):
+    return logits.new_empty(logits.shape)
+
+
+@torch.library.custom_op("v2vae::distillation_step", mutates_args=(), device_types="cuda")
+def _op_distillation_step(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor, row_weight: torch.Tensor,
+                          temperature: float) -> Tuple[torch.Tensor, torch.Tensor]:
+    return topk_distillation_step(logits, teacher_logits, teacher_index, row_weight, temperature=temperature)
+
+
+@_op_distillation_step.register_fake
+def _(logits, teacher_logits, teacher_index, row_weight, temperature):
+    return row_weight.new_empty(row_weight.shape), logits.new_empty(logits.shape)
+
+
+# The differentiable forms.
 _LIBRARY = torch.library.Library("v2vae", "FRAGMENT")
 _LIBRARY.define("linear(Tensor x, Tensor weight, Tensor? bias=None, *, Tensor? residual=None, str activation='none') -> Tensor")
 _LIBRARY.define("gated_linear(Tensor x, Tensor weight_gate, Tensor weight_up, Tensor? bias_gate=None, Tensor? bias_up=None, *, "
