@@ -226,3 +226,16 @@ def test_every_pass_enters_a_traced_graph_as_an_op():
             code = make_fx(passes)(*args).code
         for name in ("gated_forward", "linear_forward", "distillation_step", "linear_backward", "gated_backward", "distillation_forward"):
             assert f"v2vae.{name}" in code, code
+
+
+def test_a_gradient_whose_rows_lie_far_apart_is_taken_as_a_copy(monkeypatch):
+    """Row strides beyond 2^22 are refused in what a caller lays out; the stride of an incoming gradient is not the caller's doing (the
+    piece of a wide concatenation's gradient, say)."""
+    calls = without_launches(monkeypatch)
+    far = (1 << 22) + 8
+    x, w = torch.zeros(2, 5).requires_grad_(True), torch.zeros(4, 5)
+    for out, name in ((dense_ops.linear(x, w), "v2vae_linear_bwd"), (dense_ops.gated_linear(x, w, w), "v2vae_gated_bwd")):
+        for stride, taken in ((far, 4), (1 << 22, 1 << 22)):
+            dy = torch.zeros(2 * far)[:].as_strided((2, 4), (stride, 1))
+            torch.autograd.grad(out, x, dy, retain_graph=True)
+            assert calls[-1][0] == name and calls[-1][1][0].ld_dy == taken

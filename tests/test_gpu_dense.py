@@ -611,3 +611,18 @@ def test_slopes_keep_their_relative_accuracy_in_the_tails(act):
     # s (1 - 80 e s) = -79 exp(-80) = -79 * 1.8049e-35 = -1.426e-33.
     far = slopes(torch.tensor([-90.0, -1e30, -3e38, -float("inf"), 90.0, 1e30, 3e38, float("inf"), float("nan")])).cpu()
     assert far[:4].abs().max() < 1.43e-33 and bool((far[4:8] == (0.0 if act == "tanh" else 1.0)).all()) and bool(torch.isnan(far[8]))
+
+
+def test_a_layer_beside_a_very_wide_one():
+    """The gradient of a piece of a concatenation more than 2^22 wide arrives with that row stride."""
+    from volterra_vae_amd.dense_ops import gated_linear, linear
+    for dtype in DTYPES:
+        x, w, b, r, dy = linear_case(40, 50, 24, dtype, "silu", True, False, "plain", 6)
+        wide = torch.ones((40, (1 << 22) + 8), dtype=dtype, device=dev())
+        for f in (lambda *a: linear(*a, activation="silu"), lambda x, w, b: gated_linear(x, w, w, b, b)):
+            leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+            beside = torch.cat((f(*leaves), wide), 1)
+            factor = torch.zeros_like(beside)
+            factor[:, :24] = dy
+            got = torch.autograd.grad(beside, leaves, factor)
+            assert all(torch.equal(p, q) for p, q in zip(got, torch.autograd.grad(f(*leaves), leaves, dy)))

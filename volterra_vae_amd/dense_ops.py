@@ -25,6 +25,7 @@ from ._lib import Dense, Distill, check, lib
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "tanh": 4}
 MAX_TEACHER_ENTRIES = 1024
+MAX_ROW_STRIDE = 1 << 22
 _NAMES = list(ACTIVATIONS)
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -142,6 +143,11 @@ def _check_grad(dy, name, x, n):
         raise ValueError(f"{name}: expected {(x.shape[0], n)}, got {tuple(dy.shape)}")
 
 
+def _incoming(dy):
+    """A gradient in a layout that the kernels take: autograd chose the one that it comes in."""
+    return (dy if (dy.shape[1] <= 1 or dy.stride(1) == 1) and dy.stride(0) <= MAX_ROW_STRIDE else dy.contiguous()).resolve_neg()
+
+
 def _check_kept(kept, shape, x):
     _check_tensor(kept, "the kept pre-activations", len(shape), like=x, dtype=torch.float32)
     if tuple(kept.shape) != shape or not kept.is_contiguous():
@@ -219,8 +225,7 @@ class _Linear(torch.autograd.Function):
         need = ctx.needs_input_grad
         dx = dw = db = None
         if any(need[:3]):
-            g = (dy if dy.shape[1] <= 1 or dy.stride(1) == 1 else dy.contiguous()).resolve_neg()
-            dx, dw, db = _linear_backward(g, x, weight, z, ACTIVATIONS[ctx.activation], need)
+            dx, dw, db = _linear_backward(_incoming(dy), x, weight, z, ACTIVATIONS[ctx.activation], need)
         return dx, dw, db, dy if need[3] else None, None
 
 
@@ -316,8 +321,7 @@ class _Gated(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
         x, weight_gate, weight_up, gu = ctx.saved_tensors
-        g = (dh if dh.shape[1] <= 1 or dh.stride(1) == 1 else dh.contiguous()).resolve_neg()
-        return (*_gated_backward(g, x, weight_gate, weight_up, gu, ACTIVATIONS[ctx.activation], ctx.needs_input_grad), None)
+        return (*_gated_backward(_incoming(dh), x, weight_gate, weight_up, gu, ACTIVATIONS[ctx.activation], ctx.needs_input_grad), None)
 
 
 def gated_linear(x: torch.Tensor, weight_gate: torch.Tensor, weight_up: torch.Tensor, bias_gate: Optional[torch.Tensor] = None,
