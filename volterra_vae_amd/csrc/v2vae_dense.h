@@ -87,7 +87,7 @@ __device__ __forceinline__ float normal_cdf(float z, float* gauss) {
 // tanh z: below 0.55 an odd polynomial (least-squares fit of tanh(z) / z - 1 in z^2, 1e-9 at its worst), else from e = exp(-2 |z|), and
 // so its slope 4 e / (1 + e)^2 there, which keeps its relative accuracy down to e = 2^-126 (beyond |z| = 43.6 it is 0), where
 // 1 - tanh(z)^2 has none left from |z| = 9 on
-__device__ __forceinline__ float tanh_of(float z, float* slope) {
+template <bool SLOPE> __device__ __forceinline__ float tanh_of(float z, float* slope) {
     const float u = z * z, y = fabsf(z);
     float p = -0.006282466723832369f;
     p = fmaf(p, u, 0.02107775339065489f);
@@ -95,9 +95,9 @@ __device__ __forceinline__ float tanh_of(float z, float* slope) {
     p = fmaf(p, u, 0.13332601672040642f);
     p = fmaf(p, u, -0.33333318045245297f);
     const float e = exp_with_rest(-2.f * fminf(y, 60.f), 0.f), r = reciprocal(1.f + e);
-    const float large = copysignf((1.f - e) * r, z), t = y < 0.55f ? fmaf(z * u, p, z) : (z != z ? z : large);
-    *slope = y < 0.55f ? fmaf(-t, t, 1.f) : (z != z ? z : 4.f * e * r * r);
-    return t;
+    const float small = fmaf(z * u, p, z), large = copysignf((1.f - e) * r, z);
+    if constexpr (SLOPE) *slope = y < 0.55f ? fmaf(-small, small, 1.f) : (z != z ? z : 4.f * e * r * r);
+    return y < 0.55f ? small : (z != z ? z : large);
 }
 
 // act(z) and act'(z); the kinds are V2VAE_ACT_*.  For |z| beyond 80 the soft activations are their asymptotes to the last bit of
@@ -119,12 +119,8 @@ template <bool SLOPE> __device__ __forceinline__ float act_both(int kind, float 
             if constexpr (SLOPE) *slope = z != z ? z : fmaf(zc, 0.39894228040143268f * gauss, phi);
             return z != z ? z : (z < -80.f ? 0.f : z * phi);
         }
-        case V2VAE_ACT_TANH: {
-            float s;
-            const float t = tanh_of(z, &s);
-            if constexpr (SLOPE) *slope = s;
-            return t;
-        }
+        case V2VAE_ACT_TANH:
+            return tanh_of<SLOPE>(z, slope);
         default:
             if constexpr (SLOPE) *slope = 1.f;
             return z;

@@ -7,10 +7,12 @@ may overlap (windows that slide over one received sequence are a matrix with the
 Two ways to train: the functions named above are differentiable; `linear_forward` / `linear_backward`, `gated_forward` /
 `gated_backward` and `topk_distillation_step` are the same passes with every gradient an explicit result, for training loops
 that run without autograd, and for HIP graphs: these are what to capture (a backward pass of autograd that is captured while an
-eager graph of the same leaves lives ends the process).  Forward-mode derivatives are refused.  `torch.ops.v2vae.linear`, `torch.ops.v2vae.gated_linear` and
-`torch.ops.v2vae.topk_distillation` are the differentiable forms as registered ops.  Where a dispatch mode is at work (fake tensors,
-make_fx and what else traces a program), every pass enters the graph as an op with a shape function (`torch.ops.v2vae.linear_forward`,
-`linear_backward`, `gated_forward`, `gated_backward`, `distillation_forward`, `distillation_backward`, `distillation_step`).
+eager graph of the same leaves lives ends the process).  Forward-mode derivatives are refused.
+
+`torch.ops.v2vae.linear`, `torch.ops.v2vae.gated_linear` and `torch.ops.v2vae.topk_distillation` are the differentiable forms as
+registered ops.  Where a dispatch mode is at work (fake tensors, make_fx and what else traces a program), every pass enters the graph
+as an op with a shape function (`torch.ops.v2vae.linear_forward`, `linear_backward`, `gated_forward`, `gated_backward`,
+`distillation_forward`, `distillation_backward`, `distillation_step`).
 """
 from __future__ import annotations
 
@@ -57,17 +59,15 @@ def _check_tensor(t, name, dim, like=None, dtype=None):
     raise ValueError(f"{name} must have unit stride in its last dimension")
 
 
+# How many dispatch modes are at work.  They have to see an op, not the addresses of tensors that they may follow or that have no memory.
+_modes = torch._C._len_torch_dispatch_stack
+
+
 def _refuse_tangents(*tensors):
-    """The kernels carry no tangents: a dual tensor's derivative would be lost without a word."""
-    if forward_ad._current_level >= 0:
-        for t in tensors:
-            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
-                raise NotImplementedError("forward-mode derivatives: these operators have a backward pass only")
-
-
-def _traced():
-    """A dispatch mode is at work: it has to see an op, not the addresses of tensors that it may follow or that have no memory."""
-    return torch._C._len_torch_dispatch_stack() > 0
+    """Inside a forward-mode level: the kernels carry no tangents, and a dual tensor's derivative would be lost without a word."""
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("forward-mode derivatives: these operators have a backward pass only")
 
 
 def _row_stride(t):
@@ -98,14 +98,14 @@ def _enqueue(fn, name, t, *args):
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_bytes(gated, backward, *description):
+def _workspace_bytes(gated, backward, description):
     f = lib.v2vae_gated_workspace_bytes if gated else lib.v2vae_linear_workspace_bytes
-    return f(Dense(*description), backward)
+    return f(Dense.from_buffer_copy(description), backward)
 
 
 def _workspace(gated, backward, d, x):
     """Scratch memory of one call, from torch's allocator: of the current stream, or of the graph that is being captured."""
-    size = _workspace_bytes(gated, backward, d.dtype, d.activation, d.rows, d.in_, d.out, d.ld_x, d.ld_w, d.ld_w2, d.ld_res, d.ld_dy)
+    size = _workspace_bytes(gated, backward, bytes(d))
     return torch.empty(max(size, 256), dtype=torch.uint8, device=x.device) if size or backward else None
 
 
@@ -160,7 +160,8 @@ def linear_forward(x, weight, bias=None, *, residual=None, activation="none",
     """(y, z) for x [M, K], weight [N, K]: y = activation(x weight^T + bias) + residual, and, if `keep` and there is an
     activation, the float32 pre-activations z [M, N] that `linear_backward` wants (else None)."""
     act = _activation(activation)
-    _refuse_tangents(x, weight, bias, residual)
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(x, weight, bias, residual)
     _check_tensor(x, "x", 2)
     _check_layer(x, weight, "weight", bias, "bias")
     m, n = x.shape[0], weight.shape[0]
@@ -168,7 +169,7 @@ def linear_forward(x, weight, bias=None, *, residual=None, activation="none",
         _check_tensor(residual, "residual", 2, like=x)
         if tuple(residual.shape) != (m, n):
             raise ValueError(f"residual: expected {(m, n)}, got {tuple(residual.shape)}")
-    if _traced():
+    if _modes():
         y, z = torch.ops.v2vae.linear_forward(x, weight, bias, residual, activation, bool(keep))
         return y, z if keep and act else None
     d = _dense(x, weight, act, residual=residual)
@@ -196,8 +197,9 @@ def linear_backward(dy, x, weight, z=None, *, activation="none", need=(True, Tru
 
 
 def _linear_backward(dy, x, weight, z, act, need):
-    _refuse_tangents(dy, x, weight, z)
-    if _traced():
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(dy, x, weight, z)
+    if _modes():
         grads = torch.ops.v2vae.linear_backward(dy, x, weight, z if act else None, _NAMES[act], [bool(q) for q in need[:3]])
         return tuple(g if q else None for g, q in zip(grads, need))
     m, k, n = x.shape[0], x.shape[1], weight.shape[0]
@@ -261,14 +263,15 @@ def gated_forward(x, weight_gate, weight_up, bias_gate=None, bias_up=None, *, ac
     """(h, gu) for x [M, K], weights [N, K]: h = activation(x weight_gate^T + bias_gate) * (x weight_up^T + bias_up), and, if
     `keep`, the float32 pre-activations gu [2, M, N] (gate, up) that `gated_backward` wants (else None)."""
     act = _activation(activation)
-    _refuse_tangents(x, weight_gate, weight_up, bias_gate, bias_up)
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(x, weight_gate, weight_up, bias_gate, bias_up)
     _check_tensor(x, "x", 2)
     _check_layer(x, weight_gate, "weight_gate", bias_gate, "bias_gate")
     _check_layer(x, weight_up, "weight_up", bias_up, "bias_up")
     if weight_up.shape != weight_gate.shape:
         raise ValueError(f"weight_up: expected {tuple(weight_gate.shape)}, got {tuple(weight_up.shape)}")
     m, n = x.shape[0], weight_gate.shape[0]
-    if _traced():
+    if _modes():
         h, gu = torch.ops.v2vae.gated_forward(x, weight_gate, weight_up, bias_gate, bias_up, activation, bool(keep))
         return h, gu if keep else None
     d = _dense(x, weight_gate, act, w2=weight_up)
@@ -296,8 +299,9 @@ def gated_backward(dh, x, weight_gate, weight_up, gu, *, activation="silu", need
 
 
 def _gated_backward(dh, x, weight_gate, weight_up, gu, act, need):
-    _refuse_tangents(dh, x, weight_gate, weight_up, gu)
-    if _traced():
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(dh, x, weight_gate, weight_up, gu)
+    if _modes():
         grads = torch.ops.v2vae.gated_backward(dh, x, weight_gate, weight_up, gu, _NAMES[act], [bool(q) for q in need[:5]])
         return tuple(g if q else None for g, q in zip(grads, need))
     m, k, n = x.shape[0], x.shape[1], weight_gate.shape[0]
@@ -340,7 +344,8 @@ def gated_linear(x: torch.Tensor, weight_gate: torch.Tensor, weight_up: torch.Te
 
 # ------------------------------------------------------------------------------------------------ distillation
 def _check_distill(logits, teacher_logits, teacher_index, temperature):
-    _refuse_tangents(logits, teacher_logits)
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(logits, teacher_logits)
     _check_tensor(logits, "logits", 2)
     if getattr(teacher_logits, "dtype", None) not in _DTYPES:
         raise NotImplementedError("teacher_logits: a float32, bfloat16 or float16 tensor")
@@ -368,7 +373,8 @@ def _distill(logits, teacher_logits, teacher_index, temperature):
 
 
 def _check_weight(weight, logits):
-    _refuse_tangents(weight)
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(weight)
     _check_tensor(weight, "row_weight", 1, like=logits, dtype=torch.float32)
     if weight.shape[0] != logits.shape[0]:
         raise ValueError(f"row_weight: expected {logits.shape[0]} values, got {weight.shape[0]}")
@@ -378,7 +384,7 @@ def topk_distillation_step(logits, teacher_logits, teacher_index, row_weight, *,
     """(loss [M] float32, grad [M, V]): the losses of `topk_distillation` and d(sum of row_weight * loss) / d logits, one pass."""
     _check_distill(logits, teacher_logits, teacher_index, temperature)
     _check_weight(row_weight, logits)
-    if _traced():
+    if _modes():
         return torch.ops.v2vae.distillation_step(logits, teacher_logits, teacher_index, row_weight, temperature)
     d = _distill(logits, teacher_logits, teacher_index, temperature)
     loss, grad = row_weight.new_empty(row_weight.shape), logits.new_empty(logits.shape)
@@ -391,7 +397,7 @@ class _Distillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher_logits, teacher_index, temperature):
         _check_distill(logits, teacher_logits, teacher_index, temperature)
-        loss, stats = _distill_forward(logits, teacher_logits, teacher_index, temperature, True)
+        ctx.d, loss, stats = _distill_forward(logits, teacher_logits, teacher_index, temperature, True)
         ctx.save_for_backward(logits, teacher_logits, teacher_index, stats)
         ctx.temperature = temperature
         return loss
@@ -399,27 +405,36 @@ class _Distillation(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, weight):
-        _refuse_tangents(weight)
+        if forward_ad._current_level >= 0:
+            _refuse_tangents(weight)
+        logits, teacher_logits, teacher_index, stats = ctx.saved_tensors
         # hooks on saved tensors may give them back with other strides than the forward pass saw
-        return (_distill_backward(weight.contiguous().resolve_neg(), *ctx.saved_tensors, ctx.temperature), None, None, None)
+        d = ctx.d
+        if d is not None and (logits.stride(0) != d.ld_logits or teacher_logits.stride(0) != d.ld_teacher or teacher_index.stride(0) != d.ld_index):
+            d = None
+        weight = weight.contiguous().resolve_neg()
+        return _distill_backward(weight, logits, teacher_logits, teacher_index, stats, ctx.temperature, d), None, None, None
 
 
 def _distill_forward(logits, teacher_logits, teacher_index, temperature, keep):
-    if _traced():
+    """(argument block, loss, statistics), the last two as asked for; no block in a trace."""
+    if _modes():
         loss, stats = torch.ops.v2vae.distillation_forward(logits, teacher_logits, teacher_index, temperature, keep)
-        return loss, stats if keep else None
+        return None, loss, stats if keep else None
     m = logits.shape[0]
     d = _distill(logits, teacher_logits, teacher_index, temperature)
     loss = torch.empty(m, dtype=torch.float32, device=logits.device)
     stats = loss.new_empty((m, 2)) if keep else None
     _enqueue(lib.v2vae_distill_fwd, "v2vae_distill_fwd", logits, d, _p(logits), _p(teacher_logits), _p(teacher_index), _p(loss), _p(stats))
-    return loss, stats
+    return d, loss, stats
 
 
-def _distill_backward(weight, logits, teacher_logits, teacher_index, stats, temperature):
-    if _traced():
+def _distill_backward(weight, logits, teacher_logits, teacher_index, stats, temperature, d=None):
+    if _modes():
         return torch.ops.v2vae.distillation_backward(weight, logits, teacher_logits, teacher_index, stats, temperature)
-    d, grad = _distill(logits, teacher_logits, teacher_index, temperature), logits.new_empty(logits.shape)
+    if d is None:
+        d = _distill(logits, teacher_logits, teacher_index, temperature)
+    grad = logits.new_empty(logits.shape)
     _enqueue(lib.v2vae_distill_bwd, "v2vae_distill_bwd", logits, d, _p(logits), _p(teacher_logits), _p(teacher_index), _p(stats), _p(weight),
              _p(grad))
     return grad
@@ -440,7 +455,7 @@ def topk_distillation(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
     if isinstance(logits, torch.Tensor) and _grads_wanted(logits):
         return _Distillation.apply(logits, teacher_logits, teacher_index, temperature)
     _check_distill(logits, teacher_logits, teacher_index, temperature)
-    return _distill_forward(logits, teacher_logits, teacher_index, temperature, False)[0]
+    return _distill_forward(logits, teacher_logits, teacher_index, temperature, False)[1]
 
 
 # ------------------------------------------------------------------------------------------------ registered ops
@@ -501,7 +516,8 @@ def _(dh, x, weight_gate, weight_up, gu, activation, need):
 @torch.library.custom_op("v2vae::distillation_forward", mutates_args=(), device_types="cuda")
 def _op_distillation_forward(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor, temperature: float,
                              keep: bool) -> Tuple[torch.Tensor, torch.Tensor]:
-    loss, stats = _distill_forward(logits, teacher_logits, teacher_index, temperature, keep)
+    _check_distill(logits, teacher_logits, teacher_index, temperature)
+    _, loss, stats = _distill_forward(logits, teacher_logits, teacher_index, temperature, keep)
     return _filled(loss, loss, stats)
 
 
@@ -514,7 +530,9 @@ def _(logits, teacher_logits, teacher_index, temperature, keep):
 @torch.library.custom_op("v2vae::distillation_backward", mutates_args=(), device_types="cuda")
 def _op_distillation_backward(weight: torch.Tensor, logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor,
                               stats: torch.Tensor, temperature: float) -> torch.Tensor:
-    return _distill_backward(weight.contiguous(), logits, teacher_logits, teacher_index, stats.contiguous(), temperature)
+    _check_distill(logits, teacher_logits, teacher_index, temperature)
+    _check_weight(weight, logits)
+    return _distill_backward(weight, logits, teacher_logits, teacher_index, stats.contiguous(), temperature)
 
 
 @_op_distillation_backward.register_fake
