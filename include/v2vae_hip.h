@@ -375,7 +375,8 @@ int v2vae_linear_fwd(const v2vae_dense* d, const void* x, const void* w, const v
 
 /* Gradients given dy [rows][out]: with dz = dy act'(z), dx [rows][in] = dz w, dw [out][in] = dz^T x, dbias [out] = column sums
  * of dz (the residual's gradient is dy itself).  Each output may be NULL; z may be NULL without an activation.  dz is rounded to
- * the element type once before the two products (dbias is summed before that).  ws: v2vae_linear_workspace_bytes(d, 1). */
+ * the element type once before the two products (dbias is summed before that); in float16 a dz beyond 65504 becomes infinite there,
+ * whatever the size of the sums it enters.  ws: v2vae_linear_workspace_bytes(d, 1), whichever outputs are wanted. */
 int v2vae_linear_bwd(const v2vae_dense* d, const void* x, const void* w, const float* z, const void* dy, void* dx, void* dw,
                      void* dbias, void* ws, void* stream);
 size_t v2vae_linear_workspace_bytes(const v2vae_dense* d, int backward); /* 0 also for an invalid description */
@@ -386,7 +387,8 @@ int v2vae_gated_fwd(const v2vae_dense* d, const void* x, const void* wg, const v
                     void* h, float* gu, void* ws, void* stream);
 
 /* Gradients given dh [rows][out] (row stride ld_dy): dg = dh u act'(g), du = dh act(g); dx = dg wg + du wu, dwg = dg^T x,
- * dwu = du^T x, dbg / dbu the column sums.  Each output may be NULL.  ws: v2vae_gated_workspace_bytes(d, 1). */
+ * dwu = du^T x, dbg / dbu the column sums.  dg and du are rounded as dz above.  Each output may be NULL, and the others are the same to
+ * the bit.  ws: v2vae_gated_workspace_bytes(d, 1), whichever outputs are wanted. */
 int v2vae_gated_bwd(const v2vae_dense* d, const void* x, const void* wg, const void* wu, const float* gu, const void* dh,
                     void* dx, void* dwg, void* dwu, void* dbg, void* dbu, void* ws, void* stream);
 size_t v2vae_gated_workspace_bytes(const v2vae_dense* d, int backward);
@@ -395,7 +397,8 @@ size_t v2vae_gated_workspace_bytes(const v2vae_dense* d, int backward);
  * with index < 0 or t = -inf is absent; a class named twice counts twice.  With p = softmax over the present entries of t / T and
  * log q = log softmax(z / T):  loss = T^2 sum_j p_j (log p_j - log q[index_j]);  d loss / d z = T (q - sum_{index_j = v} p_j).
  * A row without present entries has loss 0 and gradient 0.  A student logit of -inf has q = 0 (loss +inf if its p is not 0).
- * An index >= vocab makes the row's loss and gradient NaN (nothing is read there). */
+ * An index >= vocab makes the row's loss and gradient NaN (nothing is read there).  The loss is computed in float: off by up to about
+ * T^2 2^-20 (2 + |log q|). */
 typedef struct v2vae_distill {
     int32_t dtype;         /* of the student's logits and their gradient: V2VAE_F32, V2VAE_BF16, V2VAE_F16 */
     int32_t teacher_dtype; /* of the teacher's logits */

@@ -7,10 +7,10 @@ namespace v2vae {
 
 // ---- dz = dy act'(z) and its column sums -------------------------------------------------------------------------------------
 // One pass over dy and the float pre-activations; memory bound.  A block owns a strip of columns and every so many rows (a chunk): all
-// blocks move through memory together (65536 x 256 float 38 us, 43 with rows that follow one another; gated 173475 x 1320 1180 and
+// blocks move through memory together (65536 x 256 float 37 us, 43 with rows that follow one another; gated 173475 x 1320 1180 and
 // 1300).  It sums its columns in float in a fixed order (per thread along the rows, then over the block's row threads) and leaves one
 // partial per chunk; k_column_join adds the chunks (4 ... 5 us).  dz is rounded to T here, once, after its contribution to the column
-// sum.  Float 65536 x 256: 5.3 TB/s; bf16 gated 4096 x 5632: 56 us (5.7 TB/s).
+// sum.  Float 65536 x 256: 5.5 TB/s; bf16 gated 4096 x 5632: 61 us (5.3 TB/s).
 struct SlopeArgs {
     const void* dy;
     int64_t ld_dy;

@@ -16,9 +16,9 @@
 // Three tiles (the rule is cut_product's): 256 x 256 on eight waves of 128 x 64, which asks memory for half as much as 128 x 128 on
 // four waves of 64 x 64; 128 x 64 for outputs of one column of tiles (60992 x 88 -> 16: 10 us, 28 with 256 x 256).  The loads of a
 // step have one step of products to arrive in, so the larger tile, with twice the products a step, waits less: bound by that
-// latency and by the clock, which the chip's power holds at 1.9 GHz under it; the matrix unit is busy 48 ... 61 % of the cycles.
-// bf16, 8192 x 4096 -> 4096: forward with residual 266 us (1030 TF), dx 248 (1110 TF), dw 241 (1140 TF); 4999 x 2048 -> 2 x 5632 gated
-// forward 247 (934 TF).  Measured and not kept: 256 x 256 on four waves of 128 x 128 (training pass 841 us against 750), loads spread
+// latency and by the clock, which the chip's power holds at 1.9 ... 2.0 GHz under it; the matrix unit is busy 40 ... 56 % of the cycles.
+// bf16, 8192 x 4096 -> 4096: forward with residual 252 us (1090 TF), dx 234 (1170 TF), dw 220 (1250 TF); 4999 x 2048 -> 2 x 5632 gated
+// forward 241 (957 TF).  Measured and not kept: 256 x 256 on four waves of 128 x 128 (training pass 841 us against 750), loads spread
 // over the step's products (gated forward 272 against 253), raised wave priority around the products (no change).
 #ifndef V2VAE_DENSE_DIRECT_H
 #define V2VAE_DENSE_DIRECT_H

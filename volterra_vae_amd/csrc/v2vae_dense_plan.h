@@ -16,7 +16,7 @@ enum { TILE_128, TILE_64, TILE_256, TILE_96, TILE_160 };  // float32: columns of
 // few rows (v2vae_dense_rows.hip); beyond, the tiled products read the weights as fast
 inline int64_t few_rows(int dtype) { return dtype == V2VAE_F32 ? 32 : 16; }
 // Parts of the contraction there.  Float on few, long weight rows: the contraction in parts, to a workgroup a compute unit (9 x 8165 -> 2 x 504: 25 us in one part,
-// 18 in four and their join).  16-bit rows, of half the bytes, end before a second launch would pay.
+// 16.7 in four and their join, kernels of 11.4 and 4.8).  16-bit rows, of half the bytes, end before a second launch would pay.
 inline int rows_splits(int dtype, int64_t in, int64_t out, bool gated) {
     if (dtype != V2VAE_F32) return 1;
     const int64_t groups = gated ? (out + 7) / 8 : (out + 15) / 16;

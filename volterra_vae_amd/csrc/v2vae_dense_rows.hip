@@ -7,8 +7,9 @@
 // memory (16 bytes a lane, any alignment); float operands are split into three bf16 pieces in registers (six products).  The
 // waves' sums are joined through LDS in a fixed order.
 //
-// Bound by the weights' bytes and the time until the first of them arrive: bf16 one row of 4096 x 4096 7.5 ... 9 us (4.5 TB/s at best), f16 five rows
-// of 2048 -> 2 x 5632 12.8 us (3.6 TB/s), float one row of 8192 x 8192 64 us (4.2 TB/s; a large copy: 5.2).  Measured and not kept: lanes
+// Bound by the weights' bytes and the time until the first of them arrive: bf16 one row of 4096 x 4096 8.6 ... 9.5 us (3.9 TB/s at best; two turns
+// a wave), f16 five rows of 2048 -> 2 x 5632 12.1 ... 13.1 us (3.5 TB/s; one turn a wave, so nothing is asked for ahead), float one row of
+// 8192 x 8192 57 us (4.7 TB/s; a large copy: 5.2).  Measured and not kept: lanes
 // in pairs of 128 bytes (no change), turns of 256 elements (spills), multiply-adds instead of the matrix unit for one row (5.4 us at
 // 4096 x 4096, but a call takes the host 9 either way).
 #include "v2vae_dense_gemm.h"

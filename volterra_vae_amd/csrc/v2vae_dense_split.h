@@ -15,10 +15,11 @@
 //  * B_ROWS, B_COLUMNS: otherwise the workgroup splits its tile on the way into LDS (contraction or rows contiguous in memory).
 //    Both operands then come from far away and run two steps ahead, in two register sets each; the last two steps are written out
 //    so that the loop's loads are unconditional and the compiler can count what is in flight.
-// Bound by issue: splitting A (44 vector instructions a step and 32 x 32 block of it) and the matrix instructions share a SIMD's
-// cycles, which is why planes pay and why wider tiles do, up to the registers: 32768 x 256 -> 2 x 512 gated forward 120 us (143 TF, or
-// 860 TF of bf16 products; 39 us of it are its bytes), its dx 99, dw 113; 65536 x 256 -> 130 39 us; 262144 x 50 -> 64 38 us, of which
-// 23 are its bytes.  Measured and not kept: blocks of zeros at the edge skipped by a branch (training pass 420 us against 405), planes
+// Bound by issue and latency: splitting A (44 vector instructions a step and 32 x 32 block of it) and the matrix instructions share a
+// SIMD's cycles, which is why planes pay and why wider tiles do, up to the registers: 32768 x 256 -> 2 x 512 gated forward 121 us (142 TF,
+// or 850 TF of bf16 products; 39 us of it are its bytes; a SIMD issues vector instructions for 41 us and is busy with matrix ones for 43),
+// its dx 95, dw 107; 65536 x 256 -> 130 38 us.  Contractions of a step or two wait more than they issue: 262144 x 50 -> 64 37 us, of which
+// 23 are its bytes, 22 vector and 5 matrix instructions, because a workgroup's epilogue has no load in flight.  Measured and not kept: blocks of zeros at the edge skipped by a branch (training pass 420 us against 405), planes
 // through registers two steps ahead (fewer waves, slower).
 // One scalar base and 32-bit lane offsets per load: strides are at most 2^22 elements.
 // Rows beyond the matrix repeat its last one (their products are not stored); contraction ends take zeros, element by element.

@@ -7,8 +7,9 @@
 // sparse terms are patched over the dense gradient afterwards by the threads that hold the entries; a class that a row names
 // twice is patched by the first of its entries with the sum, so no two threads write one address and no atomics are needed.
 //
-// Float 262144 x 64, 8 entries: loss 26 us (3.2 TB/s), gradient 36 (4.2 TB/s); bf16 4096 x 32000, 64 entries, loss and gradient 123 us
-// (4.3 TB/s; a large copy: 5.2); f16 33 x 65521 loss 7.7 us, the time of one row's loads and reductions.  Measured and not kept: 256
+// Float 262144 x 64, 8 entries: loss 26 us (3.2 TB/s), gradient 35 (4.4 TB/s), both in one pass 38 ... 41: short rows are bound by issue, the
+// vector instructions take a SIMD 24, 29 and 36 us of them.  bf16 4096 x 32000, 64 entries, loss and gradient 125 us (4.2 TB/s; a large
+// copy: 5.2); f16 33 x 65521 loss 7.8 us, the time of one row's loads and reductions.  Measured and not kept: 256
 // threads of sixteen pieces instead of 512 of eight (no change).
 #include <math.h>
 

@@ -244,7 +244,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     """activation(x weight^T + bias) + residual for x [..., K], weight [N, K], bias [N], residual [..., N], in one kernel.
 
     activation: none, relu, silu, gelu (erf form) or tanh.  Differentiable in every tensor.  Sums are float32; the backward pass
-    works from float32 pre-activations and rounds dy * activation' to the tensors' type once before the two products."""
+    works from float32 pre-activations and rounds dy * activation' to the tensors' type once before the two products (float16: beyond
+    65504 it becomes infinite there, however small the sums it enters)."""
     if not isinstance(x, torch.Tensor) or x.dim() < 1:
         raise ValueError("x must be a tensor [..., K]")
     if residual is not None and tuple(residual.shape[:-1]) != tuple(x.shape[:-1]):
@@ -331,7 +332,8 @@ class _Gated(torch.autograd.Function):
 def gated_linear(x: torch.Tensor, weight_gate: torch.Tensor, weight_up: torch.Tensor, bias_gate: Optional[torch.Tensor] = None,
                  bias_up: Optional[torch.Tensor] = None, *, activation: str = "silu") -> torch.Tensor:
     """Gated feed-forward block: activation(x weight_gate^T + bias_gate) * (x weight_up^T + bias_up) for x [..., K], weights
-    [N, K], both projections, the activation and the product in one kernel.  Differentiable in every tensor."""
+    [N, K], both projections, the activation and the product in one kernel.  Differentiable in every tensor; the gradients of both
+    pre-activations are rounded to the tensors' type as in `linear`."""
     if not isinstance(x, torch.Tensor) or x.dim() < 1:
         raise ValueError("x must be a tensor [..., K]")
     flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
@@ -449,7 +451,8 @@ def topk_distillation(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
 
     An entry with index < 0 or a teacher logit of -inf is absent; a row without present entries has loss and gradient 0; a class
     that a row names twice counts twice.  An index >= V makes the row NaN.  Differentiable in `logits`; the teacher is not.  Rows
-    of the three matrices may lie any distance apart, but may not overlap."""
+    of the three matrices may lie any distance apart, but may not overlap.  Computed in float32, the loss is off by up to about
+    T^2 2^-20 (2 + |log q|)."""
     if isinstance(teacher_logits, torch.Tensor) and teacher_logits.requires_grad and torch.is_grad_enabled():
         raise ValueError("teacher_logits: the loss is not differentiable in the teacher (pass teacher_logits.detach())")
     if isinstance(logits, torch.Tensor) and _grads_wanted(logits):
