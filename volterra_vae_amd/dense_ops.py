@@ -1,7 +1,7 @@
 """Layers and loss of a network equaliser: `linear`, `gated_linear` and `topk_distillation` over the HIP kernels.
 
 Tensors in, kernels enqueued on the current HIP stream of the tensors' device; float32, bfloat16 or float16, one type for all
-tensors of a call, on a GPU only.  Matrices need unit stride inside a row; rows may lie any distance apart, and rows of inputs
+tensors of a call, on a GPU only.  Matrices need unit stride inside a row; rows may lie apart (up to 2^22 elements), and rows of inputs
 may overlap (windows that slide over one received sequence are a matrix with the row stride `samples_per_symbol`).
 
 Two ways to train: the functions named above are differentiable; `linear_forward` / `linear_backward`, `gated_forward` /
